@@ -253,6 +253,63 @@ int32_t mpq_nvfp4_quantize_swiglu(mpq_context* ctx, const void* gate_up_dev, int
 int32_t mpq_nvfp4_dequantize(mpq_context* ctx, int64_t R, int64_t K, const uint8_t* codes_dev,
                              const uint8_t* sf_dev, float tensor_scale, float* out_dev, void* stream);
 
+/* ---- between the projections of a decoder layer ------------------------------ */
+/* No counterpart in the reference.  Rows are packed: the new tokens of request i of n are rows starts[i] .. starts[i+1]-1 of
+ * the activations (starts: n+1 int32 on the device, ascending from 0); rows behind starts[n] belong to nobody and are
+ * left as they are.  bf16 arrays are uint16_t bits.  All pointers 16-byte aligned unless a scalar or int array.  The lengths are read
+ * on the device: a captured call follows them.  These calls leave the current device as it was. */
+
+/* Norms around a block and the residual sum between them, per row of H columns (H a multiple of 8, at most 32768):
+ *   t = x;  t = t / sqrt(mean(t^2) + eps) * post_weight   if post_weight is given (the norm behind the block)
+ *   residual_out = residual + alpha * gate * t            residual NULL: 0; gate NULL: 1
+ *   y = residual_out / sqrt(mean(residual_out^2) + eps) * weight        weight NULL: 1
+ * x [M][H] fp32 or bf16; residuals fp32 [M][H], residual_out may be residual or NULL; weights fp32 [H]; gate fp32 [M][gate_stride]
+ * (a multiple of 4, at least H), or one row for all with gate_stride 0; y fp32 or bf16 [M][H], or NULL.  y must not overlap an input. */
+int32_t mpq_residual_norm(mpq_context* ctx, const void* x_dev, int32_t x_is_bf16, int64_t M, int64_t H, const float* residual_dev,
+                          float* residual_out_dev, const float* post_weight_dev, const float* gate_dev, int64_t gate_stride, float alpha,
+                          const float* weight_dev, float eps, void* y_dev, int32_t y_is_bf16, void* stream);
+
+/* A paged cache is two bf16 arrays [pages][kv_heads][page_size][head_dim], page_size a power of two from 16 to 256; the slot of a
+ * token is page * page_size + place.  Request i has its pages in row i of block_table [n][max_blocks]; pages that nobody
+ * has are the first free_count[0] entries of free [pages], a stack.
+ *
+ * mpq_kv_plan makes a step of n requests (at most 8192) from their lengths, on the device.  lens[i] tokens are in the cache;
+ * new_lens[i] >= 0 follow, or new_lens[i] < 0: the request has ended, its pages go back on the stack, in order, and its row is free
+ * for another (lens_out 0).  Then pages are taken from the stack's top in the order of the requests and written into the table.
+ *   starts [n+1]       first row of each request's new tokens
+ *   positions, slots   [tokens]: place in its request, and slot, of every new token; 0 and -1 behind the last one
+ *   lens_out, free_count_out   the lengths and the count afterwards; may be lens and free_count
+ *   missing [1]        0, or why NO request grew (ended ones are returned all the same; starts are 0, slots -1): the number of
+ *                      pages that are missing; -1: a request would not fit in max_blocks; -2: more new tokens than `tokens`. */
+int32_t mpq_kv_plan(mpq_context* ctx, int64_t n, const int32_t* new_lens_dev, const int32_t* lens_dev, int32_t* lens_out_dev, int32_t* block_table_dev,
+                    int64_t max_blocks, int32_t* free_dev, int64_t pages, const int32_t* free_count_dev, int32_t* free_count_out_dev, int32_t page_size,
+                    int64_t tokens, int32_t* starts_dev, int32_t* positions_dev, int64_t* slots_dev, int32_t* missing_dev, void* stream);
+/* Rows of a QKV projection [tokens][q heads | k heads | v heads][head_dim] (fp32 or bf16, row_stride elements apart, a multiple of 8):
+ * the first rot_dim elements of every q and k head (a multiple of 16, 0: none) are turned by pairs, (i, i + rot_dim/2) or, interleaved,
+ * (2i, 2i+1), by the angle positions[t] * frequencies[i] (fp64 [rot_dim/2]); everything is rounded to bf16 once.  q rows go to
+ * q [tokens][q_heads][head_dim]; k and v rows to k, v [tokens][kv_heads][head_dim] unless NULL, and to the cache at slots[t] unless slots is NULL.
+ * A row with slots[t] < 0 is skipped altogether; a slot behind the cache writes nothing there.  No slot may come twice.
+ * head_dim a multiple of 16, at most 256. */
+int32_t mpq_kv_append(mpq_context* ctx, const void* qkv_dev, int32_t x_is_bf16, int64_t row_stride, int64_t tokens, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                      const int32_t* positions_dev, const double* frequencies_dev, int32_t rot_dim, int32_t interleaved, uint16_t* q_dev, uint16_t* k_dev, uint16_t* v_dev,
+                      const int64_t* slots_dev, uint16_t* k_cache_dev, uint16_t* v_cache_dev, int64_t pages, int32_t page_size, void* stream);
+/* out[t][h] = softmax(scale * q[t][h] . k) . v over the keys that the token sees: with lens[i] tokens in request i's pages, the last ones of
+ * them its new tokens (their k and v are in the cache already), new token j sees the first lens[i] - new + j + 1.  A row without keys is 0.
+ * q bf16, rows of q_heads * head_dim (64 or 128) q_row_stride elements apart (a multiple of 8); query head h reads head
+ * h / (q_heads / kv_heads).  out [tokens][q_heads][head_dim], bf16 or fp32; must not overlap an input.  max_new: the most new tokens of a request, as far as the caller knows
+ * (0: not known); it chooses the kernel, not the result.  An entry of the table outside the cache reads as zeros; what lies behind
+ * lens[i] in the last page is not used, whatever it holds.  k and v of the new tokens are read by rows that do not see them:
+ * they must be finite.  Sums are fp32, the weights of v are rounded to bf16. */
+int32_t mpq_paged_attention(mpq_context* ctx, const uint16_t* q_dev, int64_t q_row_stride, int64_t tokens, int32_t q_heads, const uint16_t* k_cache_dev,
+                            const uint16_t* v_cache_dev, int64_t pages, int32_t page_size, int32_t kv_heads, int32_t head_dim, int64_t n, const int32_t* starts_dev,
+                            const int32_t* lens_dev, const int32_t* block_table_dev, int64_t max_blocks, int64_t max_new, float scale, void* out_dev, int32_t out_is_f32,
+                            void* stream);
+/* The same over whole prompts: keys and values are rows beside the queries, token j of a prompt sees its tokens 0..j.  Other prompts'
+ * rows are not used, whatever they hold. */
+int32_t mpq_prompt_attention(mpq_context* ctx, const uint16_t* q_dev, int64_t q_row_stride, const uint16_t* k_dev, int64_t k_row_stride, const uint16_t* v_dev,
+                             int64_t v_row_stride, int64_t tokens, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int64_t n, const int32_t* starts_dev, float scale,
+                             void* out_dev, int32_t out_is_f32, void* stream);
+
 /* ---- weight container ------------------------------------------------------- */
 /* Files of two kinds, one 128-byte versioned header + payload + FNV-1a checksum each:
  *   MPQ_FILE_CANONICAL  the interchange arrays (Q4: codes + fp16 scale bits; NVFP4: codes + e4m3 scales +

@@ -68,6 +68,11 @@ SIGNATURES = {
     "mpq_nvfp4_quantize_swiglu": (_i32, [_vp, _vp, _i32, _i64, _i64, _f32, _vp, _vp, _vp]),
     "mpq_swiglu": (_i32, [_vp, _vp, _i64, _i64, _vp, _vp]),
     "mpq_q4_linear_forward_swiglu": (_i32, [_vp, _vp, _vp, _i64, _vp, _vp]),
+    "mpq_residual_norm": (_i32, [_vp, _vp, _i32, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _f32, _vp, _f32, _vp, _i32, _vp]),
+    "mpq_kv_plan": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _i32, _i64, _vp, _vp, _vp, _vp, _vp]),
+    "mpq_kv_append": (_i32, [_vp, _vp, _i32, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _vp]),
+    "mpq_paged_attention": (_i32, [_vp, _vp, _i64, _i64, _i32, _vp, _vp, _i64, _i32, _i32, _i32, _i64, _vp, _vp, _vp, _i64, _i64, _f32, _vp, _i32, _vp]),
+    "mpq_prompt_attention": (_i32, [_vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _i32, _i32, _i64, _vp, _f32, _vp, _i32, _vp]),
     "mpq_file_info": (_i32, [C.c_char_p, C.POINTER(FileInfo)]),
     "mpq_canonical_save": (_i32, [C.c_char_p, _i32, _i64, _i64, _vp, _vp, _f32]),
     "mpq_canonical_load": (_i32, [C.c_char_p, _vp, _i64, _vp, _i64, C.POINTER(_f32)]),

@@ -100,6 +100,11 @@ pub struct LibMpq {
     pub mpq_nvfp4_quantize_swiglu: unsafe extern "C" fn(*mut mpq_context, *const c_void, i32, i64, i64, f32, *mut u8, *mut u8, *mut c_void) -> i32,
     pub mpq_swiglu: unsafe extern "C" fn(*mut mpq_context, *const f32, i64, i64, *mut f32, *mut c_void) -> i32,
     pub mpq_q4_linear_forward_swiglu: unsafe extern "C" fn(*mut mpq_context, *const mpq_weight, *const f32, i64, *mut f32, *mut c_void) -> i32,
+    pub mpq_residual_norm: unsafe extern "C" fn(*mut mpq_context, *const c_void, i32, i64, i64, *const f32, *mut f32, *const f32, *const f32, i64, f32, *const f32, f32, *mut c_void, i32, *mut c_void) -> i32,
+    pub mpq_kv_plan: unsafe extern "C" fn(*mut mpq_context, i64, *const i32, *const i32, *mut i32, *mut i32, i64, *mut i32, i64, *const i32, *mut i32, i32, i64, *mut i32, *mut i32, *mut i64, *mut i32, *mut c_void) -> i32,
+    pub mpq_kv_append: unsafe extern "C" fn(*mut mpq_context, *const c_void, i32, i64, i64, i32, i32, i32, *const i32, *const f64, i32, i32, *mut u16, *mut u16, *mut u16, *const i64, *mut u16, *mut u16, i64, i32, *mut c_void) -> i32,
+    pub mpq_paged_attention: unsafe extern "C" fn(*mut mpq_context, *const u16, i64, i64, i32, *const u16, *const u16, i64, i32, i32, i32, i64, *const i32, *const i32, *const i32, i64, i64, f32, *mut c_void, i32, *mut c_void) -> i32,
+    pub mpq_prompt_attention: unsafe extern "C" fn(*mut mpq_context, *const u16, i64, *const u16, i64, *const u16, i64, i64, i32, i32, i32, i64, *const i32, f32, *mut c_void, i32, *mut c_void) -> i32,
     pub mpq_file_info: unsafe extern "C" fn(*const c_char, *mut mpq_file_info_t) -> i32,
     pub mpq_canonical_save: unsafe extern "C" fn(*const c_char, i32, i64, i64, *const u8, *const c_void, f32) -> i32,
     pub mpq_canonical_load: unsafe extern "C" fn(*const c_char, *mut u8, i64, *mut c_void, i64, *mut f32) -> i32,
@@ -165,6 +170,11 @@ impl LibMpq {
                 mpq_nvfp4_quantize_swiglu: sym!(h, "mpq_nvfp4_quantize_swiglu"),
                 mpq_swiglu: sym!(h, "mpq_swiglu"),
                 mpq_q4_linear_forward_swiglu: sym!(h, "mpq_q4_linear_forward_swiglu"),
+                mpq_residual_norm: sym!(h, "mpq_residual_norm"),
+                mpq_kv_plan: sym!(h, "mpq_kv_plan"),
+                mpq_kv_append: sym!(h, "mpq_kv_append"),
+                mpq_paged_attention: sym!(h, "mpq_paged_attention"),
+                mpq_prompt_attention: sym!(h, "mpq_prompt_attention"),
                 mpq_file_info: sym!(h, "mpq_file_info"),
                 mpq_canonical_save: sym!(h, "mpq_canonical_save"),
                 mpq_canonical_load: sym!(h, "mpq_canonical_load"),

@@ -13,7 +13,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmpq.so")
 LIB_TRACE = os.path.join(HERE, "libmpq_trace.so")
-SOURCES = ["mpq.cu", "nvfp4_gemm.cu"]
+SOURCES = ["mpq.cu", "nvfp4_gemm.cu", "block.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr"]
 

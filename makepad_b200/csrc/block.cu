@@ -1,0 +1,223 @@
+// The entry points between a decoder layer's projections: norms, the paged cache, attention.
+#include <algorithm>
+
+#include "attention.cuh"
+#include "context.h"
+#include "kv_cache.cuh"
+#include "launch.h"
+#include "norm.cuh"
+#include "per_device.h"
+
+using namespace mpq;
+
+namespace {
+
+// A launch that may start beside the kernel in front of it; every kernel here waits for that one before it reads.
+template <class... P, class... A>
+cudaError_t launch_beside(const mpq_context* ctx, void (*kernel)(P...), dim3 grid, unsigned block, size_t smem, unsigned cluster, cudaStream_t s, A... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    if (ctx->pdl) {
+        at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+        at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        at[cfg.numAttrs].val.clusterDim.x = cluster;
+        at[cfg.numAttrs].val.clusterDim.y = at[cfg.numAttrs].val.clusterDim.z = 1;
+        ++cfg.numAttrs;
+    }
+    cfg.attrs = at;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
+// The context's device for the length of a call; the caller's is set again behind it.
+class OnDevice {
+public:
+    explicit OnDevice(int device)
+    {
+        if ((error = cudaGetDevice(&before_)) == cudaSuccess && before_ != device && (error = cudaSetDevice(device)) == cudaSuccess) moved_ = true;
+    }
+    ~OnDevice() { if (moved_) cudaSetDevice(before_); }
+    cudaError_t error;
+private:
+    int before_ = 0;
+    bool moved_ = false;
+};
+
+bool power_of_two(int64_t v) { return v > 0 && !(v & (v - 1)); }
+int log2_of(int64_t v) { int s = 0; while ((1ll << s) < v) ++s; return s; }
+bool page_ok(int64_t page_size) { return power_of_two(page_size) && page_size >= 16 && page_size <= 256; }
+
+constexpr int64_t MOST = 0x7FFFFFFF;
+
+}  // namespace
+
+// ---------------------------------------------------------------------------
+// norms around a block
+// ---------------------------------------------------------------------------
+template <class X, class Y>
+static cudaError_t norm_launch(const mpq_context* ctx, const NormParams& p, int64_t M, cudaStream_t s)
+{
+    // One group of eight columns per thread while there are fewer rows than SMs (latency), up to four beyond (fewer barriers per byte).
+    const int groups = p.H / 8;
+    int nv = 1;
+    while (nv < 4 && ((M > ctx->prop.multiProcessorCount && groups > 128 * nv) || groups > 1024 * nv)) nv *= 2;
+    const unsigned threads = (unsigned)((groups + nv - 1) / nv + 31) / 32 * 32;
+    auto kernel = nv == 1 ? residual_norm_kernel<1, X, Y> : nv == 2 ? residual_norm_kernel<2, X, Y> : residual_norm_kernel<4, X, Y>;
+    return launch_beside(ctx, kernel, dim3((unsigned)M), threads, 0, 1, s, p);
+}
+
+extern "C" int32_t mpq_residual_norm(mpq_context* ctx, const void* x_dev, int32_t x_is_bf16, int64_t M, int64_t H, const float* residual_dev,
+                                     float* residual_out_dev, const float* post_weight_dev, const float* gate_dev, int64_t gate_stride, float alpha,
+                                     const float* weight_dev, float eps, void* y_dev, int32_t y_is_bf16, void* stream)
+{
+    if (!ctx_ok(ctx)) return MPQ_ERR_INVALID_ARG;
+    if (!x_dev || (!residual_out_dev && !y_dev)) return fail(ctx, MPQ_ERR_INVALID_ARG, "null pointer: x, or both outputs");
+    if (M <= 0 || M > MOST || H <= 0 || H % 8) return fail(ctx, MPQ_ERR_SHAPE, "the norm needs 0 < M < 2^31 and H a positive multiple of 8 (M=%lld H=%lld)", (long long)M, (long long)H);
+    if (H > NORM_MOST_H) return fail(ctx, MPQ_ERR_UNSUPPORTED, "rows of more than %d columns", NORM_MOST_H);
+    if (gate_stride && (gate_stride < H || gate_stride % 4)) return fail(ctx, MPQ_ERR_SHAPE, "gate_stride is 0 or at least H, a multiple of 4");
+    if (!(eps >= 0.f)) return fail(ctx, MPQ_ERR_INVALID_ARG, "eps must not be negative");
+    for (const void* ptr : {x_dev, (const void*)residual_dev, (const void*)residual_out_dev, (const void*)post_weight_dev, (const void*)gate_dev, (const void*)weight_dev, (const void*)y_dev})
+        if (!aligned16(ptr)) return fail(ctx, MPQ_ERR_ALIGN, "pointers must be 16-byte aligned");
+    const OnDevice on(ctx->device);
+    CU_TRY(ctx, on.error);
+    const NormParams p = {x_dev, residual_dev, residual_out_dev, post_weight_dev, gate_dev, weight_dev, y_dev, gate_stride, (int)H, alpha, eps};
+    cudaStream_t s = (cudaStream_t)stream;
+    ctx->launches += 1;
+    if (x_is_bf16) CU_TRY(ctx, y_is_bf16 ? (norm_launch<__nv_bfloat16, __nv_bfloat16>(ctx, p, M, s)) : (norm_launch<__nv_bfloat16, float>(ctx, p, M, s)));
+    else CU_TRY(ctx, y_is_bf16 ? (norm_launch<float, __nv_bfloat16>(ctx, p, M, s)) : (norm_launch<float, float>(ctx, p, M, s)));
+    return MPQ_OK;
+}
+
+// ---------------------------------------------------------------------------
+// the paged cache
+// ---------------------------------------------------------------------------
+extern "C" int32_t mpq_kv_plan(mpq_context* ctx, int64_t n, const int32_t* new_lens_dev, const int32_t* lens_dev, int32_t* lens_out_dev, int32_t* block_table_dev,
+                               int64_t max_blocks, int32_t* free_dev, int64_t pages, const int32_t* free_count_dev, int32_t* free_count_out_dev, int32_t page_size,
+                               int64_t tokens, int32_t* starts_dev, int32_t* positions_dev, int64_t* slots_dev, int32_t* missing_dev, void* stream)
+{
+    if (!ctx_ok(ctx)) return MPQ_ERR_INVALID_ARG;
+    if (!new_lens_dev || !lens_dev || !lens_out_dev || !block_table_dev || !free_dev || !free_count_dev || !free_count_out_dev || !starts_dev || !missing_dev ||
+        (tokens > 0 && (!positions_dev || !slots_dev)))
+        return fail(ctx, MPQ_ERR_INVALID_ARG, "null pointer");
+    if (n <= 0 || max_blocks <= 0 || pages <= 0 || tokens < 0 || tokens > MOST || pages > MOST) return fail(ctx, MPQ_ERR_SHAPE, "n, max_blocks and pages must be positive, tokens not negative, all below 2^31");
+    if (!page_ok(page_size)) return fail(ctx, MPQ_ERR_SHAPE, "page_size must be a power of two from 16 to 256 (%d)", page_size);
+    if (max_blocks > MOST / page_size) return fail(ctx, MPQ_ERR_SHAPE, "max_blocks * page_size must be below 2^31");
+    if (n > PLAN_MOST_N) return fail(ctx, MPQ_ERR_UNSUPPORTED, "more than %d requests", PLAN_MOST_N);
+    const OnDevice on(ctx->device);
+    CU_TRY(ctx, on.error);
+    static PerDeviceOnce raised;
+    const size_t smem = 5 * sizeof(int) * (size_t)n;
+    if (raised.needs(ctx->device)) {
+        CU_TRY(ctx, cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 5 * (int)sizeof(int) * PLAN_MOST_N));
+        raised.mark(ctx->device);
+    }
+    const PlanParams p = {new_lens_dev, lens_dev, lens_out_dev, block_table_dev, free_dev, free_count_dev, free_count_out_dev, starts_dev, positions_dev, slots_dev, missing_dev,
+                          (int)n, page_size, (int)pages, (int)max_blocks, tokens};
+    // one CTA while it has about one token and one request per thread
+    const unsigned ctas = n <= PLAN_THREADS / 2 && tokens <= PLAN_THREADS ? 1 : PLAN_CLUSTER;
+    ctx->launches += 1;
+    CU_TRY(ctx, launch_beside(ctx, kv_plan_kernel, dim3(ctas), PLAN_THREADS, smem, ctas, (cudaStream_t)stream, p));
+    return MPQ_OK;
+}
+
+extern "C" int32_t mpq_kv_append(mpq_context* ctx, const void* qkv_dev, int32_t x_is_bf16, int64_t row_stride, int64_t tokens, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                                 const int32_t* positions_dev, const double* frequencies_dev, int32_t rot_dim, int32_t interleaved, uint16_t* q_dev, uint16_t* k_dev, uint16_t* v_dev,
+                                 const int64_t* slots_dev, uint16_t* k_cache_dev, uint16_t* v_cache_dev, int64_t pages, int32_t page_size, void* stream)
+{
+    if (!ctx_ok(ctx)) return MPQ_ERR_INVALID_ARG;
+    if (!qkv_dev || !q_dev || (rot_dim > 0 && (!positions_dev || !frequencies_dev)) || (slots_dev && (!k_cache_dev || !v_cache_dev))) return fail(ctx, MPQ_ERR_INVALID_ARG, "null pointer");
+    if (tokens <= 0 || tokens > MOST || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || q_heads > 4096)
+        return fail(ctx, MPQ_ERR_SHAPE, "tokens must be positive, q_heads a multiple of kv_heads, at most 4096 (tokens=%lld, %d and %d heads)", (long long)tokens, q_heads, kv_heads);
+    if (head_dim <= 0 || head_dim % 16 || head_dim > APPEND_MOST_D) return fail(ctx, MPQ_ERR_SHAPE, "head_dim must be a multiple of 16 up to %d (%d)", APPEND_MOST_D, head_dim);
+    if (rot_dim < 0 || rot_dim % 16 || rot_dim > head_dim) return fail(ctx, MPQ_ERR_SHAPE, "rot_dim must be a multiple of 16 up to head_dim (%d)", rot_dim);
+    if (row_stride < (int64_t)(q_heads + 2 * kv_heads) * head_dim || row_stride % 8) return fail(ctx, MPQ_ERR_SHAPE, "row_stride must be a multiple of 8 and hold the heads (%lld)", (long long)row_stride);
+    if (slots_dev && (!page_ok(page_size) || pages <= 0 || pages > MOST)) return fail(ctx, MPQ_ERR_SHAPE, "pages must be positive, page_size a power of two from 16 to 256 (%lld pages of %d)", (long long)pages, page_size);
+    for (const void* ptr : {qkv_dev, (const void*)q_dev, (const void*)k_dev, (const void*)v_dev, (const void*)k_cache_dev, (const void*)v_cache_dev})
+        if (!aligned16(ptr)) return fail(ctx, MPQ_ERR_ALIGN, "rows and caches must be 16-byte aligned");
+    const OnDevice on(ctx->device);
+    CU_TRY(ctx, on.error);
+    auto bf = [](uint16_t* ptr) { return reinterpret_cast<__nv_bfloat16*>(ptr); };
+    const AppendParams p = {qkv_dev, row_stride, positions_dev, frequencies_dev, slots_dev, bf(q_dev), bf(k_dev), bf(v_dev), bf(k_cache_dev), bf(v_cache_dev),
+                            slots_dev ? pages * page_size : 0, slots_dev ? log2_of(page_size) : 0, q_heads, kv_heads, head_dim, rot_dim};
+    auto kernel = x_is_bf16 ? (interleaved ? kv_append_kernel<__nv_bfloat16, true> : kv_append_kernel<__nv_bfloat16, false>)
+                            : (interleaved ? kv_append_kernel<float, true> : kv_append_kernel<float, false>);
+    ctx->launches += 1;
+    CU_TRY(ctx, launch_beside(ctx, kernel, dim3((unsigned)tokens), APPEND_THREADS, 0, 1, (cudaStream_t)stream, p));
+    return MPQ_OK;
+}
+
+// ---------------------------------------------------------------------------
+// attention
+// ---------------------------------------------------------------------------
+// what both forms want of their arguments
+static int32_t attention_check(mpq_context* ctx, const AttnParams& p, int64_t n, int64_t q_heads, int64_t kv_heads, int32_t head_dim, int64_t q_stride)
+{
+    if (!p.q || !p.k || !p.v || !p.starts || !p.out) return fail(ctx, MPQ_ERR_INVALID_ARG, "null pointer");
+    if (p.tokens <= 0 || p.tokens > MOST || n <= 0 || n > MOST) return fail(ctx, MPQ_ERR_SHAPE, "tokens and n must be positive and below 2^31");
+    if (q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || q_heads > 4096)
+        return fail(ctx, MPQ_ERR_SHAPE, "q_heads must be a multiple of kv_heads, at most 4096 (%lld and %lld)", (long long)q_heads, (long long)kv_heads);
+    if (head_dim != 64 && head_dim != 128) return fail(ctx, MPQ_ERR_SHAPE, "head_dim must be 64 or 128 (%d)", head_dim);
+    if (q_stride < q_heads * head_dim || q_stride % 8) return fail(ctx, MPQ_ERR_SHAPE, "a row stride must be a multiple of 8 and hold the heads");
+    if (!(p.scale == p.scale) || p.scale - p.scale != 0.f) return fail(ctx, MPQ_ERR_INVALID_ARG, "scale must be finite");
+    if (!aligned16(p.q) || !aligned16(p.k) || !aligned16(p.v) || !aligned16(p.out)) return fail(ctx, MPQ_ERR_ALIGN, "q, k, v and out must be 16-byte aligned");
+    return MPQ_OK;
+}
+
+static int32_t attention_launch(mpq_context* ctx, const AttnParams& p, int32_t head_dim, cudaStream_t s)
+{
+    const OnDevice on(ctx->device);
+    CU_TRY(ctx, on.error);
+    ctx->launches += 1;
+    CU_TRY(ctx, launch_beside(ctx, head_dim == 64 ? attention_rows_kernel<64> : attention_rows_kernel<128>, dim3((unsigned)((p.tokens + 3) / 4), p.q_heads), 128, 0, 1, s, p));
+    return MPQ_OK;
+}
+
+extern "C" int32_t mpq_paged_attention(mpq_context* ctx, const uint16_t* q_dev, int64_t q_row_stride, int64_t tokens, int32_t q_heads, const uint16_t* k_cache_dev,
+                                       const uint16_t* v_cache_dev, int64_t pages, int32_t page_size, int32_t kv_heads, int32_t head_dim, int64_t n, const int32_t* starts_dev,
+                                       const int32_t* lens_dev, const int32_t* block_table_dev, int64_t max_blocks, int64_t max_new, float scale, void* out_dev, int32_t out_is_f32,
+                                       void* stream)
+{
+    if (!ctx_ok(ctx)) return MPQ_ERR_INVALID_ARG;
+    AttnParams p = {};
+    auto bf = [](const uint16_t* ptr) { return reinterpret_cast<const __nv_bfloat16*>(ptr); };
+    p.q = bf(q_dev); p.k = bf(k_cache_dev); p.v = bf(v_cache_dev);
+    p.q_stride = q_row_stride;
+    p.starts = starts_dev; p.lens = lens_dev; p.table = block_table_dev;
+    p.width = max_blocks; p.pages = pages;
+    p.tokens = tokens; p.n = (int)std::min(n, MOST); p.q_heads = q_heads; p.kv_heads = kv_heads;
+    p.scale = scale; p.out = out_dev; p.out_f32 = out_is_f32 != 0;
+    const int32_t st = attention_check(ctx, p, n, q_heads, kv_heads, head_dim, q_row_stride);
+    if (st) return st;
+    if (!lens_dev || !block_table_dev) return fail(ctx, MPQ_ERR_INVALID_ARG, "null pointer");
+    if (!page_ok(page_size) || pages <= 0 || pages > MOST) return fail(ctx, MPQ_ERR_SHAPE, "pages must be positive, page_size a power of two from 16 to 256 (%lld pages of %d)", (long long)pages, page_size);
+    if (max_blocks <= 0 || max_blocks > MOST / page_size) return fail(ctx, MPQ_ERR_SHAPE, "max_blocks * page_size must be positive and below 2^31");
+    if (max_new < 0) return fail(ctx, MPQ_ERR_SHAPE, "max_new must not be negative");
+    p.page_shift = log2_of(page_size);
+    return attention_launch(ctx, p, head_dim, (cudaStream_t)stream);
+}
+
+extern "C" int32_t mpq_prompt_attention(mpq_context* ctx, const uint16_t* q_dev, int64_t q_row_stride, const uint16_t* k_dev, int64_t k_row_stride, const uint16_t* v_dev,
+                                        int64_t v_row_stride, int64_t tokens, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int64_t n, const int32_t* starts_dev, float scale,
+                                        void* out_dev, int32_t out_is_f32, void* stream)
+{
+    if (!ctx_ok(ctx)) return MPQ_ERR_INVALID_ARG;
+    AttnParams p = {};
+    auto bf = [](const uint16_t* ptr) { return reinterpret_cast<const __nv_bfloat16*>(ptr); };
+    p.q = bf(q_dev); p.k = bf(k_dev); p.v = bf(v_dev);
+    p.q_stride = q_row_stride; p.k_stride = k_row_stride; p.v_stride = v_row_stride;
+    p.starts = starts_dev;
+    p.tokens = tokens; p.n = (int)std::min(n, MOST); p.q_heads = q_heads; p.kv_heads = kv_heads;
+    p.scale = scale; p.out = out_dev; p.out_f32 = out_is_f32 != 0;
+    const int32_t st = attention_check(ctx, p, n, q_heads, kv_heads, head_dim, q_row_stride);
+    if (st) return st;
+    for (int64_t stride : {k_row_stride, v_row_stride})
+        if (stride < (int64_t)kv_heads * head_dim || stride % 8) return fail(ctx, MPQ_ERR_SHAPE, "a row stride must be a multiple of 8 and hold the heads");
+    return attention_launch(ctx, p, head_dim, (cudaStream_t)stream);
+}
