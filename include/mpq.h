@@ -76,7 +76,7 @@ const char* mpq_status_string(int32_t status);
 /* Text of the last error recorded on this context (thread-compatible, not thread-safe). */
 const char* mpq_last_error(const mpq_context* ctx);
 /* Reads the device-side status words (this synchronises with all prior work on
- * the GPU): the Q4 and NVFP4 kernels' and, once mpq_q4_linear_forward_static
+ * the GPU): the Q4, NVFP4 and attention kernels' and, once mpq_q4_linear_forward_static
  * has run on this device, the one inside its static array.
  * MPQ_ERR_PEER_TIMEOUT if a bounded wait inside a kernel ran out since the
  * last poll; the word is then cleared. */
@@ -299,7 +299,8 @@ int32_t mpq_kv_append(mpq_context* ctx, const void* qkv_dev, int32_t x_is_bf16, 
  * h / (q_heads / kv_heads).  out [tokens][q_heads][head_dim], bf16 or fp32; must not overlap an input.  max_new: the most new tokens of a request, as far as the caller knows
  * (0: not known); it chooses the kernel, not the result.  An entry of the table outside the cache reads as zeros; what lies behind
  * lens[i] in the last page is not used, whatever it holds.  k and v of the new tokens are read by rows that do not see them:
- * they must be finite.  Sums are fp32, the weights of v are rounded to bf16. */
+ * they must be finite.  Sums are fp32, the weights of v are rounded to bf16.
+ * scale must be finite and not negative. */
 int32_t mpq_paged_attention(mpq_context* ctx, const uint16_t* q_dev, int64_t q_row_stride, int64_t tokens, int32_t q_heads, const uint16_t* k_cache_dev,
                             const uint16_t* v_cache_dev, int64_t pages, int32_t page_size, int32_t kv_heads, int32_t head_dim, int64_t n, const int32_t* starts_dev,
                             const int32_t* lens_dev, const int32_t* block_table_dev, int64_t max_blocks, int64_t max_new, float scale, void* out_dev, int32_t out_is_f32,

@@ -4,90 +4,180 @@
 //
 // of its request (lens keys, the last `new` of them the request's own new tokens).  Query head h reads head h / (q heads / kv heads) of
 // the keys.  A row that sees no key is zero.
+//
+// One pass over the keys with the running maximum and sum of each row; a unit whose keys are shared by several CTAs (attention_plan.h)
+// leaves (maximum, sum, unscaled o) of each piece in scratch, and the CTA that is last to arrive adds them in the order of the keys: no waiting, and the
+// same bits whoever is last.
 #pragma once
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "attention_plan.h"
 #include "norm.cuh"
+#include "nvfp4_ptx.cuh"
+#include "settle.cuh"
 
 namespace mpq {
 
 // keys and values: pages of a cache, or rows beside the queries
 struct AttnParams {
-    const __nv_bfloat16 *q, *k, *v;
-    int64_t q_stride, k_stride, v_stride;   // elements between tokens (k, v: without a table)
+    const __nv_bfloat16* q;
+    int64_t q_stride;                       // elements between tokens
     const int32_t *starts, *lens, *table;   // lens, table: null without a cache
     int64_t width;                          // entries of a table row
     int64_t pages;
     int page_shift;
     int64_t tokens;
-    int n, q_heads, kv_heads;
-    float scale;
+    int n, q_heads, kv_heads, group;
+    float scale_log2;                       // scale / ln 2: the weights are powers of two
     void* out;
     int out_f32;
+    float* partial;                         // pieces of cut units; null: units stay whole
+    uint32_t* arrived;                      // per CTA: pieces of the unit that it opened
+    int* status;
 };
 
-// rows, first row and keys of request i, within the arrays whatever the lengths say
-struct AttnRequest {
-    int first, rows, keys;
-};
+constexpr uint32_t ATTN_TRIES = 1u << 17;   // of a suspended wait (up to 4 us each)
+
 __device__ __forceinline__ AttnRequest attn_request(const AttnParams& p, int i)
 {
-    const int64_t a = min(max((int64_t)p.starts[i], (int64_t)0), p.tokens), b = min(max((int64_t)p.starts[i + 1], a), p.tokens);
-    AttnRequest r;
-    r.first = (int)a;
-    r.rows = (int)(b - a);
-    r.keys = p.lens ? (int)min((int64_t)max(p.lens[i], 0), p.width << p.page_shift) : r.rows;
-    return r;
+    return attn_request(p.starts[i], p.starts[i + 1], p.tokens, p.lens != nullptr, p.lens ? p.lens[i] : 0, p.width << p.page_shift);
 }
 
-// the simplest form: a warp per query row, its keys one after the other
-template <int D>
-__global__ void __launch_bounds__(128) attention_rows_kernel(const __grid_constant__ AttnParams p)
+// a CTA's place in the order of all tiles
+struct AttnPlace {
+    int64_t total, unit;                    // all tiles; first tile of the unit
+    int64_t block;
+    int request, head;
+};
+
+// Where the CTA's run begins: every CTA adds up all requests.  By all threads, with a barrier in it.
+template <int ROWS, int TILE>
+__device__ __forceinline__ AttnPlace attn_locate(const AttnParams& p, bool whole)
 {
-    asm volatile("griddepcontrol.launch_dependents;");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    constexpr int PER = D / 32;
-    const int lane = threadIdx.x & 31, h = blockIdx.y, kh = h / (p.q_heads / p.kv_heads);
-    const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (t >= p.tokens) return;
-    int i = 0;
-    AttnRequest r = {};
-    for (; i < p.n; ++i) {
-        r = attn_request(p, i);
-        if (t >= r.first && t < r.first + r.rows) break;
+    __shared__ long long s_sums[32];
+    __shared__ long long s_total;
+    __shared__ AttnPlace s_place;
+    const int threads = blockDim.x, warps = threads >> 5, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int per = (p.n + threads - 1) / threads, i0 = min(p.n, (int)threadIdx.x * per), i1 = min(p.n, i0 + per);
+    long long mine = 0;
+    for (int i = i0; i < i1; ++i) {
+        const AttnRequest r = attn_request(p, i);
+        const int64_t blocks = attn_blocks(r, p.group, ROWS);
+        for (int64_t b = 0; b < blocks; ++b) mine += whole ? 1 : attn_block_tiles(r, p.group, b, ROWS, TILE);
     }
-    if (i == p.n) return;
-    const int seen = max(0, min(r.keys, r.keys - r.rows + (int)(t - r.first) + 1));
-    float q[PER], o[PER], m = -INFINITY, l = 0.f;
-    for (int e = 0; e < PER; ++e) { q[e] = __bfloat162float(p.q[t * p.q_stride + (int64_t)h * D + lane * PER + e]); o[e] = 0.f; }
-    for (int j = 0; j < seen; ++j) {
-        const __nv_bfloat16 *k, *v;
-        if (p.table) {
-            const int page = p.table[i * p.width + (j >> p.page_shift)];
-            const int64_t at = ((((int64_t)page * p.kv_heads + kh) << p.page_shift) + (j & ((1 << p.page_shift) - 1))) * D;
-            k = v = nullptr;                                   // an entry outside the cache reads as zeros
-            if (page >= 0 && page < p.pages) { k = p.k + at; v = p.v + at; }
-        } else {
-            k = p.k + (r.first + j) * p.k_stride + (int64_t)kh * D;
-            v = p.v + (r.first + j) * p.v_stride + (int64_t)kh * D;
+    mine *= p.kv_heads;
+    long long run = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(~0u, run, o);
+        if (lane >= o) run += up;
+    }
+    if (lane == 31) s_sums[warp] = run;
+    __syncthreads();
+    long long before = run - mine, total = 0;
+    for (int w = 0; w < warps; ++w) {
+        if (w < warp) before += s_sums[w];
+        total += s_sums[w];
+    }
+    if (threadIdx.x == 0) s_total = total;
+    const int64_t ctas = min((int64_t)gridDim.x, (int64_t)total), lo = blockIdx.x < ctas ? attn_run(blockIdx.x, total, ctas) : total;
+    if (mine && before <= lo && lo < before + mine) {
+        int64_t at = before;
+        for (int i = i0; i < i1; ++i) {
+            const AttnRequest r = attn_request(p, i);
+            const int64_t blocks = attn_blocks(r, p.group, ROWS);
+            for (int64_t b = 0; b < blocks; ++b) {
+                const int64_t cost = whole ? 1 : attn_block_tiles(r, p.group, b, ROWS, TILE), all = cost * p.kv_heads;
+                if (lo < at + all) {
+                    const int head = (int)((lo - at) / cost);
+                    s_place = AttnPlace{0, at + head * cost, b, i, head};
+                    b = blocks;
+                    i = i1;
+                }
+                at += all;
+            }
         }
-        float s = 0.f;
-        for (int e = 0; e < PER; ++e) s = fmaf(q[e], k ? __bfloat162float(k[lane * PER + e]) : 0.f, s);
-        for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(~0u, s, x);
-        s *= p.scale;
-        const float m2 = fmaxf(m, s), a = m == -INFINITY ? 0.f : __expf(m - m2), w = __expf(s - m2);
-        l = l * a + w;
-        for (int e = 0; e < PER; ++e) o[e] = o[e] * a + w * (v ? __bfloat162float(v[lane * PER + e]) : 0.f);
-        m = m2;
     }
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-    for (int e = 0; e < PER; ++e) {
-        const int64_t at = (t * p.q_heads + h) * D + lane * PER + e;
-        if (p.out_f32) static_cast<float*>(p.out)[at] = o[e] * inv;
-        else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(o[e] * inv);
+    __syncthreads();
+    AttnPlace place = s_place;
+    place.total = s_total;
+    return place;
+}
+
+// The units of a CTA's run, one after the other.  The next request's lengths are fetched when this one's are first used.
+template <int ROWS, int TILE>
+struct AttnWalk {
+    AttnRequest r, next;
+    int64_t lo, hi, unit, block, blocks, total, ctas;
+    int request, head, tiles;
+    bool whole;
+
+    __device__ __forceinline__ void fetch(const AttnParams& p, int i)
+    {
+        if (i < p.n) next = attn_request(p, i);
     }
+    __device__ __forceinline__ void enter(const AttnParams& p)
+    {
+        r = next;
+        blocks = attn_blocks(r, p.group, ROWS);
+        fetch(p, request + 1);
+    }
+    __device__ __forceinline__ void size(const AttnParams& p) { tiles = attn_block_tiles(r, p.group, block, ROWS, TILE); }
+
+    __device__ __forceinline__ void begin(const AttnParams& p, const AttnPlace& at, bool whole_units)
+    {
+        whole = whole_units;
+        total = at.total;
+        ctas = min((int64_t)gridDim.x, total);
+        lo = blockIdx.x < ctas ? attn_run(blockIdx.x, total, ctas) : total;
+        hi = blockIdx.x < ctas ? attn_run(blockIdx.x + 1, total, ctas) : total;
+        if (lo >= hi) return;
+        unit = at.unit; block = at.block; request = at.request; head = at.head;
+        fetch(p, request);
+        enter(p);
+        size(p);
+    }
+    __device__ __forceinline__ bool more() const { return unit < hi; }
+    __device__ __forceinline__ int cost() const { return whole ? 1 : tiles; }
+    // tiles of the unit that are this CTA's: [first, end)
+    __device__ __forceinline__ int first() const { return whole || lo <= unit ? 0 : (int)(lo - unit); }
+    __device__ __forceinline__ int end() const { return whole || unit + tiles <= hi ? tiles : (int)(hi - unit); }
+    __device__ __forceinline__ void step(const AttnParams& p)
+    {
+        unit += cost();
+        if (++head < p.kv_heads || unit >= hi) return;
+        head = 0;
+        if (++block >= blocks) {
+            block = 0;
+            do {
+                ++request;
+                enter(p);
+            } while (!blocks);                                 // (there is one: unit < hi)
+        }
+        size(p);
+    }
+    // CTAs that have the unit's pieces
+    __device__ __forceinline__ int opener() const { return attn_owner(unit, total, ctas); }
+    __device__ __forceinline__ int closer() const { return attn_owner(unit + cost() - 1, total, ctas); }
+};
+
+// a wait that gives up: after that nothing is waited for any more, and the kernel runs to its end
+__device__ __forceinline__ void attn_wait(uint32_t bar, uint32_t parity, volatile int* abort, int* status, int code)
+{
+    if (*abort) return;
+    if (!bar_wait(bar, parity, ATTN_TRIES)) {
+        *abort = 1;
+        atomicExch(status, code);
+    }
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int a, int b, int c, int d, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(dst), "l"(map), "r"(a), "r"(b), "r"(c), "r"(d), "r"(bar) : "memory");
 }
 
 }  // namespace mpq

@@ -2,6 +2,8 @@
 #include <algorithm>
 
 #include "attention.cuh"
+#include "attention_few.cuh"
+#include "attention_rows.cuh"
 #include "context.h"
 #include "kv_cache.cuh"
 #include "launch.h"
@@ -156,26 +158,94 @@ extern "C" int32_t mpq_kv_append(mpq_context* ctx, const void* qkv_dev, int32_t 
 // ---------------------------------------------------------------------------
 // attention
 // ---------------------------------------------------------------------------
+namespace {
+
+// keys and values of a call: the pages of a cache, or rows
+struct AttnKeys {
+    const uint16_t *k, *v;
+    int64_t k_stride, v_stride;      // elements between rows (without pages)
+    int64_t pages;
+    int page_size;
+    int64_t max_new;
+};
+
+}  // namespace
+
 // what both forms want of their arguments
-static int32_t attention_check(mpq_context* ctx, const AttnParams& p, int64_t n, int64_t q_heads, int64_t kv_heads, int32_t head_dim, int64_t q_stride)
+static int32_t attention_check(mpq_context* ctx, const AttnParams& p, const AttnKeys& kv, int64_t n, int64_t q_heads, int64_t kv_heads, int32_t head_dim, float scale)
 {
-    if (!p.q || !p.k || !p.v || !p.starts || !p.out) return fail(ctx, MPQ_ERR_INVALID_ARG, "null pointer");
+    if (!p.q || !kv.k || !kv.v || !p.starts || !p.out) return fail(ctx, MPQ_ERR_INVALID_ARG, "null pointer");
     if (p.tokens <= 0 || p.tokens > MOST || n <= 0 || n > MOST) return fail(ctx, MPQ_ERR_SHAPE, "tokens and n must be positive and below 2^31");
     if (q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || q_heads > 4096)
         return fail(ctx, MPQ_ERR_SHAPE, "q_heads must be a multiple of kv_heads, at most 4096 (%lld and %lld)", (long long)q_heads, (long long)kv_heads);
     if (head_dim != 64 && head_dim != 128) return fail(ctx, MPQ_ERR_SHAPE, "head_dim must be 64 or 128 (%d)", head_dim);
-    if (q_stride < q_heads * head_dim || q_stride % 8) return fail(ctx, MPQ_ERR_SHAPE, "a row stride must be a multiple of 8 and hold the heads");
-    if (!(p.scale == p.scale) || p.scale - p.scale != 0.f) return fail(ctx, MPQ_ERR_INVALID_ARG, "scale must be finite");
-    if (!aligned16(p.q) || !aligned16(p.k) || !aligned16(p.v) || !aligned16(p.out)) return fail(ctx, MPQ_ERR_ALIGN, "q, k, v and out must be 16-byte aligned");
+    if (p.q_stride < q_heads * head_dim || p.q_stride % 8) return fail(ctx, MPQ_ERR_SHAPE, "a row stride must be a multiple of 8 and hold the heads");
+    if (!(scale >= 0.f) || scale - scale != 0.f) return fail(ctx, MPQ_ERR_INVALID_ARG, "scale must be finite and not negative");
+    if (!aligned16(p.q) || !aligned16(kv.k) || !aligned16(kv.v) || !aligned16(p.out)) return fail(ctx, MPQ_ERR_ALIGN, "q, k, v and out must be 16-byte aligned");
     return MPQ_OK;
 }
 
-static int32_t attention_launch(mpq_context* ctx, const AttnParams& p, int32_t head_dim, cudaStream_t s)
+static void attention_params(AttnParams* p, const uint16_t* q, int64_t q_stride, int64_t tokens, int64_t n, const int32_t* starts, int32_t q_heads, int32_t kv_heads, float scale, void* out,
+                             int32_t out_is_f32)
+{
+    *p = AttnParams{};
+    p->q = reinterpret_cast<const __nv_bfloat16*>(q);
+    p->q_stride = q_stride;
+    p->starts = starts;
+    p->tokens = tokens; p->n = (int)std::min(n, MOST);
+    p->q_heads = q_heads; p->kv_heads = kv_heads; p->group = kv_heads > 0 ? q_heads / kv_heads : 0;
+    p->scale_log2 = scale * 1.44269504088896340736f;
+    p->out = out; p->out_f32 = out_is_f32 != 0;
+}
+
+// The pieces of cut units: as much as the kernel with the largest wants, by the first call outside a capture.  Without it units stay whole.
+static void attention_scratch(mpq_context* ctx, AttnParams* p, cudaStream_t s)
+{
+    const size_t need = 2 * (size_t)ctx->prop.multiProcessorCount * FewShape<128>::PIECE * sizeof(float);
+    if (ctx->attn_partial.bytes() < need && !stream_captures(s)) ctx->attn_partial.reserve(need);
+    p->partial = ctx->attn_partial.bytes() >= need ? ctx->attn_partial.as<float>() : nullptr;
+    p->arrived = ctx->attn_arrived;
+    p->status = ctx->attn_status;
+}
+
+// a cache [pages][kv heads][page size][D] as boxes of `keys` keys of a page and head, in halves of 64 elements
+static bool cache_map(CUtensorMap* map, const void* base, const AttnKeys& kv, int kv_heads, int D, int keys)
+{
+    const uint64_t dims[4] = {64, (uint64_t)kv.page_size, (uint64_t)D / 64, (uint64_t)kv.pages * kv_heads};
+    const uint64_t strides[3] = {2ull * D, 128, 2ull * D * kv.page_size};
+    const uint32_t box[4] = {64, (uint32_t)keys, (uint32_t)D / 64, 1};
+    return make_bf16_map(map, base, 4, dims, strides, box);
+}
+
+template <int D, int BOX>
+static int32_t attention_few(mpq_context* ctx, const AttnParams& p, const AttnKeys& kv, cudaStream_t s)
+{
+    static PerDeviceOnce raised;
+    if (raised.needs(ctx->device)) {
+        CU_TRY(ctx, cudaFuncSetAttribute(attention_few_kernel<D, BOX>, cudaFuncAttributeMaxDynamicSharedMemorySize, FewShape<D>::SMEM));
+        raised.mark(ctx->device);
+    }
+    CUtensorMap map_k, map_v;
+    if (!cache_map(&map_k, kv.k, kv, p.kv_heads, D, BOX) || !cache_map(&map_v, kv.v, kv, p.kv_heads, D, BOX)) return fail(ctx, MPQ_ERR_CUDA, "cuTensorMapEncodeTiled failed for the cache");
+    ctx->launches += 1;
+    CU_TRY(ctx, launch_beside(ctx, attention_few_kernel<D, BOX>, dim3(std::min(ctx->prop.multiProcessorCount, ATTN_COUNTERS)), FEW_THREADS, FewShape<D>::SMEM, 1, s, map_k, map_v, p));
+    return MPQ_OK;
+}
+
+static int32_t attention_launch(mpq_context* ctx, AttnParams p, const AttnKeys& kv, int32_t head_dim, cudaStream_t s)
 {
     const OnDevice on(ctx->device);
     CU_TRY(ctx, on.error);
+    attention_scratch(ctx, &p, s);
+    const int64_t most_new = kv.max_new > 0 ? std::min(kv.max_new, p.tokens) : p.tokens;
+    if (p.table && most_new * p.group <= FEW_ROWS) {
+        if (head_dim == 64) return kv.page_size == 16 ? attention_few<64, 16>(ctx, p, kv, s) : attention_few<64, 32>(ctx, p, kv, s);
+        return kv.page_size == 16 ? attention_few<128, 16>(ctx, p, kv, s) : attention_few<128, 32>(ctx, p, kv, s);
+    }
+    auto bf = [](const uint16_t* ptr) { return reinterpret_cast<const __nv_bfloat16*>(ptr); };
     ctx->launches += 1;
-    CU_TRY(ctx, launch_beside(ctx, head_dim == 64 ? attention_rows_kernel<64> : attention_rows_kernel<128>, dim3((unsigned)((p.tokens + 3) / 4), p.q_heads), 128, 0, 1, s, p));
+    CU_TRY(ctx, launch_beside(ctx, head_dim == 64 ? attention_rows_kernel<64> : attention_rows_kernel<128>, dim3((unsigned)((p.tokens + 3) / 4), p.q_heads), 128, 0, 1, s,
+                              bf(kv.k), bf(kv.v), kv.k_stride, kv.v_stride, p));
     return MPQ_OK;
 }
 
@@ -185,22 +255,19 @@ extern "C" int32_t mpq_paged_attention(mpq_context* ctx, const uint16_t* q_dev, 
                                        void* stream)
 {
     if (!ctx_ok(ctx)) return MPQ_ERR_INVALID_ARG;
-    AttnParams p = {};
-    auto bf = [](const uint16_t* ptr) { return reinterpret_cast<const __nv_bfloat16*>(ptr); };
-    p.q = bf(q_dev); p.k = bf(k_cache_dev); p.v = bf(v_cache_dev);
-    p.q_stride = q_row_stride;
-    p.starts = starts_dev; p.lens = lens_dev; p.table = block_table_dev;
-    p.width = max_blocks; p.pages = pages;
-    p.tokens = tokens; p.n = (int)std::min(n, MOST); p.q_heads = q_heads; p.kv_heads = kv_heads;
-    p.scale = scale; p.out = out_dev; p.out_f32 = out_is_f32 != 0;
-    const int32_t st = attention_check(ctx, p, n, q_heads, kv_heads, head_dim, q_row_stride);
+    AttnParams p;
+    attention_params(&p, q_dev, q_row_stride, tokens, n, starts_dev, q_heads, kv_heads, scale, out_dev, out_is_f32);
+    const AttnKeys kv = {k_cache_dev, v_cache_dev, 0, 0, pages, page_size, max_new};
+    const int32_t st = attention_check(ctx, p, kv, n, q_heads, kv_heads, head_dim, scale);
     if (st) return st;
     if (!lens_dev || !block_table_dev) return fail(ctx, MPQ_ERR_INVALID_ARG, "null pointer");
     if (!page_ok(page_size) || pages <= 0 || pages > MOST) return fail(ctx, MPQ_ERR_SHAPE, "pages must be positive, page_size a power of two from 16 to 256 (%lld pages of %d)", (long long)pages, page_size);
+    if (pages >= MOST / kv_heads) return fail(ctx, MPQ_ERR_UNSUPPORTED, "pages * kv_heads must be below 2^31");
     if (max_blocks <= 0 || max_blocks > MOST / page_size) return fail(ctx, MPQ_ERR_SHAPE, "max_blocks * page_size must be positive and below 2^31");
     if (max_new < 0) return fail(ctx, MPQ_ERR_SHAPE, "max_new must not be negative");
-    p.page_shift = log2_of(page_size);
-    return attention_launch(ctx, p, head_dim, (cudaStream_t)stream);
+    p.lens = lens_dev; p.table = block_table_dev;
+    p.width = max_blocks; p.pages = pages; p.page_shift = log2_of(page_size);
+    return attention_launch(ctx, p, kv, head_dim, (cudaStream_t)stream);
 }
 
 extern "C" int32_t mpq_prompt_attention(mpq_context* ctx, const uint16_t* q_dev, int64_t q_row_stride, const uint16_t* k_dev, int64_t k_row_stride, const uint16_t* v_dev,
@@ -208,16 +275,12 @@ extern "C" int32_t mpq_prompt_attention(mpq_context* ctx, const uint16_t* q_dev,
                                         void* out_dev, int32_t out_is_f32, void* stream)
 {
     if (!ctx_ok(ctx)) return MPQ_ERR_INVALID_ARG;
-    AttnParams p = {};
-    auto bf = [](const uint16_t* ptr) { return reinterpret_cast<const __nv_bfloat16*>(ptr); };
-    p.q = bf(q_dev); p.k = bf(k_dev); p.v = bf(v_dev);
-    p.q_stride = q_row_stride; p.k_stride = k_row_stride; p.v_stride = v_row_stride;
-    p.starts = starts_dev;
-    p.tokens = tokens; p.n = (int)std::min(n, MOST); p.q_heads = q_heads; p.kv_heads = kv_heads;
-    p.scale = scale; p.out = out_dev; p.out_f32 = out_is_f32 != 0;
-    const int32_t st = attention_check(ctx, p, n, q_heads, kv_heads, head_dim, q_row_stride);
+    AttnParams p;
+    attention_params(&p, q_dev, q_row_stride, tokens, n, starts_dev, q_heads, kv_heads, scale, out_dev, out_is_f32);
+    const AttnKeys kv = {k_dev, v_dev, k_row_stride, v_row_stride, 0, 0, 0};
+    const int32_t st = attention_check(ctx, p, kv, n, q_heads, kv_heads, head_dim, scale);
     if (st) return st;
     for (int64_t stride : {k_row_stride, v_row_stride})
         if (stride < (int64_t)kv_heads * head_dim || stride % 8) return fail(ctx, MPQ_ERR_SHAPE, "a row stride must be a multiple of 8 and hold the heads");
-    return attention_launch(ctx, p, head_dim, (cudaStream_t)stream);
+    return attention_launch(ctx, p, kv, head_dim, (cudaStream_t)stream);
 }

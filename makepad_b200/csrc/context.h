@@ -48,6 +48,10 @@ struct mpq_context {
     int q4_depth;             // most ring stages per warp
     int q4_pre;               // stages copied before the dependency resolves (the rest right after the activation loads)
     bool q4_slab4;            // M > 4 as slabs of four rows through the streaming kernel
+    // attention: pieces of units that CTAs share, then per CTA a counter of their arrivals, and a status word
+    mpq::Scratch attn_partial;
+    uint32_t* attn_arrived;
+    int* attn_status;
     mpq::Nvfp4Scratch fp4;
     mpq::StagedUpload upload;  // pinned slots through which weights travel to the device
     cudaStream_t upload_stream;
@@ -55,6 +59,7 @@ struct mpq_context {
 
 namespace mpq {
 
+constexpr int ATTN_COUNTERS = 512;      // CTAs of an attention kernel, at most
 constexpr uint32_t CTX_MAGIC = 0x4D505143u;
 
 inline int32_t fail(mpq_context* ctx, int32_t code, const char* fmt, ...)

@@ -96,6 +96,8 @@ extern "C" int32_t mpq_context_create(int32_t device, mpq_context** out)
     c->q4_partials_ctas = 0;
     c->q4_status = nullptr;
     c->upload_stream = nullptr;
+    c->attn_arrived = nullptr;
+    c->attn_status = nullptr;
     if (cudaSetDevice(device) != cudaSuccess || cudaGetDeviceProperties(&c->prop, device) != cudaSuccess) {
         delete c;
         return fail(nullptr, MPQ_ERR_CUDA, "");
@@ -108,6 +110,17 @@ extern "C" int32_t mpq_context_create(int32_t device, mpq_context** out)
         delete c;
         return fail(nullptr, MPQ_ERR_CUDA, "");
     }
+    // (here and not in the first attention call: that one may be in a capture)
+    void* counters = nullptr;
+    if (cudaMalloc(&counters, (ATTN_COUNTERS + 1) * sizeof(uint32_t)) != cudaSuccess || cudaMemset(counters, 0, (ATTN_COUNTERS + 1) * sizeof(uint32_t)) != cudaSuccess ||
+        cudaStreamSynchronize(nullptr) != cudaSuccess) {
+        cudaFree(counters);
+        cudaStreamDestroy(c->upload_stream);
+        delete c;
+        return fail(nullptr, MPQ_ERR_CUDA, "");
+    }
+    c->attn_arrived = static_cast<uint32_t*>(counters);
+    c->attn_status = reinterpret_cast<int*>(c->attn_arrived + ATTN_COUNTERS);
     const char* e = getenv("MPQ_PDL");
     c->pdl = !(e && e[0] == '0');
     e = getenv("MPQ_Q4_VARIANT");
@@ -155,6 +168,8 @@ extern "C" int32_t mpq_context_destroy(mpq_context* ctx)
     ctx->swiglu_buf.release();
     ctx->q4_partial.release();
     cudaFree(ctx->q4_status);
+    ctx->attn_partial.release();
+    cudaFree(ctx->attn_arrived);
     ctx->fp4.release();
     ctx->upload.release();
     cudaStreamDestroy(ctx->upload_stream);
@@ -1421,9 +1436,9 @@ extern "C" int32_t mpq_context_poll_status(mpq_context* ctx)
     CU_TRY(ctx, cudaSetDevice(ctx->device));
     // the third word is the one mpq_q4_linear_forward_static uses when its caller passes no status pointer
     unsigned char* stat = (ctx->device >= 0 && ctx->device < PerDeviceOnce::MAX_DEVICES) ? g_q4_static_ptr[ctx->device] : nullptr;
-    int* words[3] = {ctx->q4_status, ctx->fp4.status, reinterpret_cast<int*>(stat)};
-    const char* names[3] = {"Q4", "NVFP4 GEMM", "Q4 static-scratch"};
-    for (int i = 0; i < 3; ++i) {
+    int* words[4] = {ctx->q4_status, ctx->fp4.status, reinterpret_cast<int*>(stat), ctx->attn_status};
+    const char* names[4] = {"Q4", "NVFP4 GEMM", "Q4 static-scratch", "attention"};
+    for (int i = 0; i < 4; ++i) {
         if (!words[i]) continue;
         int v = 0;
         CU_TRY(ctx, cudaMemcpy(&v, words[i], sizeof(int), cudaMemcpyDeviceToHost));    // synchronises with prior work
@@ -1432,6 +1447,7 @@ extern "C" int32_t mpq_context_poll_status(mpq_context* ctx)
         if (i == 0 && ctx->q4_partials)                  // ... and the slots the aborted launch may have left full
             cudaMemset(ctx->q4_partials, 0, (size_t)ctx->q4_partials_ctas * Q4S_SLOT_BYTES_PER_CTA);
         if (i == 2) cudaMemset(stat + 256, 0, Q4_STATIC_SLOT_BYTES);
+        if (i == 3) cudaMemset(ctx->attn_arrived, 0, ATTN_COUNTERS * sizeof(uint32_t));
         return fail(ctx, MPQ_ERR_PEER_TIMEOUT, "a bounded device-side wait ran out (%s kernel, code %d)", names[i], v);
     }
     return MPQ_OK;

@@ -57,6 +57,9 @@ void nvfp4_weight_map(Nvfp4Dev& w);
 // TMA map of a Q4 tile stream (see Q4Dev::map)
 bool make_q4_stream_map(CUtensorMap* map, const void* stream, int nrp, int nchunks);
 
+// TMA map of a bf16 array, innermost dimension first; strides in bytes from the second dimension on; 128-byte swizzle, zeros outside
+bool make_bf16_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box);
+
 // launches the tensor-pipe ceiling probe (see nvfp4_mma_probe_kernel); *flop = the flop it executes
 int32_t nvfp4_mma_probe_launch(Nvfp4Scratch& scratch, int device, int sm_count, int mmas, cudaStream_t s, double* flop, std::string& err);
 

@@ -1104,6 +1104,17 @@ bool make_q4_stream_map(CUtensorMap* map, const void* stream, int nrp, int nchun
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool make_bf16_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box)
+{
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    cuuint64_t d[5], st[5];
+    cuuint32_t b[5], one[5] = {1u, 1u, 1u, 1u, 1u};
+    for (int i = 0; i < rank; ++i) { d[i] = dims[i]; b[i] = box[i]; if (i) st[i - 1] = strides[i - 1]; }
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(base), d, st, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 void nvfp4_weight_map(Nvfp4Dev& w) { w.mapped = make_map(&w.map_first, w.codes, w.N, w.K, 128) && make_map(&w.map_second, w.codes, w.N, w.K, BN - 128); }
 
 // CTA pairs the device can keep resident at once (0: the pair kernel cannot be used)

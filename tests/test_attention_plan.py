@@ -1,0 +1,72 @@
+"""How the attention kernels cut their work (attention_plan.h), compiled for the host: every tile of every unit belongs to one CTA, pieces are counted
+by the CTAs that have them, and lengths that say nonsense stay inside the arrays."""
+import os
+import subprocess
+import tempfile
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+PROGRAM = r"""
+#include "attention_plan.h"
+#include <cstdio>
+#include <random>
+#include <vector>
+using namespace mpq;
+int main()
+{
+    std::mt19937 rng(1);
+    auto pick = [&](int a, int b) { return a + (int)(rng() % (unsigned)(b - a + 1)); };
+    long bad = 0;
+    for (int trial = 0; trial < 4000; ++trial) {
+        // owners of tiles agree with the runs, for fewer and for more tiles than CTAs
+        const int64_t ctas0 = pick(1, 160), total = pick(1, trial % 2 ? 300 : 100000), ctas = ctas0 < total ? ctas0 : total;
+        if (attn_run(0, total, ctas) != 0 || attn_run(ctas, total, ctas) != total) ++bad;
+        for (int64_t c = 0; c < ctas; ++c) {
+            const int64_t lo = attn_run(c, total, ctas), hi = attn_run(c + 1, total, ctas);
+            if (lo >= hi) ++bad;
+            if (attn_owner(lo, total, ctas) != c || attn_owner(hi - 1, total, ctas) != c) ++bad;
+        }
+    }
+    if (attn_owner((1ll << 46) - 1, 1ll << 46, 148) != 147) ++bad;
+    for (int trial = 0; trial < 3000; ++trial) {
+        const int group = pick(1, 20), rows = trial % 2 ? 16 : 256, tile = 128;
+        const int64_t tokens = pick(1, 900), start = pick(-5, 1000), next = pick(-5, 1000);
+        const bool paged = trial % 3 != 0;
+        const int64_t most = 16 * pick(1, 200), len = pick(-3, 4000);
+        const AttnRequest r = attn_request(start, next, tokens, paged, len, most);
+        if (r.first < 0 || r.rows < 0 || r.first + r.rows > tokens || r.keys < 0 || (paged && r.keys > most) || (!paged && r.keys != r.rows)) ++bad;
+        const int64_t blocks = attn_blocks(r, group, rows);
+        int64_t counted = 0;
+        for (int64_t b = 0; b < blocks; ++b) {
+            const int mine = attn_block_rows(r, group, b, rows);
+            if (mine < 1 || mine > rows) ++bad;
+            counted += mine;
+            // keys of the block: the most that any of its rows sees, by counting
+            int seen = 0;
+            for (int i = 0; i < mine; ++i) {
+                const int64_t j = (b * rows + i) / group;
+                int n = 0;
+                const int64_t last = (int64_t)r.keys - r.rows + j;
+                if (last >= 0) n = (int)(last + 1 < r.keys ? last + 1 : r.keys);
+                if (n != attn_seen(r, j)) ++bad;
+                seen = n > seen ? n : seen;
+            }
+            if (seen != attn_block_keys(r, group, b, rows)) ++bad;
+            const int tiles = attn_block_tiles(r, group, b, rows, tile);
+            if (tiles < 1 || tiles * tile < seen || (tiles > 1 && (tiles - 1) * tile >= seen)) ++bad;
+        }
+        if (counted != (int64_t)r.rows * group) ++bad;
+    }
+    std::printf("%ld\n", bad);
+    return bad != 0;
+}
+"""
+
+
+def test_the_cut_of_the_work():
+    with tempfile.TemporaryDirectory() as tmp:
+        src, exe = os.path.join(tmp, "t.cpp"), os.path.join(tmp, "t")
+        open(src, "w").write(PROGRAM)
+        subprocess.check_call(["g++", "-std=c++17", "-O1", "-Wall", "-I", os.path.join(ROOT, "makepad_b200", "csrc"), src, "-o", exe])
+        out = subprocess.run([exe], capture_output=True, text=True)
+        assert out.returncode == 0 and out.stdout.strip() == "0", out.stdout + out.stderr
