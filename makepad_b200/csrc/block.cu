@@ -3,7 +3,7 @@
 
 #include "attention.cuh"
 #include "attention_few.cuh"
-#include "attention_rows.cuh"
+#include "attention_many.cuh"
 #include "context.h"
 #include "kv_cache.cuh"
 #include "launch.h"
@@ -194,26 +194,35 @@ static void attention_params(AttnParams* p, const uint16_t* q, int64_t q_stride,
     p->starts = starts;
     p->tokens = tokens; p->n = (int)std::min(n, MOST);
     p->q_heads = q_heads; p->kv_heads = kv_heads; p->group = kv_heads > 0 ? q_heads / kv_heads : 0;
-    p->scale_log2 = scale * 1.44269504088896340736f;
+    p->scale_log2 = std::max(scale * 1.44269504088896340736f, 1e-30f);     // (0 would make NaN of the -inf that stands for a key that is not seen)
     p->out = out; p->out_f32 = out_is_f32 != 0;
 }
 
 // The pieces of cut units: as much as the kernel with the largest wants, by the first call outside a capture.  Without it units stay whole.
 static void attention_scratch(mpq_context* ctx, AttnParams* p, cudaStream_t s)
 {
-    const size_t need = 2 * (size_t)ctx->prop.multiProcessorCount * FewShape<128>::PIECE * sizeof(float);
+    const size_t need = 2 * (size_t)ctx->prop.multiProcessorCount * ManyShape<128>::PIECE * sizeof(float);
     if (ctx->attn_partial.bytes() < need && !stream_captures(s)) ctx->attn_partial.reserve(need);
     p->partial = ctx->attn_partial.bytes() >= need ? ctx->attn_partial.as<float>() : nullptr;
     p->arrived = ctx->attn_arrived;
     p->status = ctx->attn_status;
 }
 
-// a cache [pages][kv heads][page size][D] as boxes of `keys` keys of a page and head, in halves of 64 elements
-static bool cache_map(CUtensorMap* map, const void* base, const AttnKeys& kv, int kv_heads, int D, int keys)
+// a cache [pages][kv heads][page size][D] as boxes of `keys` keys of a page and head, `halves` times 64 elements
+static bool cache_map(CUtensorMap* map, const void* base, const AttnKeys& kv, int kv_heads, int D, int keys, int halves)
 {
     const uint64_t dims[4] = {64, (uint64_t)kv.page_size, (uint64_t)D / 64, (uint64_t)kv.pages * kv_heads};
     const uint64_t strides[3] = {2ull * D, 128, 2ull * D * kv.page_size};
-    const uint32_t box[4] = {64, (uint32_t)keys, (uint32_t)D / 64, 1};
+    const uint32_t box[4] = {64, (uint32_t)keys, (uint32_t)halves, 1};
+    return make_bf16_map(map, base, 4, dims, strides, box);
+}
+
+// rows [tokens][kv heads][D], `stride` elements apart, as boxes of `keys` rows of a head, 64 elements
+static bool rows_map(CUtensorMap* map, const void* base, int64_t tokens, int64_t stride, int kv_heads, int D, int keys)
+{
+    const uint64_t dims[4] = {64, (uint64_t)tokens, (uint64_t)D / 64, (uint64_t)kv_heads};
+    const uint64_t strides[3] = {2ull * stride, 128, 2ull * D};
+    const uint32_t box[4] = {64, (uint32_t)keys, 1, 1};
     return make_bf16_map(map, base, 4, dims, strides, box);
 }
 
@@ -226,9 +235,29 @@ static int32_t attention_few(mpq_context* ctx, const AttnParams& p, const AttnKe
         raised.mark(ctx->device);
     }
     CUtensorMap map_k, map_v;
-    if (!cache_map(&map_k, kv.k, kv, p.kv_heads, D, BOX) || !cache_map(&map_v, kv.v, kv, p.kv_heads, D, BOX)) return fail(ctx, MPQ_ERR_CUDA, "cuTensorMapEncodeTiled failed for the cache");
+    if (!cache_map(&map_k, kv.k, kv, p.kv_heads, D, BOX, D / 64) || !cache_map(&map_v, kv.v, kv, p.kv_heads, D, BOX, D / 64)) return fail(ctx, MPQ_ERR_CUDA, "cuTensorMapEncodeTiled failed for the cache");
     ctx->launches += 1;
     CU_TRY(ctx, launch_beside(ctx, attention_few_kernel<D, BOX>, dim3(std::min(ctx->prop.multiProcessorCount, ATTN_COUNTERS)), FEW_THREADS, FewShape<D>::SMEM, 1, s, map_k, map_v, p));
+    return MPQ_OK;
+}
+
+template <int D, bool PAGED>
+static int32_t attention_many(mpq_context* ctx, const AttnParams& p, const AttnKeys& kv, cudaStream_t s)
+{
+    static PerDeviceOnce raised;
+    if (raised.needs(ctx->device)) {
+        CU_TRY(ctx, cudaFuncSetAttribute(attention_many_kernel<D, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, ManyShape<D>::SMEM));
+        raised.mark(ctx->device);
+    }
+    CUtensorMap maps[2];
+    for (int i = 0; i < 2; ++i) {
+        const void* base = i ? kv.v : kv.k;
+        const bool made = PAGED ? cache_map(&maps[i], base, kv, p.kv_heads, D, std::min(kv.page_size, MANY_TILE), 1)
+                                : rows_map(&maps[i], base, p.tokens, i ? kv.v_stride : kv.k_stride, p.kv_heads, D, MANY_TILE);
+        if (!made) return fail(ctx, MPQ_ERR_CUDA, "cuTensorMapEncodeTiled failed for the keys or values");
+    }
+    ctx->launches += 1;
+    CU_TRY(ctx, launch_beside(ctx, attention_many_kernel<D, PAGED>, dim3(std::min(ctx->prop.multiProcessorCount, ATTN_COUNTERS / 2)), MANY_THREADS, ManyShape<D>::SMEM, 1, s, maps[0], maps[1], p));
     return MPQ_OK;
 }
 
@@ -242,11 +271,8 @@ static int32_t attention_launch(mpq_context* ctx, AttnParams p, const AttnKeys& 
         if (head_dim == 64) return kv.page_size == 16 ? attention_few<64, 16>(ctx, p, kv, s) : attention_few<64, 32>(ctx, p, kv, s);
         return kv.page_size == 16 ? attention_few<128, 16>(ctx, p, kv, s) : attention_few<128, 32>(ctx, p, kv, s);
     }
-    auto bf = [](const uint16_t* ptr) { return reinterpret_cast<const __nv_bfloat16*>(ptr); };
-    ctx->launches += 1;
-    CU_TRY(ctx, launch_beside(ctx, head_dim == 64 ? attention_rows_kernel<64> : attention_rows_kernel<128>, dim3((unsigned)((p.tokens + 3) / 4), p.q_heads), 128, 0, 1, s,
-                              bf(kv.k), bf(kv.v), kv.k_stride, kv.v_stride, p));
-    return MPQ_OK;
+    if (p.table) return head_dim == 64 ? attention_many<64, true>(ctx, p, kv, s) : attention_many<128, true>(ctx, p, kv, s);
+    return head_dim == 64 ? attention_many<64, false>(ctx, p, kv, s) : attention_many<128, false>(ctx, p, kv, s);
 }
 
 extern "C" int32_t mpq_paged_attention(mpq_context* ctx, const uint16_t* q_dev, int64_t q_row_stride, int64_t tokens, int32_t q_heads, const uint16_t* k_cache_dev,
