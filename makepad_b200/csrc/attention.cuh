@@ -30,7 +30,8 @@ struct AttnParams {
     int64_t pages;
     int page_shift;
     int64_t tokens;
-    int n, q_heads, kv_heads, group;
+    int n, q_heads, kv_heads;
+    AttnDivisor group;
     float scale_log2;                       // scale / ln 2: the weights are powers of two
     void* out;
     int out_f32;
@@ -49,24 +50,54 @@ __device__ __forceinline__ AttnRequest attn_request(const AttnParams& p, int i)
 // a CTA's place in the order of all tiles
 struct AttnPlace {
     int64_t total, unit;                    // all tiles; first tile of the unit
-    int64_t block;
-    int request, head;
+    int block, request, head;
 };
 
-// Where the CTA's run begins: every CTA adds up all requests.  By all threads, with a barrier in it.
-template <int ROWS, int TILE>
-__device__ __forceinline__ AttnPlace attn_locate(const AttnParams& p, bool whole)
+// How a kernel cuts its work: rows of a block, keys of a tile, what a unit costs beside its tiles, and whether a warp (of WARPS) adds up
+// a request's blocks (many of them), while there are few requests
+template <int ROWS_, int TILE_, int EXTRA_, int WARPS_>
+struct AttnCut {
+    static constexpr int ROWS = ROWS_, TILE = TILE_, EXTRA = EXTRA_, WARPS = WARPS_;
+};
+template <class Cut>
+__device__ __forceinline__ int attn_unit_cost(const AttnParams& p, const AttnRequest& r, int b, bool whole)
+{
+    return whole ? 1 : attn_block_tiles(r, p.group, b, Cut::ROWS, Cut::TILE) + Cut::EXTRA;
+}
+
+// Where the CTA's run begins: every CTA adds up all requests.  By all threads, with barriers in it; `room` is shared memory of 4 bytes per thread.
+template <class Cut>
+__device__ __forceinline__ AttnPlace attn_locate(const AttnParams& p, bool whole, uint32_t* room)
 {
     __shared__ long long s_sums[32];
-    __shared__ long long s_total;
+    __shared__ long long s_total, s_before;
+    __shared__ int s_request;
     __shared__ AttnPlace s_place;
     const int threads = blockDim.x, warps = threads >> 5, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const bool by_warps = Cut::WARPS && p.n <= threads;
     const int per = (p.n + threads - 1) / threads, i0 = min(p.n, (int)threadIdx.x * per), i1 = min(p.n, i0 + per);
     long long mine = 0;
-    for (int i = i0; i < i1; ++i) {
-        const AttnRequest r = attn_request(p, i);
-        const int64_t blocks = attn_blocks(r, p.group, ROWS);
-        for (int64_t b = 0; b < blocks; ++b) mine += whole ? 1 : attn_block_tiles(r, p.group, b, ROWS, TILE);
+    if (by_warps) {
+        // the warp's requests, a lane each, then one after the other with a lane per block
+        AttnRequest all = {};
+        if (warp + warps * lane < p.n) all = attn_request(p, warp + warps * lane);
+        for (int k = 0; warp + warps * k < p.n; ++k) {
+            AttnRequest r;
+            r.first = __shfl_sync(~0u, all.first, k); r.rows = __shfl_sync(~0u, all.rows, k); r.keys = __shfl_sync(~0u, all.keys, k);
+            const int blocks = attn_blocks(r, p.group.d, Cut::ROWS);
+            uint32_t sum = 0;
+            for (int b = lane; b < blocks; b += 32) sum += attn_unit_cost<Cut>(p, r, b, whole);
+            sum = __reduce_add_sync(~0u, sum);
+            if (lane == 0) room[warp + warps * k] = sum;
+        }
+        __syncthreads();
+        if ((int)threadIdx.x < p.n) mine = room[threadIdx.x];
+    } else {
+        for (int i = i0; i < i1; ++i) {
+            const AttnRequest r = attn_request(p, i);
+            const int blocks = attn_blocks(r, p.group.d, Cut::ROWS);
+            for (int b = 0; b < blocks; ++b) mine += attn_unit_cost<Cut>(p, r, b, whole);
+        }
     }
     mine *= p.kv_heads;
     long long run = mine;
@@ -76,6 +107,7 @@ __device__ __forceinline__ AttnPlace attn_locate(const AttnParams& p, bool whole
         if (lane >= o) run += up;
     }
     if (lane == 31) s_sums[warp] = run;
+    if (threadIdx.x == 0) s_request = -1;
     __syncthreads();
     long long before = run - mine, total = 0;
     for (int w = 0; w < warps; ++w) {
@@ -85,20 +117,49 @@ __device__ __forceinline__ AttnPlace attn_locate(const AttnParams& p, bool whole
     if (threadIdx.x == 0) s_total = total;
     const int64_t ctas = min((int64_t)gridDim.x, (int64_t)total), lo = blockIdx.x < ctas ? attn_run(blockIdx.x, total, ctas) : total;
     if (mine && before <= lo && lo < before + mine) {
-        int64_t at = before;
-        for (int i = i0; i < i1; ++i) {
-            const AttnRequest r = attn_request(p, i);
-            const int64_t blocks = attn_blocks(r, p.group, ROWS);
-            for (int64_t b = 0; b < blocks; ++b) {
-                const int64_t cost = whole ? 1 : attn_block_tiles(r, p.group, b, ROWS, TILE), all = cost * p.kv_heads;
-                if (lo < at + all) {
-                    const int head = (int)((lo - at) / cost);
-                    s_place = AttnPlace{0, at + head * cost, b, i, head};
-                    b = blocks;
-                    i = i1;
+        if (by_warps) {
+            s_request = threadIdx.x;
+            s_before = before;
+        } else {
+            int64_t at = before;
+            for (int i = i0; i < i1; ++i) {
+                const AttnRequest r = attn_request(p, i);
+                const int blocks = attn_blocks(r, p.group.d, Cut::ROWS);
+                for (int b = 0; b < blocks; ++b) {
+                    const int cost = attn_unit_cost<Cut>(p, r, b, whole);
+                    const int64_t all = (int64_t)cost * p.kv_heads;
+                    if (lo < at + all) {
+                        const int head = (int)(lo - at) / cost;
+                        s_place = AttnPlace{0, at + (int64_t)head * cost, b, i, head};
+                        b = blocks;
+                        i = i1;
+                    }
+                    at += all;
                 }
-                at += all;
             }
+        }
+    }
+    __syncthreads();
+    if (by_warps && s_request >= 0 && warp == 0) {
+        const AttnRequest r = attn_request(p, s_request);
+        const int blocks = attn_blocks(r, p.group.d, Cut::ROWS);
+        long long at = s_before;
+        for (int b0 = 0; b0 < blocks; b0 += 32) {
+            const int cost = b0 + lane < blocks ? attn_unit_cost<Cut>(p, r, b0 + lane, whole) : 0;
+            long long sum = (long long)cost * p.kv_heads;
+            const long long own = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long up = __shfl_up_sync(~0u, sum, o);
+                if (lane >= o) sum += up;
+            }
+            const long long from = at + sum - own;
+            if (own && from <= lo && lo < from + own) {
+                const int head = (int)(lo - from) / cost;
+                s_place = AttnPlace{0, from + (long long)head * cost, b0 + lane, s_request, head};
+            }
+            at += __shfl_sync(~0u, sum, 31);
+            if (at > lo) break;
         }
     }
     __syncthreads();
@@ -108,11 +169,11 @@ __device__ __forceinline__ AttnPlace attn_locate(const AttnParams& p, bool whole
 }
 
 // The units of a CTA's run, one after the other.  The next request's lengths are fetched when this one's are first used.
-template <int ROWS, int TILE>
+template <class Cut>
 struct AttnWalk {
     AttnRequest r, next;
-    int64_t lo, hi, unit, block, blocks, total, ctas;
-    int request, head, tiles;
+    int64_t lo, hi, unit, total;
+    int block, blocks, request, head, tiles, ctas;
     bool whole;
 
     __device__ __forceinline__ void fetch(const AttnParams& p, int i)
@@ -122,26 +183,28 @@ struct AttnWalk {
     __device__ __forceinline__ void enter(const AttnParams& p)
     {
         r = next;
-        blocks = attn_blocks(r, p.group, ROWS);
+        blocks = attn_blocks(r, p.group.d, Cut::ROWS);
         fetch(p, request + 1);
     }
-    __device__ __forceinline__ void size(const AttnParams& p) { tiles = attn_block_tiles(r, p.group, block, ROWS, TILE); }
+    __device__ __forceinline__ void size(const AttnParams& p) { tiles = attn_block_tiles(r, p.group, block, Cut::ROWS, Cut::TILE); }
 
     __device__ __forceinline__ void begin(const AttnParams& p, const AttnPlace& at, bool whole_units)
     {
         whole = whole_units;
         total = at.total;
-        ctas = min((int64_t)gridDim.x, total);
-        lo = blockIdx.x < ctas ? attn_run(blockIdx.x, total, ctas) : total;
-        hi = blockIdx.x < ctas ? attn_run(blockIdx.x + 1, total, ctas) : total;
+        ctas = (int)min((int64_t)gridDim.x, total);
+        lo = (int)blockIdx.x < ctas ? attn_run(blockIdx.x, total, ctas) : total;
+        hi = (int)blockIdx.x < ctas ? attn_run(blockIdx.x + 1, total, ctas) : total;
+        unit = hi;
         if (lo >= hi) return;
         unit = at.unit; block = at.block; request = at.request; head = at.head;
         fetch(p, request);
         enter(p);
         size(p);
+        if (!whole && lo >= unit + tiles) step(p);             // (what is left of the unit is what it costs beside its tiles)
     }
     __device__ __forceinline__ bool more() const { return unit < hi; }
-    __device__ __forceinline__ int cost() const { return whole ? 1 : tiles; }
+    __device__ __forceinline__ int cost() const { return whole ? 1 : tiles + Cut::EXTRA; }
     // tiles of the unit that are this CTA's: [first, end)
     __device__ __forceinline__ int first() const { return whole || lo <= unit ? 0 : (int)(lo - unit); }
     __device__ __forceinline__ int end() const { return whole || unit + tiles <= hi ? tiles : (int)(hi - unit); }
@@ -159,9 +222,10 @@ struct AttnWalk {
         }
         size(p);
     }
-    // CTAs that have the unit's pieces
+    // whether other CTAs have tiles of the unit, and the CTAs that have some
+    __device__ __forceinline__ bool cut() const { return !whole && (unit < lo || unit + tiles > hi); }
     __device__ __forceinline__ int opener() const { return attn_owner(unit, total, ctas); }
-    __device__ __forceinline__ int closer() const { return attn_owner(unit + cost() - 1, total, ctas); }
+    __device__ __forceinline__ int closer() const { return attn_owner(unit + tiles - 1, total, ctas); }
 };
 
 // a wait that gives up: after that nothing is waited for any more, and the kernel runs to its end

@@ -14,6 +14,8 @@ namespace mpq {
 
 constexpr int FEW_ROWS = 16, FEW_TILE = 128, FEW_WARPS = 4, FEW_KEYS = FEW_TILE / FEW_WARPS, FEW_THREADS = 32 * (FEW_WARPS + 1);
 
+using FewCut = AttnCut<FEW_ROWS, FEW_TILE, 0, 0>;
+
 template <int D>
 struct FewShape {
     static constexpr int WARP_BYTES = FEW_KEYS * D * 2;                      // keys (or values) of one warp
@@ -65,8 +67,8 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const bool whole = !p.partial;
-    const AttnPlace place = attn_locate<FEW_ROWS, FEW_TILE>(p, whole);       // (its barriers publish the mbarriers)
-    AttnWalk<FEW_ROWS, FEW_TILE> u;
+    const AttnPlace place = attn_locate<FewCut>(p, whole, nullptr);       // (its barriers publish the mbarriers)
+    AttnWalk<FewCut> u;
     u.begin(p, place, whole);
 
     if (warp == FEW_WARPS) {
@@ -75,8 +77,7 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         const int box = lane % BOXES, what = lane / BOXES;                   // 0: k, 1: v
         int s = 0;
         uint32_t phase = 1;
-        if (u.lo < u.hi)
-            for (; u.more(); u.step(p)) {
+        for (; u.more(); u.step(p)) {
                 const int32_t* row = p.table + u.request * p.width;
                 const int end = u.end();
                 for (int t = u.first(); t < end; ++t) {
@@ -98,7 +99,7 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                     if (++s == S::STAGES) { s = 0; phase ^= 1u; }
                 }
             }
-    } else if (u.lo < u.hi) {
+    } else {
         const int g = lane >> 2, tq = lane & 3;
         float* join = reinterpret_cast<float*>(smem_dyn + (smem0 - s2u(smem_dyn)) + S::STAGES * S::STAGE_BYTES);
         // ldmatrix: lane -> row of the matrix that it points to
@@ -106,16 +107,16 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         int s = 0;
         uint32_t phase = 0;
         for (; u.more(); u.step(p)) {
-            const int rows = attn_block_rows(u.r, p.group, u.block, FEW_ROWS);
-            const int64_t row0 = u.block * FEW_ROWS;
+            const int rows = attn_block_rows(u.r, p.group.d, u.block, FEW_ROWS);
+            const int row0 = u.block * FEW_ROWS;
             // keys that rows g and g + 8 see
-            const int seen0 = attn_seen(u.r, (row0 + min(g, rows - 1)) / p.group), seen1 = attn_seen(u.r, (row0 + min(g + 8, rows - 1)) / p.group);
-            const int seen_all = attn_seen(u.r, row0 / p.group);             // by every row of the block
+            const int seen0 = attn_seen(u.r, p.group.of(row0 + min(g, rows - 1))), seen1 = attn_seen(u.r, p.group.of(row0 + min(g + 8, rows - 1)));
+            const int seen_all = attn_seen(u.r, p.group.of(row0));             // by every row of the block
             uint32_t qa[D / 16][4];
             {
                 auto row_of = [&](int r) {
-                    const int64_t at = row0 + min(r, rows - 1), tok = at / p.group;
-                    return p.q + (u.r.first + tok) * p.q_stride + (int64_t)(u.head * p.group + (int)(at - tok * p.group)) * D + 2 * tq;
+                    const int at = row0 + min(r, rows - 1), tok = p.group.of(at);
+                    return p.q + (int64_t)(u.r.first + tok) * p.q_stride + ((u.head - tok) * (int)p.group.d + at) * D + 2 * tq;
                 };
                 const __nv_bfloat16 *q0 = row_of(g), *q1 = row_of(g + 8);
 #pragma unroll
@@ -239,13 +240,13 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                 *reinterpret_cast<float2*>(at + 8 * D) = make_float2(o[i][2] * f1, o[i][3] * f1);
             }
             few_sync();
-            const int opener = u.opener(), closer = u.closer();
-            const bool cut = !whole && opener != closer;
+            const bool cut = u.cut();
+            const int opener = cut ? u.opener() : 0, closer = cut ? u.closer() : 0;
             // a row's columns and what stands beside them; `slot` of scratch: what this CTA opened, or what it continues
             auto slot = [&](int cta) { return p.partial + (int64_t)(2 * cta + (cta == opener ? 1 : 0)) * S::PIECE; };
             auto store = [&](int r, int c, float v) {
-                const int64_t at = row0 + r, tok = at / p.group;
-                const int64_t to = ((u.r.first + tok) * p.q_heads + u.head * p.group + (int)(at - tok * p.group)) * D + c;
+                const int at = row0 + r, tok = p.group.of(at);
+                const int64_t to = ((int64_t)(u.r.first + tok) * p.q_heads + (u.head - tok) * (int)p.group.d + at) * D + c;
                 if (p.out_f32) static_cast<float*>(p.out)[to] = v;
                 else static_cast<__nv_bfloat16*>(p.out)[to] = __float2bfloat16_rn(v);
             };

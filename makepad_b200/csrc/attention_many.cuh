@@ -19,7 +19,8 @@
 namespace mpq {
 
 constexpr int MANY_ROWS = 256, MANY_TILE = 128, MANY_THREADS = 384;
-constexpr int MANY_REGS_WORK = 216, MANY_REGS_REST = 72;         // 2 x 216 + 72 = 3 x 168, what a thread is launched with
+constexpr int MANY_REGS_WORK = 200, MANY_REGS_REST = 104;        // 2 x 200 + 104 = 3 x 168, what a thread is launched with
+using ManyCut = AttnCut<MANY_ROWS, MANY_TILE, 1, MANY_THREADS / 32>;
 constexpr float MANY_LATE = 8.f;                                  // log2 of how far a row's maximum runs ahead of the one in use
 
 template <int D>
@@ -74,7 +75,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
 attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnParams p)
 {
     using S = ManyShape<D>;
-    using Walk = AttnWalk<MANY_ROWS, MANY_TILE>;
+    using Walk = AttnWalk<ManyCut>;
     extern __shared__ unsigned char smem_dyn[];
     __shared__ uint32_t s_tmem_base;
     __shared__ volatile int s_abort;
@@ -110,21 +111,19 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const bool whole = !p.partial;
-    const AttnPlace place = attn_locate<MANY_ROWS, MANY_TILE>(p, whole);
+    const AttnPlace place = attn_locate<ManyCut>(p, whole, reinterpret_cast<uint32_t*>(smem_dyn));
     Walk u;
     u.begin(p, place, whole);
-    const bool any = u.lo < u.hi;
     // tiles of keys of row tile t of the unit: up to this one (none where it has no rows)
     auto tiles_of = [&](int t) {
-        const int rows = attn_block_rows(u.r, p.group, u.block, MANY_ROWS) - 128 * t;
+        const int rows = attn_block_rows(u.r, p.group.d, u.block, MANY_ROWS) - 128 * t;
         if (rows <= 0) return 0;
-        const int keys = attn_seen(u.r, (u.block * MANY_ROWS + 128 * t + min(rows, 128) - 1) / p.group);
-        return keys <= MANY_TILE ? 1 : (keys + MANY_TILE - 1) / MANY_TILE;
+        return attn_tiles(attn_seen(u.r, p.group.of(u.block * MANY_ROWS + 128 * t + min(rows, 128) - 1)), MANY_TILE);
     };
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(MANY_REGS_REST));
-        if (warp == 8 && any) {
+        if (warp == 8) {
             // ---- MMA issue
             const uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);                 // bf16 x bf16 -> f32, both K-major
             const uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);      // V: rows along K
@@ -204,7 +203,7 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     if (j + 1 < end) advance();
                 }
             }
-        } else if (warp == 9 && any) {
+        } else if (warp == 9) {
             // ---- keys and values: a lane per box and half
             int s = 0;
             uint32_t phase = 1;
@@ -239,23 +238,28 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     }
                 }
             }
-        } else if (warp >= 10 && any) {
+        } else if (warp >= 10) {
             // ---- rows of Q: 16 bytes at a time into the swizzled tiles
             uint32_t phase = 1;
             const int tid = threadIdx.x - 320;
-            constexpr int CH = D / 8;
+            constexpr int CH = D / 8, STEP = 64 / CH;
+            const int c = tid % CH, r0 = tid / CH;
             for (; u.more(); u.step(p)) {
                 attn_wait(bar.q_empty, phase, &s_abort, p.status, 58);
                 phase ^= 1u;
-                const int rows = attn_block_rows(u.r, p.group, u.block, MANY_ROWS);
-                const int64_t row0 = u.block * MANY_ROWS;
-                const int all = rows <= 128 ? 128 : 256;
-                for (int i = tid; i < all * CH; i += 64) {
-                    const int r = i / CH, c = i % CH;
-                    const int64_t at = row0 + min(r, rows - 1), tok = at / p.group;
-                    const __nv_bfloat16* src = p.q + (u.r.first + tok) * p.q_stride + (int64_t)(u.head * p.group + (int)(at - tok * p.group)) * D + c * 8;
+                const int rows = attn_block_rows(u.r, p.group.d, u.block, MANY_ROWS);
+                // thread: chunk c of every fourth (or eighth) row; token and head of the row go on with it
+                const int all = rows <= 128 ? 128 : 256, group = p.group.d;
+                const int tok_step = p.group.of(STEP), head_step = STEP - tok_step * group;
+                int tok = p.group.of(u.block * MANY_ROWS + r0), head = u.block * MANY_ROWS + r0 - tok * group;
+#pragma unroll 4
+                for (int r = r0; r < all; r += STEP) {
+                    const __nv_bfloat16* src = p.q + (int64_t)(u.r.first + (r < rows ? tok : 0)) * p.q_stride + (u.head * group + head) * D + c * 8;
                     const uint32_t dst = smem0 + (r >> 7) * S::TILE_BYTES + (c >> 3) * S::HALF_BYTES + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4);
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(r < rows ? 16 : 0) : "memory");
+                    tok += tok_step;
+                    head += head_step;
+                    if (head >= group) { head -= group; ++tok; }
                 }
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -269,35 +273,41 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + lanes + 128 * t, to = tmem + lanes + 256 + 128 * t;
         uint32_t s_phase = 0, o_phase = 0;
-        if (any)
             for (; u.more(); u.step(p)) {
-                const int rows = attn_block_rows(u.r, p.group, u.block, MANY_ROWS) - 128 * t;
+                const int rows = attn_block_rows(u.r, p.group.d, u.block, MANY_ROWS) - 128 * t;
                 if (rows <= 0) continue;
-                const int64_t at = u.block * MANY_ROWS + 128 * t + min(row, rows - 1), tok = at / p.group;
-                const int seen = attn_seen(u.r, tok), seen_all = attn_seen(u.r, (u.block * MANY_ROWS + 128 * t) / p.group);
+                const int at = u.block * MANY_ROWS + 128 * t + min(row, rows - 1), tok = p.group.of(at);
+                const int seen = attn_seen(u.r, tok), seen_all = attn_seen(u.r, p.group.of(u.block * MANY_ROWS + 128 * t));
                 const int first = u.first(), end = min(u.end(), tiles_of(t));
                 float m = -INFINITY, l = 0.f;                                  // m in units of the scores as they come
                 for (int j = first; j < end; ++j) {
                     attn_wait(bar.s_full + 8 * t, s_phase, &s_abort, p.status, 59);
                     s_phase ^= 1u;
                     tc_fence_after();
-                    uint32_t x[4][32];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) tc_ld32(ts + 32 * c, x[c]);
-                    tc_ld_wait();
-                    if ((j + 1) * MANY_TILE > seen_all) {
-                        const int left = seen - j * MANY_TILE;
-#pragma unroll
-                        for (int c = 0; c < 4; ++c)
+                    // S is read twice, for the maximum and for the weights: 128 registers less, for 128 cycles of tensor memory
+                    const bool ragged = (j + 1) * MANY_TILE > seen_all;
+                    const int left = seen - j * MANY_TILE;
+                    auto hide = [&](uint32_t (&x)[32], int c) {
+                        if (ragged) {
 #pragma unroll
                             for (int i = 0; i < 32; ++i)
-                                if (32 * c + i >= left) x[c][i] = 0xFF800000u;
-                    }
+                                if (32 * c + i >= left) x[i] = 0xFF800000u;
+                        }
+                    };
                     float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
+                    for (int c = 0; c < 4; c += 2) {
+                        uint32_t x[2][32];
+                        tc_ld32(ts + 32 * c, x[0]);
+                        tc_ld32(ts + 32 * c + 32, x[1]);
+                        tc_ld_wait();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) y[i & 3] = fmaxf(y[i & 3], __uint_as_float(x[c][i]));
+                        for (int h = 0; h < 2; ++h) {
+                            hide(x[h], c + h);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) y[i & 3] = fmaxf(y[i & 3], __uint_as_float(x[h][i]));
+                        }
+                    }
                     const float top = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
                     if (j == first) m = top;
                     else if (__any_sync(~0u, (top - m) * p.scale_log2 > MANY_LATE)) {
@@ -305,7 +315,7 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                         const float m2 = fmaxf(m, top), f = m2 == -INFINITY ? 1.f : ex2((m - m2) * p.scale_log2);
                         m = m2;
                         l *= f;
-#pragma unroll
+#pragma unroll 1
                         for (int c = 0; c < D / 32; ++c) {
                             uint32_t o[32];
                             tc_ld32(to + 32 * c, o);
@@ -318,17 +328,24 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     }
                     const float base = m == -INFINITY ? 0.f : m * p.scale_log2;
                     float sum[2] = {0.f, 0.f};
+                    // (the weights of 32 keys take the place of 16 scores that have been read: the next 32 are, before they are overwritten)
+                    uint32_t x[2][32];
+                    tc_ld32(ts, x[0]);
+                    tc_ld_wait();
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
+                        if (c < 3) tc_ld32(ts + 32 * (c + 1), x[(c + 1) & 1]);
+                        hide(x[c & 1], c);
                         uint32_t w[16];
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            const float e0 = ex2(fmaf(__uint_as_float(x[c][2 * i]), p.scale_log2, -base)), e1 = ex2(fmaf(__uint_as_float(x[c][2 * i + 1]), p.scale_log2, -base));
+                            const float e0 = ex2(fmaf(__uint_as_float(x[c & 1][2 * i]), p.scale_log2, -base)), e1 = ex2(fmaf(__uint_as_float(x[c & 1][2 * i + 1]), p.scale_log2, -base));
                             sum[0] += e0;
                             sum[1] += e1;
                             // bf16 is what the tensor cores take beside bf16 values; the sum keeps the weights as they were
                             w[i] = pack_bf16(e0, e1);
                         }
+                        if (c < 3) tc_ld_wait();
                         tc_st16(ts + 16 * c, w);
                     }
                     l += sum[0] + sum[1];
@@ -343,9 +360,9 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     o_phase ^= 1u;
                     tc_fence_after();
                 }
-                const int opener = u.opener(), closer = u.closer();
-                const bool cut = !whole && opener != closer;
-                const int64_t to_row = ((u.r.first + tok) * p.q_heads + u.head * p.group + (int)(at - tok * p.group)) * D;
+                const bool cut = u.cut();
+                const int opener = cut ? u.opener() : 0, closer = cut ? u.closer() : 0;
+                const int64_t to_row = ((int64_t)(u.r.first + tok) * p.q_heads + (u.head - tok) * (int)p.group.d + at) * D;
                 auto store16 = [&](int c, const float* v) {                    // 16 columns from c on
                     if (row >= rows) return;
                     if (p.out_f32) {

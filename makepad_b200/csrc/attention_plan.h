@@ -3,8 +3,9 @@
 // The new tokens of a request and the query heads that share a head of keys are its rows, packed token by token: row = token * group +
 // head in the group.  A block is up to ROWS consecutive rows; a unit is a block and a head of keys; its tiles are the TILE keys at a time that
 // its last row sees (one, empty, where it sees none: its rows of zeros are written all the same).  The tiles of all units in order
-// (request, block, head) are cut into equal runs, one per CTA, wherever that falls: no shape leaves SMs idle.  A unit that a cut falls into has a piece
-// in each CTA from the one with its first tile to the one with its last.  A CTA opens at most one such unit (its last) and continues at most one (its first).
+// (request, block, head) are cut into equal runs, one per CTA, wherever that falls: no shape leaves SMs idle.  What a unit costs beside its tiles (its
+// queries, its end) counts as `extra` tiles behind them that nobody works on.  A unit that a cut falls into has a piece in each CTA from the one with its
+// first tile to the one with its last.  A CTA opens at most one such unit (its last) and continues at most one (its first).
 #pragma once
 #include <stdint.h>
 
@@ -31,27 +32,44 @@ MPQ_BOTH AttnRequest attn_request(int64_t start, int64_t next, int64_t tokens, b
     return r;
 }
 
-MPQ_BOTH int64_t attn_blocks(const AttnRequest& r, int group, int block_rows) { return ((int64_t)r.rows * group + block_rows - 1) / block_rows; }
+// x / d for x < 2^31, without a division: (x + mulhi(x, mul)) >> shift
+struct AttnDivisor {
+    uint32_t d, mul, shift;
+    MPQ_BOTH int of(int x) const
+    {
+#ifdef __CUDA_ARCH__
+        return (int)((__umulhi((uint32_t)x, mul) + (uint32_t)x) >> shift);
+#else
+        return (int)(((uint32_t)(((uint64_t)(uint32_t)x * mul) >> 32) + (uint32_t)x) >> shift);
+#endif
+    }
+};
+inline AttnDivisor attn_divisor(uint32_t d)
+{
+    AttnDivisor a = {d, 0, 0};
+    while ((1ull << a.shift) < d) ++a.shift;
+    a.mul = (uint32_t)((((1ull << a.shift) - d) << 32) / d + 1);
+    return a;
+}
+
+// (rows * group is below 2^31; block_rows and tile are powers of two)
+MPQ_BOTH int attn_blocks(const AttnRequest& r, int group, int block_rows) { return (int)(((uint32_t)(r.rows * group) + block_rows - 1) / (uint32_t)block_rows); }
 // keys that new token j sees
-MPQ_BOTH int attn_seen(const AttnRequest& r, int64_t j)
+MPQ_BOTH int attn_seen(const AttnRequest& r, int j)
 {
-    const int64_t s = (int64_t)r.keys - r.rows + j + 1;
-    return s < 0 ? 0 : s > r.keys ? r.keys : (int)s;
+    const int s = r.keys - (r.rows - 1 - j);
+    return s < 0 ? 0 : s;
 }
-// rows of block b, and keys that the last one of its rows from `from` on (at most `count`) sees
-MPQ_BOTH int attn_block_rows(const AttnRequest& r, int group, int64_t b, int block_rows)
+// rows of block b, and the tiles of keys that the last of its rows sees
+MPQ_BOTH int attn_block_rows(const AttnRequest& r, int group, int b, int block_rows)
 {
-    const int64_t left = (int64_t)r.rows * group - b * block_rows;
-    return left < block_rows ? (int)left : block_rows;
+    const int left = r.rows * group - b * block_rows;
+    return left < block_rows ? left : block_rows;
 }
-MPQ_BOTH int attn_block_keys(const AttnRequest& r, int group, int64_t b, int block_rows)
+MPQ_BOTH int attn_tiles(int keys, int tile) { return keys <= tile ? 1 : (int)(((uint32_t)keys + tile - 1) / (uint32_t)tile); }
+MPQ_BOTH int attn_block_tiles(const AttnRequest& r, const AttnDivisor& group, int b, int block_rows, int tile)
 {
-    return attn_seen(r, (b * block_rows + attn_block_rows(r, group, b, block_rows) - 1) / group);
-}
-MPQ_BOTH int attn_block_tiles(const AttnRequest& r, int group, int64_t b, int block_rows, int tile)
-{
-    const int keys = attn_block_keys(r, group, b, block_rows);
-    return keys <= tile ? 1 : (keys + tile - 1) / tile;
+    return attn_tiles(attn_seen(r, group.of(b * block_rows + attn_block_rows(r, (int)group.d, b, block_rows) - 1)), tile);
 }
 
 // run of CTA c of `ctas` (at most `total` of them have one), and the CTA that has tile t

@@ -178,6 +178,7 @@ static int32_t attention_check(mpq_context* ctx, const AttnParams& p, const Attn
     if (p.tokens <= 0 || p.tokens > MOST || n <= 0 || n > MOST) return fail(ctx, MPQ_ERR_SHAPE, "tokens and n must be positive and below 2^31");
     if (q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || q_heads > 4096)
         return fail(ctx, MPQ_ERR_SHAPE, "q_heads must be a multiple of kv_heads, at most 4096 (%lld and %lld)", (long long)q_heads, (long long)kv_heads);
+    if (p.tokens * p.group.d > MOST) return fail(ctx, MPQ_ERR_UNSUPPORTED, "tokens * q_heads / kv_heads must be below 2^31");
     if (head_dim != 64 && head_dim != 128) return fail(ctx, MPQ_ERR_SHAPE, "head_dim must be 64 or 128 (%d)", head_dim);
     if (p.q_stride < q_heads * head_dim || p.q_stride % 8) return fail(ctx, MPQ_ERR_SHAPE, "a row stride must be a multiple of 8 and hold the heads");
     if (!(scale >= 0.f) || scale - scale != 0.f) return fail(ctx, MPQ_ERR_INVALID_ARG, "scale must be finite and not negative");
@@ -193,7 +194,7 @@ static void attention_params(AttnParams* p, const uint16_t* q, int64_t q_stride,
     p->q_stride = q_stride;
     p->starts = starts;
     p->tokens = tokens; p->n = (int)std::min(n, MOST);
-    p->q_heads = q_heads; p->kv_heads = kv_heads; p->group = kv_heads > 0 ? q_heads / kv_heads : 0;
+    p->q_heads = q_heads; p->kv_heads = kv_heads; p->group = attn_divisor(kv_heads > 0 && q_heads >= kv_heads ? q_heads / kv_heads : 1);
     p->scale_log2 = std::max(scale * 1.44269504088896340736f, 1e-30f);     // (0 would make NaN of the -inf that stands for a key that is not seen)
     p->out = out; p->out_f32 = out_is_f32 != 0;
 }
@@ -267,7 +268,7 @@ static int32_t attention_launch(mpq_context* ctx, AttnParams p, const AttnKeys& 
     CU_TRY(ctx, on.error);
     attention_scratch(ctx, &p, s);
     const int64_t most_new = kv.max_new > 0 ? std::min(kv.max_new, p.tokens) : p.tokens;
-    if (p.table && most_new * p.group <= FEW_ROWS) {
+    if (p.table && most_new * p.group.d <= FEW_ROWS) {
         if (head_dim == 64) return kv.page_size == 16 ? attention_few<64, 16>(ctx, p, kv, s) : attention_few<64, 32>(ctx, p, kv, s);
         return kv.page_size == 16 ? attention_few<128, 16>(ctx, p, kv, s) : attention_few<128, 32>(ctx, p, kv, s);
     }

@@ -28,6 +28,13 @@ int main()
         }
     }
     if (attn_owner((1ll << 46) - 1, 1ll << 46, 148) != 147) ++bad;
+    for (int d = 1; d <= 4096; ++d) {
+        const AttnDivisor by = attn_divisor(d);
+        for (int k = 0; k < 200; ++k) {
+            const int x = k < 50 ? (int)(0x7FFFFFFF - k) : k < 100 ? k : (int)(rng() & 0x7FFFFFFF), y = x / d * d;
+            for (int v : {x, y, y > 0 ? y - 1 : 0}) bad += by.of(v) != v / d;
+        }
+    }
     for (int trial = 0; trial < 3000; ++trial) {
         const int group = pick(1, 20), rows = trial % 2 ? 16 : 256, tile = 128;
         const int64_t tokens = pick(1, 900), start = pick(-5, 1000), next = pick(-5, 1000);
@@ -35,24 +42,24 @@ int main()
         const int64_t most = 16 * pick(1, 200), len = pick(-3, 4000);
         const AttnRequest r = attn_request(start, next, tokens, paged, len, most);
         if (r.first < 0 || r.rows < 0 || r.first + r.rows > tokens || r.keys < 0 || (paged && r.keys > most) || (!paged && r.keys != r.rows)) ++bad;
-        const int64_t blocks = attn_blocks(r, group, rows);
+        const AttnDivisor by = attn_divisor(group);
+        const int blocks = attn_blocks(r, group, rows);
         int64_t counted = 0;
-        for (int64_t b = 0; b < blocks; ++b) {
+        for (int b = 0; b < blocks; ++b) {
             const int mine = attn_block_rows(r, group, b, rows);
             if (mine < 1 || mine > rows) ++bad;
             counted += mine;
             // keys of the block: the most that any of its rows sees, by counting
             int seen = 0;
             for (int i = 0; i < mine; ++i) {
-                const int64_t j = (b * rows + i) / group;
+                const int j = (b * rows + i) / group;
                 int n = 0;
                 const int64_t last = (int64_t)r.keys - r.rows + j;
                 if (last >= 0) n = (int)(last + 1 < r.keys ? last + 1 : r.keys);
                 if (n != attn_seen(r, j)) ++bad;
                 seen = n > seen ? n : seen;
             }
-            if (seen != attn_block_keys(r, group, b, rows)) ++bad;
-            const int tiles = attn_block_tiles(r, group, b, rows, tile);
+            const int tiles = attn_block_tiles(r, by, b, rows, tile);
             if (tiles < 1 || tiles * tile < seen || (tiles > 1 && (tiles - 1) * tile >= seen)) ++bad;
         }
         if (counted != (int64_t)r.rows * group) ++bad;
