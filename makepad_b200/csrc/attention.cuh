@@ -65,14 +65,15 @@ __device__ __forceinline__ int attn_unit_cost(const AttnParams& p, const AttnReq
     return whole ? 1 : attn_block_tiles(r, p.group, b, Cut::ROWS, Cut::TILE) + Cut::EXTRA;
 }
 
+struct AttnShared {
+    long long sums[32], total, before;
+    AttnPlace place;
+    int request;
+};
 // Where the CTA's run begins: every CTA adds up all requests.  By all threads, with barriers in it; `room` is shared memory of 4 bytes per thread.
 template <class Cut>
-__device__ __forceinline__ AttnPlace attn_locate(const AttnParams& p, bool whole, uint32_t* room)
+__device__ __forceinline__ AttnPlace attn_locate(const AttnParams& p, bool whole, AttnShared& sh, uint32_t* room)
 {
-    __shared__ long long s_sums[32];
-    __shared__ long long s_total, s_before;
-    __shared__ int s_request;
-    __shared__ AttnPlace s_place;
     const int threads = blockDim.x, warps = threads >> 5, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const bool by_warps = Cut::WARPS && p.n <= threads;
     const int per = (p.n + threads - 1) / threads, i0 = min(p.n, (int)threadIdx.x * per), i1 = min(p.n, i0 + per);
@@ -106,20 +107,20 @@ __device__ __forceinline__ AttnPlace attn_locate(const AttnParams& p, bool whole
         const long long up = __shfl_up_sync(~0u, run, o);
         if (lane >= o) run += up;
     }
-    if (lane == 31) s_sums[warp] = run;
-    if (threadIdx.x == 0) s_request = -1;
+    if (lane == 31) sh.sums[warp] = run;
+    if (threadIdx.x == 0) sh.request = -1;
     __syncthreads();
     long long before = run - mine, total = 0;
     for (int w = 0; w < warps; ++w) {
-        if (w < warp) before += s_sums[w];
-        total += s_sums[w];
+        if (w < warp) before += sh.sums[w];
+        total += sh.sums[w];
     }
-    if (threadIdx.x == 0) s_total = total;
+    if (threadIdx.x == 0) sh.total = total;
     const int64_t ctas = min((int64_t)gridDim.x, (int64_t)total), lo = blockIdx.x < ctas ? attn_run(blockIdx.x, total, ctas) : total;
     if (mine && before <= lo && lo < before + mine) {
         if (by_warps) {
-            s_request = threadIdx.x;
-            s_before = before;
+            sh.request = threadIdx.x;
+            sh.before = before;
         } else {
             int64_t at = before;
             for (int i = i0; i < i1; ++i) {
@@ -130,7 +131,7 @@ __device__ __forceinline__ AttnPlace attn_locate(const AttnParams& p, bool whole
                     const int64_t all = (int64_t)cost * p.kv_heads;
                     if (lo < at + all) {
                         const int head = (int)(lo - at) / cost;
-                        s_place = AttnPlace{0, at + (int64_t)head * cost, b, i, head};
+                        sh.place = AttnPlace{0, at + (int64_t)head * cost, b, i, head};
                         b = blocks;
                         i = i1;
                     }
@@ -140,10 +141,10 @@ __device__ __forceinline__ AttnPlace attn_locate(const AttnParams& p, bool whole
         }
     }
     __syncthreads();
-    if (by_warps && s_request >= 0 && warp == 0) {
-        const AttnRequest r = attn_request(p, s_request);
+    if (by_warps && sh.request >= 0 && warp == 0) {
+        const AttnRequest r = attn_request(p, sh.request);
         const int blocks = attn_blocks(r, p.group.d, Cut::ROWS);
-        long long at = s_before;
+        long long at = sh.before;
         for (int b0 = 0; b0 < blocks; b0 += 32) {
             const int cost = b0 + lane < blocks ? attn_unit_cost<Cut>(p, r, b0 + lane, whole) : 0;
             long long sum = (long long)cost * p.kv_heads;
@@ -156,15 +157,15 @@ __device__ __forceinline__ AttnPlace attn_locate(const AttnParams& p, bool whole
             const long long from = at + sum - own;
             if (own && from <= lo && lo < from + own) {
                 const int head = (int)(lo - from) / cost;
-                s_place = AttnPlace{0, from + (long long)head * cost, b0 + lane, s_request, head};
+                sh.place = AttnPlace{0, from + (long long)head * cost, b0 + lane, sh.request, head};
             }
             at += __shfl_sync(~0u, sum, 31);
             if (at > lo) break;
         }
     }
     __syncthreads();
-    AttnPlace place = s_place;
-    place.total = s_total;
+    AttnPlace place = sh.place;
+    place.total = sh.total;
     return place;
 }
 
@@ -228,13 +229,27 @@ struct AttnWalk {
     __device__ __forceinline__ int closer() const { return attn_owner(unit + tiles - 1, total, ctas); }
 };
 
-// a wait that gives up: after that nothing is waited for any more, and the kernel runs to its end
+// Waits that give up: after that nothing is waited for any more, and the kernel runs to its end.  The first one is suspended, the second looks at the
+// barrier all the time: what stands around a suspended wait costs 200 cycles also where the barrier has been reached, which is where most
+// hand-offs of the tensor cores are.
+constexpr uint32_t ATTN_LOOKS = 1u << 25;
 __device__ __forceinline__ void attn_wait(uint32_t bar, uint32_t parity, volatile int* abort, int* status, int code)
 {
     if (*abort) return;
     if (!bar_wait(bar, parity, ATTN_TRIES)) {
         *abort = 1;
         atomicExch(status, code);
+    }
+}
+__device__ __forceinline__ void attn_spin(uint32_t bar, uint32_t parity, volatile int* abort, int* status, int code)
+{
+    for (uint32_t n = 0; !bar_test(bar, parity); ++n) {
+        if ((n & 1023u) == 1023u && *abort) return;
+        if (n > ATTN_LOOKS) {
+            *abort = 1;
+            atomicExch(status, code);
+            return;
+        }
     }
 }
 

@@ -50,6 +50,7 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     extern __shared__ unsigned char smem_dyn[];
     __shared__ volatile int s_abort;
     __shared__ int s_last;
+    __shared__ AttnShared s_shared;
     __shared__ float s_max[FEW_WARPS][FEW_ROWS], s_sum[FEW_WARPS][FEW_ROWS];
     __shared__ __align__(8) uint64_t s_bars[S::STAGES * (FEW_WARPS + 1)];
     const uint32_t smem0 = (s2u(smem_dyn) + 1023u) & ~1023u, bars = s2u(s_bars);
@@ -67,7 +68,7 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const bool whole = !p.partial;
-    const AttnPlace place = attn_locate<FewCut>(p, whole, nullptr);       // (its barriers publish the mbarriers)
+    const AttnPlace place = attn_locate<FewCut>(p, whole, s_shared, nullptr);       // (its barriers publish the mbarriers)
     AttnWalk<FewCut> u;
     u.begin(p, place, whole);
 

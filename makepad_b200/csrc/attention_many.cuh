@@ -2,33 +2,57 @@
 //
 // A unit is 256 rows (two tiles of 128) and a head of keys; its keys come 128 at a time.  Per tile and 128 keys:
 //   S = Q K^T      tcgen05.mma kind::f16, Q and K from shared memory, S in tensor memory
-//   P = 2^(S - m)  a thread per row: S to registers, running maximum m and sum, P back over S as bf16
+//   P = 2^(S - m)  S to registers, running maximum m and sum, P back over S as bf16
 //   O += P V       P from tensor memory, V from shared memory (as it lies: keys are its rows, the MMA's K), O in tensor memory
-// While the threads of one tile work on their S, the tensor core does the other tile's products: 4 x 128 x 128 x D x 2 flop per 128 keys
-// in two bursts of 1024 cycles, which is also what 2 x 128 x 128 exponentials take.
+// P lies over S, so the chain of a tile is S, softmax, P V, next S; while one tile's softmax runs the tensor core does the other tile's products
+// (1024 cycles at D = 128).  The softmax is therefore made short: two teams of four warps per tile, a thread per row and half of the
+// keys; a quarter of the exponentials by polynomial (power2); the product begins with the first half of each team's keys.
+// Cycles per 128 keys of both tiles: a team per tile 3960, with issue, waits and exponentials as below TEAMS; tensor pipe 2048.
 //
 // The maximum that the weights stand against follows late: only when a row's own maximum is 2^8 above it is O scaled (read, multiplied, written
 // back); until then the weights just grow, which costs neither bf16 nor fp32 any of their bits.
 //
-// ROLES, 12 warps: two teams of four (a tile each): softmax, epilogue.  Warp 8 issues the MMAs, warp 9 fetches keys and values (TMA, by pages or
-// by rows), warps 10 and 11 the rows of Q (any number of heads shares a head of keys, so a tile's rows are no box), a unit ahead.
-// Tensor memory: S0, S1, O0, O1 of 128 columns each, all of it.
+// ROLES, 20 warps: 0..15 softmax and epilogue (tile, half, quarter of the rows).  16 and 17 issue the MMAs, a tile each: one warp for both had its
+// own bookkeeping between the tiles' products.  18 fetches keys and values (TMA, by pages or by rows), 19 walks the units and says to the others what
+// each is, ahead of them.  A tile's rows of Q (any number of heads shares a head of keys, so they are no box) are copied by its softmax teams behind
+// their last weights, while the last product runs.  Tensor memory: S0, S1, O0, O1 of 128 columns each, all of it.
 #pragma once
+#include <type_traits>
+
 #include "attention.cuh"
 
 namespace mpq {
 
-constexpr int MANY_ROWS = 256, MANY_TILE = 128, MANY_THREADS = 384;
-constexpr int MANY_REGS_WORK = 200, MANY_REGS_REST = 104;        // 2 x 200 + 104 = 3 x 168, what a thread is launched with
+constexpr int MANY_ROWS = 256, MANY_TILE = 128, MANY_THREADS = 640;
+constexpr int MANY_REGS_WORK = 104, MANY_REGS_REST = 64;         // 4 x 104 + 64 = 5 x 96, what a thread is launched with
 using ManyCut = AttnCut<MANY_ROWS, MANY_TILE, 1, MANY_THREADS / 32>;
+constexpr int MANY_POWERS = 4;                                    // every so many pairs of weights by a polynomial: see power2
 constexpr float MANY_LATE = 8.f;                                  // log2 of how far a row's maximum runs ahead of the one in use
+
+constexpr int MANY_UNITS = 4;                                     // units that are known at a time
+struct ManyUnit {
+    int there;                               // 0: no more units
+    int first, end, ends[2];                 // tiles of keys of this CTA: all, and up to where the row tiles want them
+    int keys, new_rows, first_row;           // of the request
+    int row0, rows, head, request;           // first packed row of the block, rows of it
+    int cut, opener, closer;                 // whether other CTAs have tiles of the unit, and which
+};
+struct ManyShared {
+    uint64_t q_full[2], s_full[2], p_half[2], p_full[2], o_full[2], o_empty[2], kv_full[8], kv_empty[8], unit_full[MANY_UNITS], unit_empty[MANY_UNITS];
+    ManyUnit units[MANY_UNITS];
+    float top[2][2][128];                    // a row's maximum over the keys of each team
+    AttnShared locate;
+    uint32_t tmem;
+    int last[2];
+    volatile int abort;
+};
 
 template <int D>
 struct ManyShape {
     static constexpr int HALVES = D / 64, HALF_BYTES = 128 * 128;            // 128 keys (or rows) of 64 elements, 128-byte swizzle
     static constexpr int TILE_BYTES = HALVES * HALF_BYTES;
     static constexpr int STAGES = D == 128 ? 5 : 8;                          // K and V tiles in turn
-    static constexpr int SMEM = 1024 + (2 + STAGES) * TILE_BYTES;
+    static constexpr int SMEM = (2 + STAGES) * TILE_BYTES + sizeof(ManyShared);
     static constexpr int PIECE = MANY_ROWS * (D + 2);                        // floats of a piece in scratch: o, maxima, sums
 };
 
@@ -56,18 +80,79 @@ __device__ __forceinline__ uint64_t smem_desc_sw128_mn(uint32_t addr)
     d |= (uint64_t)2 << 61;
     return d;
 }
+// one lane of a converged warp
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t pred;
+    asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(pred));
+    return pred != 0;
+}
+// a value that is the same in all lanes, where the compiler cannot see it: operands of an MMA that it does not know to be uniform go from a register to a
+// uniform one in front of every instruction (16 MMAs took 1760 cycles to issue; their pipe time is 1024)
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(~0u, x, 0); }
 __device__ __forceinline__ float ex2(float x)
 {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// NaN wins
+__device__ __forceinline__ float max_nan(float a, float b, float c)
+{
+    float y;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+// two fp32 in a register pair
+__device__ __forceinline__ uint64_t pair_of(uint32_t a, uint32_t b)
+{
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(a), "r"(b));
+    return v;
+}
+__device__ __forceinline__ uint64_t pair_of(float a, float b) { return pair_of(__float_as_uint(a), __float_as_uint(b)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ uint32_t bf16_pair(uint64_t v)
+{
+    uint32_t w;
+    asm("{\n\t.reg .f32 a, b;\n\tmov.b64 {a, b}, %1;\n\tcvt.rn.bf16x2.f32 %0, b, a;\n\t}" : "=r"(w) : "l"(v));
+    return w;
+}
+__device__ __forceinline__ uint64_t ex2_pair(uint64_t t) { return pair_of(ex2(__uint_as_float((uint32_t)t)), ex2(__uint_as_float((uint32_t)(t >> 32)))); }
+// 2^t of both by multiplications and additions, for t <= 8 (below -126: 2^-126): t = n + f with |f| <= 1/2, by adding and taking away 1.5 * 2^23,
+// whose low bits are then n; 2^f by the polynomial of degree 3 with the least relative error there, 7.5e-5 (a linear programme over 4001
+// points), a twentieth of what bf16 rounds off; n goes into the exponent.
+__device__ __forceinline__ uint64_t power2(uint64_t t)
+{
+    const float lo = fmaxf(__uint_as_float((uint32_t)t), -126.f), hi = fmaxf(__uint_as_float((uint32_t)(t >> 32)), -126.f);
+    const uint64_t x = pair_of(lo, hi), big = pair_of(12582912.f, 12582912.f), n = add2(x, big);
+    const uint64_t f = add2(x, fma2(n, pair_of(-1.f, -1.f), big));
+    uint64_t y = fma2(f, pair_of(0.0551716685295105f, 0.0551716685295105f), pair_of(0.2426111251115799f, 0.2426111251115799f));
+    y = fma2(y, f, pair_of(0.6932609677314758f, 0.6932609677314758f));
+    y = fma2(y, f, pair_of(0.9999280571937561f, 0.9999280571937561f));
+    return pair_of((uint32_t)y + ((uint32_t)n << 23), (uint32_t)(y >> 32) + ((uint32_t)(n >> 32) << 23));
+}
+// registers of a load from tensor memory that is waited for here: nothing that reads them moves in front of it
 template <int N>
-__device__ __forceinline__ void team_sync(int team) { asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(N) : "memory"); }
-
-struct ManyBars {
-    uint32_t q_full, q_empty, s_full, p_full, o_full, o_empty, kv_full, kv_empty;
-};
+__device__ __forceinline__ void tc_ld_wait_for(uint32_t (&r)[N])
+{
+    tc_ld_wait();
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+}
+template <int N>
+__device__ __forceinline__ void team_sync(int barrier) { asm volatile("bar.sync %0, %1;" ::"r"(barrier), "n"(N) : "memory"); }
 
 // PAGED: boxes of a page's keys; else boxes of 128 rows beside the queries
 template <int D, bool PAGED>
@@ -76,148 +161,161 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 {
     using S = ManyShape<D>;
     using Walk = AttnWalk<ManyCut>;
-    extern __shared__ unsigned char smem_dyn[];
-    __shared__ uint32_t s_tmem_base;
-    __shared__ volatile int s_abort;
-    __shared__ int s_last[2];
-    __shared__ __align__(8) uint64_t s_bars[10 + 2 * S::STAGES];
-    const uint32_t smem0 = (s2u(smem_dyn) + 1023u) & ~1023u, smem_kv = smem0 + 2 * S::TILE_BYTES, b0 = s2u(s_bars);
-    const ManyBars bar = {b0, b0 + 8, b0 + 16, b0 + 32, b0 + 48, b0 + 64, b0 + 80, b0 + 80 + 8 * S::STAGES};
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    extern __shared__ __align__(1024) unsigned char smem_many[];              // (no other shared memory: 227 KB are just enough)
+    ManyShared& sh = *reinterpret_cast<ManyShared*>(smem_many + (2 + S::STAGES) * S::TILE_BYTES);
+    const uint32_t smem0 = s2u(smem_many), smem_kv = smem0 + 2 * S::TILE_BYTES;
+    const uint32_t q_full = s2u(sh.q_full), s_full = s2u(sh.s_full), p_half = s2u(sh.p_half), p_full = s2u(sh.p_full), o_full = s2u(sh.o_full),
+                   o_empty = s2u(sh.o_empty), kv_full = s2u(sh.kv_full), kv_empty = s2u(sh.kv_empty), unit_full = s2u(sh.unit_full), unit_empty = s2u(sh.unit_empty);
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (smem0 & 1023u) {                                                       // (the swizzle counts on it; so does every tile's address)
+        if (threadIdx.x == 0) atomicExch(p.status, 50);
+        return;
+    }
     if (threadIdx.x == 0) {
-        s_abort = 0;
-        bar_init(bar.q_full, 64);
-        bar_init(bar.q_empty, 1);
+        sh.abort = 0;
         for (int t = 0; t < 2; ++t) {
-            bar_init(bar.s_full + 8 * t, 1);
-            bar_init(bar.p_full + 8 * t, 128);
-            bar_init(bar.o_full + 8 * t, 1);
-            bar_init(bar.o_empty + 8 * t, 128);
+            bar_init(q_full + 8 * t, 256);
+            bar_init(s_full + 8 * t, 1);
+            bar_init(p_half + 8 * t, 256);
+            bar_init(p_full + 8 * t, 256);
+            bar_init(o_full + 8 * t, 1);
+            bar_init(o_empty + 8 * t, 256);
         }
         for (int s = 0; s < S::STAGES; ++s) {
-            bar_init(bar.kv_full + 8 * s, 1);
-            bar_init(bar.kv_empty + 8 * s, 1);
+            bar_init(kv_full + 8 * s, 1);
+            bar_init(kv_empty + 8 * s, 2);
+        }
+        for (int i = 0; i < MANY_UNITS; ++i) {
+            bar_init(unit_full + 8 * i, 1);
+            bar_init(unit_empty + 8 * i, 19);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s2u(&s_tmem_base)), "r"(512) : "memory");
+    if (warp == 16) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s2u(&sh.tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = s_tmem_base;
+    const uint32_t tmem = (uint32_t)uniform((int)sh.tmem);
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const bool whole = !p.partial;
-    const AttnPlace place = attn_locate<ManyCut>(p, whole, reinterpret_cast<uint32_t*>(smem_dyn));
-    Walk u;
-    u.begin(p, place, whole);
-    // tiles of keys of row tile t of the unit: up to this one (none where it has no rows)
-    auto tiles_of = [&](int t) {
-        const int rows = attn_block_rows(u.r, p.group.d, u.block, MANY_ROWS) - 128 * t;
-        if (rows <= 0) return 0;
-        return attn_tiles(attn_seen(u.r, p.group.of(u.block * MANY_ROWS + 128 * t + min(rows, 128) - 1)), MANY_TILE);
+    const AttnPlace place = attn_locate<ManyCut>(p, whole, sh.locate, reinterpret_cast<uint32_t*>(smem_many));
+    // the units, for the warps that are told of them: the next one, or false behind the last
+    int unit_at = 0;
+    uint32_t unit_phase = 0;
+    auto next_unit = [&](ManyUnit& u) {
+        attn_spin(unit_full + 8 * unit_at, unit_phase, &sh.abort, p.status, 62);
+        if (sh.abort) return false;
+        u = sh.units[unit_at];
+        __syncwarp();
+        if (lane == 0) bar_arrive(unit_empty + 8 * unit_at);
+        if (++unit_at == MANY_UNITS) { unit_at = 0; unit_phase ^= 1u; }
+        return u.there != 0;
     };
+    ManyUnit u;
 
-    if (warp >= 8) {
+    if (warp >= 16) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(MANY_REGS_REST));
-        if (warp == 8) {
-            // ---- MMA issue
-            const uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);                 // bf16 x bf16 -> f32, both K-major
-            const uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);      // V: rows along K
+        if (warp < 18) {
+            // ---- MMA issue of tile t
+            const int t = warp - 16;
+            constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);             // bf16 x bf16 -> f32, both K-major
+            constexpr uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);      // V: rows along K
+            const uint32_t ts = tmem + 128 * t, to = tmem + 256 + 128 * t, mine = 8 * t;
+            const uint64_t a = smem_desc_sw128(smem0 + t * S::TILE_BYTES);
             int s = 0;
-            uint32_t kv_phase = 0, q_phase = 0, p_phase[2] = {0, 0}, oe_phase[2] = {1, 1};
+            uint32_t kv_phase = 0, q_phase = 0, p_phase = 0, oe_phase = 1;
             auto advance = [&] { if (++s == S::STAGES) { s = 0; kv_phase ^= 1u; } };
-            auto issue_s = [&](int t, int stage) {
-                if (lane == 0) {
-                    const uint64_t a = smem_desc_sw128(smem0 + t * S::TILE_BYTES), b = smem_desc_sw128(smem_kv + stage * S::TILE_BYTES);
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        const uint64_t off = (uint64_t)(((k >> 2) * S::HALF_BYTES + (k & 3) * 32) >> 4);
-                        tc_mma_f16_ss(tmem + 128 * t, a + off, b + off, idesc_s, k ? 1u : 0u);
-                    }
-                    tc_commit(bar.s_full + 8 * t);
+            while (next_unit(u)) {
+                const int first = u.first, end = u.end, e = t ? u.ends[1] : u.ends[0], keys = u.keys;
+                if (first < e) {
+                    attn_spin(q_full + mine, q_phase, &sh.abort, p.status, 51);
+                    q_phase ^= 1u;
                 }
-            };
-            for (; u.more(); u.step(p)) {
-                const int first = u.first(), end = u.end(), e[2] = {min(end, tiles_of(0)), min(end, tiles_of(1))};
-                attn_wait(bar.q_full, q_phase, &s_abort, p.status, 51);
-                q_phase ^= 1u;
-                attn_wait(bar.kv_full + 8 * s, kv_phase, &s_abort, p.status, 52);
-                tc_fence_after();
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-                    if (first < e[t]) issue_s(t, s);
-                if (lane == 0) {
-                    tc_commit(bar.kv_empty + 8 * s);
-                    if (first + 1 >= end) tc_commit(bar.q_empty);
-                }
-                advance();
-                for (int j = first; j < end; ++j) {
-                    const int v = s;
-                    attn_wait(bar.kv_full + 8 * v, kv_phase, &s_abort, p.status, 53);
-                    advance();
-                    const int left = u.r.keys - j * MANY_TILE;
-                    if (left < MANY_TILE) {
-                        // values behind the last key may be anything, and 0 * NaN is not 0
-                        const int rows = MANY_TILE - max(left, 0), from = max(left, 0);
-                        for (int i = lane; i < rows * 8 * S::HALVES; i += 32) {
-                            const int h = i / (rows * 8), at = i - h * rows * 8;
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(smem_kv + v * S::TILE_BYTES + h * S::HALF_BYTES + from * 128 + at * 16), "r"(0) : "memory");
+                // j: the keys whose scores are made; then (and before the next ones) the product with the values of those before
+                for (int j = first; j <= end; ++j) {
+                    if (j > first) {
+                        const int v = uniform(s);
+                        attn_spin(kv_full + 8 * v, kv_phase, &sh.abort, p.status, 53);
+                        advance();
+                        const int from = max(keys - (j - 1) * MANY_TILE, 0);
+                        if (from < MANY_TILE) {
+                            // values behind the last key may be anything, and 0 * NaN is not 0 (both tiles' warps write the same zeros)
+                            const int rows = MANY_TILE - from;
+                            for (int i = lane; i < rows * 8 * S::HALVES; i += 32) {
+                                const int h = i >= rows * 8 ? 1 : 0, at = i - h * rows * 8;
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(smem_kv + v * S::TILE_BYTES + h * S::HALF_BYTES + from * 128 + at * 16), "r"(0) : "memory");
+                            }
+                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                            __syncwarp();
                         }
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        if (j <= e) {
+                            const uint64_t b = smem_desc_sw128_mn(smem_kv + v * S::TILE_BYTES);
+                            const uint32_t go_on = j > first + 1 ? 1u : 0u;
+                            // (the first 32 keys of each team, then the others)
+                            auto product = [&](int part) {
+#pragma unroll
+                                for (int q = 0; q < 4; ++q) {
+                                    const int k = (q >> 1) * 4 + 2 * part + (q & 1);
+                                    tc_mma_f16_ts(to, ts + 8 * k, b + (uint64_t)((k * 16 * 128) >> 4), idesc_o, part || q ? 1u : go_on);
+                                }
+                            };
+                            if (j == first + 1) {
+                                attn_spin(o_empty + mine, oe_phase, &sh.abort, p.status, 54);
+                                oe_phase ^= 1u;
+                            }
+                            attn_spin(p_half + mine, p_phase, &sh.abort, p.status, 61);
+                            tc_fence_after();
+                            if (elect_one()) product(0);
+                            __syncwarp();
+                            attn_spin(p_full + mine, p_phase, &sh.abort, p.status, 55);
+                            p_phase ^= 1u;
+                            tc_fence_after();
+                            if (elect_one()) {
+                                product(1);
+                                if (j == e) tc_commit(o_full + mine);
+                                tc_commit(kv_empty + 8 * v);
+                            }
+                            __syncwarp();
+                        } else if (elect_one()) tc_commit(kv_empty + 8 * v);
+                    }
+                    if (j < end) {
+                        const int k0 = uniform(s);
+                        attn_spin(kv_full + 8 * k0, kv_phase, &sh.abort, p.status, 56);
+                        advance();
+                        tc_fence_after();
+                        const uint64_t b = smem_desc_sw128(smem_kv + k0 * S::TILE_BYTES);
+                        if (elect_one()) {
+                            if (j < e) {
+#pragma unroll
+                                for (int k = 0; k < D / 16; ++k) {
+                                    const uint64_t off = (uint64_t)(((k >> 2) * S::HALF_BYTES + (k & 3) * 32) >> 4);
+                                    tc_mma_f16_ss(ts, a + off, b + off, idesc_s, k ? 1u : 0u);
+                                }
+                                tc_commit(s_full + mine);
+                            }
+                            tc_commit(kv_empty + 8 * k0);
+                        }
                         __syncwarp();
                     }
-#pragma unroll
-                    for (int t = 0; t < 2; ++t)
-                        if (j < e[t]) {
-                            if (j == first) {
-                                attn_wait(bar.o_empty + 8 * t, oe_phase[t], &s_abort, p.status, 54);
-                                oe_phase[t] ^= 1u;
-                            }
-                            attn_wait(bar.p_full + 8 * t, p_phase[t], &s_abort, p.status, 55);
-                            p_phase[t] ^= 1u;
-                            tc_fence_after();
-                            if (lane == 0) {
-                                const uint64_t b = smem_desc_sw128_mn(smem_kv + v * S::TILE_BYTES);
-#pragma unroll
-                                for (int k = 0; k < MANY_TILE / 16; ++k)
-                                    tc_mma_f16_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * k, b + (uint64_t)((k * 16 * 128) >> 4), idesc_o, j > first || k ? 1u : 0u);
-                                if (j + 1 == e[t]) tc_commit(bar.o_full + 8 * t);
-                            }
-                            if (j + 1 < e[t]) {
-                                attn_wait(bar.kv_full + 8 * s, kv_phase, &s_abort, p.status, 56);
-                                tc_fence_after();
-                                issue_s(t, s);
-                            }
-                        }
-                    if (lane == 0) {
-                        tc_commit(bar.kv_empty + 8 * v);
-                        if (j + 1 < end) {
-                            tc_commit(bar.kv_empty + 8 * s);
-                            if (j + 2 >= end) tc_commit(bar.q_empty);
-                        }
-                    }
-                    if (j + 1 < end) advance();
                 }
             }
-        } else if (warp == 9) {
+        } else if (warp == 18) {
             // ---- keys and values: a lane per box and half
             int s = 0;
             uint32_t phase = 1;
             const int shift = PAGED ? min(p.page_shift, 7) : 7, boxes = MANY_TILE >> shift;
             const int h = lane % S::HALVES, box = lane / S::HALVES;
             const uint32_t box_bytes = 128u << shift;                          // of one half
-            for (; u.more(); u.step(p)) {
+            while (next_unit(u)) {
                 const int32_t* row = PAGED ? p.table + u.request * p.width : nullptr;
-                const int end = u.end();
-                for (int j = u.first(); j < end; ++j) {
+                for (int j = u.first; j < u.end; ++j) {
                     const int key = j * MANY_TILE + (box << shift);
-                    const bool mine = box < boxes && key < u.r.keys;
-                    // at least one box is asked for, so that the barrier has something to count: of a unit without keys the first
-                    const int there = (max(min(u.r.keys, (j + 1) * MANY_TILE) - j * MANY_TILE, 0) + (1 << shift) - 1) >> shift;
+                    const bool mine = box < boxes && key < u.keys;
+                    const int there = (max(min(u.keys - j * MANY_TILE, MANY_TILE), 0) + (1 << shift) - 1) >> shift;
                     int page = 0;
                     if (PAGED && mine) {
                         page = row[key >> p.page_shift];
@@ -225,230 +323,277 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     }
 #pragma unroll
                     for (int what = 0; what < 2; ++what) {
-                        attn_wait(bar.kv_empty + 8 * s, phase, &s_abort, p.status, 57);
-                        if (lane == 0) bar_expect_tx(bar.kv_full + 8 * s, there * S::HALVES * box_bytes);
+                        attn_wait(kv_empty + 8 * s, phase, &sh.abort, p.status, 57);
+                        if (lane == 0) bar_expect_tx(kv_full + 8 * s, there * S::HALVES * box_bytes);
                         __syncwarp();
                         if (mine) {
                             const uint32_t dst = smem_kv + s * S::TILE_BYTES + h * S::HALF_BYTES + box * box_bytes;
                             const CUtensorMap* map = what ? &map_v : &map_k;
-                            if (PAGED) tma_load_4d(dst, map, 0, key & ((1 << p.page_shift) - 1), h, page * p.kv_heads + u.head, bar.kv_full + 8 * s);
-                            else tma_load_4d(dst, map, 0, u.r.first + key, h, u.head, bar.kv_full + 8 * s);
+                            if (PAGED) tma_load_4d(dst, map, 0, key & ((1 << p.page_shift) - 1), h, page * p.kv_heads + u.head, kv_full + 8 * s);
+                            else tma_load_4d(dst, map, 0, u.first_row + key, h, u.head, kv_full + 8 * s);
                         }
+                        __syncwarp();
                         if (++s == S::STAGES) { s = 0; phase ^= 1u; }
                     }
                 }
             }
-        } else if (warp >= 10) {
-            // ---- rows of Q: 16 bytes at a time into the swizzled tiles
+        } else {
+            // ---- the units
+            Walk w;
+            w.begin(p, place, whole);
             uint32_t phase = 1;
-            const int tid = threadIdx.x - 320;
-            constexpr int CH = D / 8, STEP = 64 / CH;
-            const int c = tid % CH, r0 = tid / CH;
-            for (; u.more(); u.step(p)) {
-                attn_wait(bar.q_empty, phase, &s_abort, p.status, 58);
-                phase ^= 1u;
-                const int rows = attn_block_rows(u.r, p.group.d, u.block, MANY_ROWS);
-                // thread: chunk c of every fourth (or eighth) row; token and head of the row go on with it
-                const int all = rows <= 128 ? 128 : 256, group = p.group.d;
-                const int tok_step = p.group.of(STEP), head_step = STEP - tok_step * group;
-                int tok = p.group.of(u.block * MANY_ROWS + r0), head = u.block * MANY_ROWS + r0 - tok * group;
-#pragma unroll 4
-                for (int r = r0; r < all; r += STEP) {
-                    const __nv_bfloat16* src = p.q + (int64_t)(u.r.first + (r < rows ? tok : 0)) * p.q_stride + (u.head * group + head) * D + c * 8;
-                    const uint32_t dst = smem0 + (r >> 7) * S::TILE_BYTES + (c >> 3) * S::HALF_BYTES + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4);
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(r < rows ? 16 : 0) : "memory");
-                    tok += tok_step;
-                    head += head_step;
-                    if (head >= group) { head -= group; ++tok; }
+            int at = 0;
+            for (bool there = true; there && !sh.abort;) {
+                there = w.more();
+                attn_wait(unit_empty + 8 * at, phase, &sh.abort, p.status, 63);
+                if (lane == 0) {
+                    ManyUnit n = {};
+                    n.there = there;
+                    if (there) {
+                        n.first = w.first(); n.end = w.end();
+                        n.keys = w.r.keys; n.new_rows = w.r.rows; n.first_row = w.r.first;
+                        n.row0 = w.block * MANY_ROWS; n.rows = attn_block_rows(w.r, p.group.d, w.block, MANY_ROWS);
+                        n.head = w.head; n.request = w.request;
+                        n.cut = w.cut();
+                        if (n.cut) { n.opener = w.opener(); n.closer = w.closer(); }
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) {
+                            const int rows = min(n.rows - 128 * t, 128);
+                            n.ends[t] = rows <= 0 ? 0 : min(n.end, attn_tiles(attn_seen(w.r, p.group.of(n.row0 + 128 * t + rows - 1)), MANY_TILE));
+                        }
+                    }
+                    sh.units[at] = n;
+                    bar_arrive(unit_full + 8 * at);
                 }
-                asm volatile("cp.async.wait_all;" ::: "memory");
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                bar_arrive(bar.q_full);
+                __syncwarp();
+                if (++at == MANY_UNITS) { at = 0; phase ^= 1u; }
+                if (there) w.step(p);
             }
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(MANY_REGS_WORK));
-        // ---- a thread per row
-        const int t = warp >> 2, row = threadIdx.x & 127;                      // (a warp of a team reaches the lanes 32 (warp % 4) ..)
-        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t ts = tmem + lanes + 128 * t, to = tmem + lanes + 256 + 128 * t;
+        // ---- a thread per row and half of a tile's keys (and, at the end, half of the columns of O); a warp reaches the lanes 32 (warp % 4) ..
+        const int t = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3, row = quarter * 32 + lane;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        const uint32_t ts = tmem + lanes + 128 * t, to = tmem + lanes + 256 + 128 * t + half * (D / 2);
+        const int pair = 1 + 4 * t + quarter;                                  // barrier of the two warps with these rows
         uint32_t s_phase = 0, o_phase = 0;
-            for (; u.more(); u.step(p)) {
-                const int rows = attn_block_rows(u.r, p.group.d, u.block, MANY_ROWS) - 128 * t;
-                if (rows <= 0) continue;
-                const int at = u.block * MANY_ROWS + 128 * t + min(row, rows - 1), tok = p.group.of(at);
-                const int seen = attn_seen(u.r, tok), seen_all = attn_seen(u.r, p.group.of(u.block * MANY_ROWS + 128 * t));
-                const int first = u.first(), end = min(u.end(), tiles_of(t));
-                float m = -INFINITY, l = 0.f;                                  // m in units of the scores as they come
-                for (int j = first; j < end; ++j) {
-                    attn_wait(bar.s_full + 8 * t, s_phase, &s_abort, p.status, 59);
-                    s_phase ^= 1u;
-                    tc_fence_after();
-                    // S is read twice, for the maximum and for the weights: 128 registers less, for 128 cycles of tensor memory
-                    const bool ragged = (j + 1) * MANY_TILE > seen_all;
-                    const int left = seen - j * MANY_TILE;
-                    auto hide = [&](uint32_t (&x)[32], int c) {
-                        if (ragged) {
+        // The next unit's rows of Q, 16 bytes at a time into the swizzled tile: chunk c of every sixteenth (or thirty-second) row; token and head of
+        // the row go on with it.  (The tile is free: this thread has seen the last S that was made of it.)
+        auto fetch_q = [&] {
+            constexpr int CH = D / 8, STEP = 256 / CH;
+            attn_spin(unit_full + 8 * unit_at, unit_phase, &sh.abort, p.status, 64);
+            const ManyUnit& n = sh.units[unit_at];
+            const int rows = n.rows - 128 * t;
+            if (!n.there || n.first >= n.ends[t]) return false;
+            const int c = threadIdx.x % CH, r0 = (threadIdx.x & 255) / CH, group = p.group.d;
+            const int tok_step = p.group.of(STEP), head_step = STEP - tok_step * group;
+            int tok = p.group.of(n.row0 + 128 * t + r0), head = n.row0 + 128 * t + r0 - tok * group;
+            const __nv_bfloat16* base = p.q + (int64_t)n.first_row * p.q_stride + (int64_t)n.head * group * D + c * 8;
 #pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (32 * c + i >= left) x[i] = 0xFF800000u;
-                        }
-                    };
-                    float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            for (int r = r0; r < 128; r += STEP) {
+                const __nv_bfloat16* src = base + (r < rows ? tok * p.q_stride + head * D : 0);
+                const uint32_t dst = smem0 + t * S::TILE_BYTES + (c >> 3) * S::HALF_BYTES + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(r < rows ? 16 : 0) : "memory");
+                tok += tok_step;
+                head += head_step;
+                if (head >= group) { head -= group; ++tok; }
+            }
+            return true;
+        };
+        auto q_there = [&] {
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            bar_arrive(q_full + 8 * t);
+        };
+        if (fetch_q()) q_there();
+        while (next_unit(u)) {
+            const int rows = u.rows - 128 * t;
+            if (rows <= 0) {
+                if (fetch_q()) q_there();
+                continue;
+            }
+            const int at = u.row0 + 128 * t + min(row, rows - 1), tok = p.group.of(at);
+            const int first = u.first, end = t ? u.ends[1] : u.ends[0];
+            // key from which on the row sees none, and the first row's: counted from this thread's keys of the tile
+            const int origin = u.keys - u.new_rows + 1 - first * MANY_TILE - 64 * half;
+            int left = origin + tok, left_all = origin + p.group.of(u.row0 + 128 * t);
+            float m = -INFINITY, l = 0.f;                                      // m in units of the scores as they come; l of this half
+            for (int j = first; j < end; ++j, left -= MANY_TILE, left_all -= MANY_TILE) {
+                attn_spin(s_full + 8 * t, s_phase, &sh.abort, p.status, 59);
+                s_phase ^= 1u;
+                tc_fence_after();
+                uint32_t x[2][32];
 #pragma unroll
-                    for (int c = 0; c < 4; c += 2) {
-                        uint32_t x[2][32];
-                        tc_ld32(ts + 32 * c, x[0]);
-                        tc_ld32(ts + 32 * c + 32, x[1]);
-                        tc_ld_wait();
+                for (int c = 0; c < 2; ++c) tc_ld32(ts + 64 * half + 32 * c, x[c]);
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            hide(x[h], c + h);
+                for (int c = 0; c < 2; ++c) tc_ld_wait_for(x[c]);
+                const bool ragged = left_all < 64;
+                if (ragged) {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) y[i & 3] = fmaxf(y[i & 3], __uint_as_float(x[h][i]));
-                        }
-                    }
-                    const float top = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
-                    if (j == first) m = top;
-                    else if (__any_sync(~0u, (top - m) * p.scale_log2 > MANY_LATE)) {
-                        // (this S came behind the last product into O)
-                        const float m2 = fmaxf(m, top), f = m2 == -INFINITY ? 1.f : ex2((m - m2) * p.scale_log2);
-                        m = m2;
-                        l *= f;
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (32 * c + i >= left) x[c][i] = 0xFF800000u;
+                }
+                float y[2];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    y[c] = max_nan(__uint_as_float(x[c][0]), __uint_as_float(x[c][1]), __uint_as_float(x[c][2]));
+#pragma unroll
+                    for (int i = 3; i < 31; i += 2) y[c] = max_nan(y[c], __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]));
+                    y[c] = max_nan(y[c], y[c], __uint_as_float(x[c][31]));
+                }
+                float top = max_nan(y[0], y[1], y[1]);
+                // (the other team's reading of the last one is behind its arrival at p_full, which this S waited for)
+                sh.top[t][half][row] = top;
+                team_sync<64>(pair);
+                top = max_nan(top, sh.top[t][half ^ 1][row], -INFINITY);
+                if (top == INFINITY) top = NAN;                                // (what inf - inf would make of the row)
+                if (j == first) m = top;
+                else if (__any_sync(~0u, !((top - m) * p.scale_log2 <= MANY_LATE))) {
+                    // (this S came behind the last product into O)
+                    const float m2 = max_nan(m, top, top), f = m2 == -INFINITY ? 1.f : ex2((m - m2) * p.scale_log2);
+                    m = m2;
+                    l *= f;
 #pragma unroll 1
-                        for (int c = 0; c < D / 32; ++c) {
-                            uint32_t o[32];
-                            tc_ld32(to + 32 * c, o);
-                            tc_ld_wait();
+                    for (int c = 0; c < D / 2; c += 16) {
+                        uint32_t o[16];
+                        tc_ld16(to + c, o);
+                        tc_ld_wait_for(o);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                            tc_st16(to + 32 * c, o);
-                            tc_st16(to + 32 * c + 16, o + 16);
-                        }
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        tc_st16(to + c, o);
                     }
-                    const float base = m == -INFINITY ? 0.f : m * p.scale_log2;
-                    float sum[2] = {0.f, 0.f};
-                    // (the weights of 32 keys take the place of 16 scores that have been read: the next 32 are, before they are overwritten)
-                    uint32_t x[2][32];
-                    tc_ld32(ts, x[0]);
-                    tc_ld_wait();
+                }
+                const float base = m == -INFINITY ? 0.f : m * p.scale_log2;
+                const uint64_t scale2 = pair_of(p.scale_log2, p.scale_log2), base2 = pair_of(-base, -base);
+                uint64_t sum[2] = {0, 0};
+                auto weights = [&](auto with_powers) {
+                    constexpr bool POWERS = decltype(with_powers)::value;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        if (c < 3) tc_ld32(ts + 32 * (c + 1), x[(c + 1) & 1]);
-                        hide(x[c & 1], c);
+                    for (int c = 0; c < 2; ++c) {
                         uint32_t w[16];
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            const float e0 = ex2(fmaf(__uint_as_float(x[c & 1][2 * i]), p.scale_log2, -base)), e1 = ex2(fmaf(__uint_as_float(x[c & 1][2 * i + 1]), p.scale_log2, -base));
-                            sum[0] += e0;
-                            sum[1] += e1;
+                            const uint64_t a = fma2(pair_of(x[c][2 * i], x[c][2 * i + 1]), scale2, base2);
+                            const uint64_t e = POWERS && i % MANY_POWERS == MANY_POWERS - 1 ? power2(a) : ex2_pair(a);
+                            sum[i & 1] = add2(sum[i & 1], e);
                             // bf16 is what the tensor cores take beside bf16 values; the sum keeps the weights as they were
-                            w[i] = pack_bf16(e0, e1);
+                            w[i] = bf16_pair(e);
                         }
-                        if (c < 3) tc_ld_wait();
-                        tc_st16(ts + 16 * c, w);
-                    }
-                    l += sum[0] + sum[1];
-                    tc_st_wait();
-                    tc_fence_before();
-                    bar_arrive(bar.p_full + 8 * t);
-                }
-                // ---- the unit's end: O, unscaled
-                const bool some = first < end;
-                if (some) {
-                    attn_wait(bar.o_full + 8 * t, o_phase, &s_abort, p.status, 60);
-                    o_phase ^= 1u;
-                    tc_fence_after();
-                }
-                const bool cut = u.cut();
-                const int opener = cut ? u.opener() : 0, closer = cut ? u.closer() : 0;
-                const int64_t to_row = ((int64_t)(u.r.first + tok) * p.q_heads + (u.head - tok) * (int)p.group.d + at) * D;
-                auto store16 = [&](int c, const float* v) {                    // 16 columns from c on
-                    if (row >= rows) return;
-                    if (p.out_f32) {
-                        float* out = static_cast<float*>(p.out) + to_row + c;
-#pragma unroll
-                        for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(out + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-                    } else {
-                        uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(p.out) + to_row + c);
-                        uint32_t w[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-                        *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
-                        *reinterpret_cast<uint4*>(out + 4) = make_uint4(w[4], w[5], w[6], w[7]);
+                        tc_st16(ts + 32 * half + 16 * c, w);
+                        tc_st_wait();
+                        tc_fence_before();
+                        bar_arrive((c ? p_full : p_half) + 8 * t);
                     }
                 };
-                // a piece: [column / 4][row][4], so that a warp's threads lie beside each other; then maxima, sums
-                auto slot = [&](int cta) { return p.partial + (int64_t)(2 * cta + (cta == opener ? 1 : 0)) * S::PIECE; };
-                const int mine = 128 * t + row;
-                const float inv = l == 0.f ? 0.f : 1.f / l;
-                if (some) {
+                if (ragged) weights(std::false_type{});
+                else weights(std::true_type{});
+                const uint64_t both = add2(sum[0], sum[1]);
+                l += __uint_as_float((uint32_t)both) + __uint_as_float((uint32_t)(both >> 32));
+            }
+            // ---- the unit's end: O, unscaled, and the sums of both halves
+            const bool some = first < end, fetched = fetch_q();
+            if (some) {
+                attn_spin(o_full + 8 * t, o_phase, &sh.abort, p.status, 60);
+                o_phase ^= 1u;
+                tc_fence_after();
+            }
+            if (fetched) q_there();
+            sh.top[t][half][row] = l;                                          // (behind o_full, so behind the other team's last reading, too)
+            team_sync<64>(pair);
+            l += sh.top[t][half ^ 1][row];
+            team_sync<64>(pair);                                               // (the next unit's maxima go there)
+            const bool cut = u.cut;
+            const int opener = u.opener, closer = u.closer;
+            const int64_t to_row = ((int64_t)(u.first_row + tok) * p.q_heads + (u.head - tok) * (int)p.group.d + at) * D + half * (D / 2);
+            auto store16 = [&](int c, const float* v) {                        // 16 columns from c on, of this thread's half
+                if (row >= rows) return;
+                if (p.out_f32) {
+                    float* out = static_cast<float*>(p.out) + to_row + c;
 #pragma unroll
-                    for (int c = 0; c < D; c += 16) {
-                        uint32_t o[16];
-                        tc_ld16(to + c, o);
-                        tc_ld_wait();
-                        float v[16];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(o[i]) * (cut ? 1.f : inv);
-                        if (!cut) store16(c, v);
-                        else {
-                            float4* to4 = reinterpret_cast<float4*>(slot(blockIdx.x)) + (c >> 2) * MANY_ROWS + mine;
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) to4[i * MANY_ROWS] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-                        }
-                    }
-                    tc_fence_before();
-                    bar_arrive(bar.o_empty + 8 * t);
+                    for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(out + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                } else {
+                    uint4* out = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + to_row + c);
+                    out[0] = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+                    out[1] = make_uint4(pack_bf16(v[8], v[9]), pack_bf16(v[10], v[11]), pack_bf16(v[12], v[13]), pack_bf16(v[14], v[15]));
                 }
-                if (cut) {
+            };
+            // a piece: [column / 4][row][4], so that a warp's threads lie beside each other; then maxima, sums
+            const int mine = 128 * t + row, col4 = half * (D / 8);
+            auto slot = [&](int cta) { return p.partial + (int64_t)(2 * cta + (cta == opener ? 1 : 0)) * S::PIECE; };
+            if (some) {
+                const float scale = cut ? 1.f : l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+                for (int c = 0; c < D / 2; c += 16) {
+                    uint32_t o[16];
+                    tc_ld16(to + c, o);
+                    tc_ld_wait_for(o);
+                    float v[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(o[i]) * scale;
+                    if (!cut) store16(c, v);
+                    else {
+                        float4* to4 = reinterpret_cast<float4*>(slot(blockIdx.x)) + (col4 + (c >> 2)) * MANY_ROWS + mine;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) to4[i * MANY_ROWS] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                    }
+                }
+                tc_fence_before();
+                bar_arrive(o_empty + 8 * t);
+            }
+            if (cut) {
+                if (half == 0) {
                     float* head = slot(blockIdx.x) + MANY_ROWS * D;
                     head[mine] = m == -INFINITY ? m : m * p.scale_log2;
                     head[MANY_ROWS + mine] = l;
+                }
+                __threadfence();
+                team_sync<256>(9 + t);
+                if ((threadIdx.x & 255) == 0) {
+                    const uint32_t before = atomicAdd(p.arrived + 2 * opener + t, 1u);
+                    sh.last[t] = before == (uint32_t)(closer - opener);
+                    if (sh.last[t]) p.arrived[2 * opener + t] = 0;
                     __threadfence();
-                    team_sync<128>(t);
-                    if (row == 0) {
-                        const uint32_t before = atomicAdd(p.arrived + 2 * opener + t, 1u);
-                        s_last[t] = before == (uint32_t)(closer - opener);
-                        if (s_last[t]) p.arrived[2 * opener + t] = 0;
-                        __threadfence();
+                }
+                team_sync<256>(9 + t);
+                if (sh.last[t]) {
+                    float top = -INFINITY, sum = 0.f;
+                    for (int cta = opener; cta <= closer; ++cta) top = max_nan(top, __ldcg(slot(cta) + MANY_ROWS * D + mine), -INFINITY);
+                    for (int cta = opener; cta <= closer; ++cta) {
+                        const float mm = __ldcg(slot(cta) + MANY_ROWS * D + mine);
+                        if (mm != -INFINITY) sum = fmaf(exp2f(mm - top), __ldcg(slot(cta) + MANY_ROWS * D + MANY_ROWS + mine), sum);
                     }
-                    team_sync<128>(t);
-                    if (s_last[t]) {
-                        float top = -INFINITY, sum = 0.f;
-                        for (int cta = opener; cta <= closer; ++cta) top = fmaxf(top, __ldcg(slot(cta) + MANY_ROWS * D + mine));
+                    const float scale = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll 1
+                    for (int c = 0; c < D / 2; c += 16) {
+                        float v[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) v[i] = 0.f;
                         for (int cta = opener; cta <= closer; ++cta) {
                             const float mm = __ldcg(slot(cta) + MANY_ROWS * D + mine);
-                            if (mm != -INFINITY) sum = fmaf(exp2f(mm - top), __ldcg(slot(cta) + MANY_ROWS * D + MANY_ROWS + mine), sum);
-                        }
-                        const float scale = sum == 0.f ? 0.f : 1.f / sum;
-                        for (int c = 0; c < D; c += 16) {
-                            float v[16];
+                            if (mm == -INFINITY) continue;                     // (nothing of this piece is seen: its o need not be there)
+                            const float f = exp2f(mm - top) * scale;
+                            const float4* from = reinterpret_cast<const float4*>(slot(cta)) + (col4 + (c >> 2)) * MANY_ROWS + mine;
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) v[i] = 0.f;
-                            for (int cta = opener; cta <= closer; ++cta) {
-                                const float mm = __ldcg(slot(cta) + MANY_ROWS * D + mine);
-                                if (mm == -INFINITY) continue;                 // (nothing of this piece is seen: its o was not written)
-                                const float f = exp2f(mm - top) * scale;
-                                const float4* from = reinterpret_cast<const float4*>(slot(cta)) + (c >> 2) * MANY_ROWS + mine;
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    const float4 a = __ldcg(from + i * MANY_ROWS);
-                                    v[4 * i] = fmaf(a.x, f, v[4 * i]); v[4 * i + 1] = fmaf(a.y, f, v[4 * i + 1]);
-                                    v[4 * i + 2] = fmaf(a.z, f, v[4 * i + 2]); v[4 * i + 3] = fmaf(a.w, f, v[4 * i + 3]);
-                                }
+                            for (int i = 0; i < 4; ++i) {
+                                const float4 a = __ldcg(from + i * MANY_ROWS);
+                                v[4 * i] = fmaf(a.x, f, v[4 * i]); v[4 * i + 1] = fmaf(a.y, f, v[4 * i + 1]);
+                                v[4 * i + 2] = fmaf(a.z, f, v[4 * i + 2]); v[4 * i + 3] = fmaf(a.w, f, v[4 * i + 3]);
                             }
-                            store16(c, v);
                         }
+                        store16(c, v);
                     }
-                    team_sync<128>(t);                                         // (s_last is the next unit's then)
                 }
+                team_sync<256>(9 + t);                                         // (sh.last is the next unit's then)
             }
+        }
     }
     tc_fence_before();
     __syncthreads();
-    settle_after_timeout(s_abort);
-    if (warp == 8) {
+    settle_after_timeout(sh.abort);
+    if (warp == 16) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
