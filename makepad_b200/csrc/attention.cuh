@@ -35,8 +35,10 @@ struct AttnParams {
     float scale_log2;                       // scale / ln 2: the weights are powers of two
     void* out;
     int out_f32;
-    float* partial;                         // pieces of cut units; null: units stay whole
-    uint32_t* arrived;                      // per CTA: pieces of the unit that it opened
+    float* partial;                         // pieces of cut units, two per run; null: units stay whole
+    uint32_t* arrived;                      // per run: pieces of the unit that it opened
+    int most_parts;                         // of attn_parts, for which there is room
+    int64_t kv_bytes;                       // of a key and its value in all heads
     int* status;
 };
 
@@ -47,135 +49,94 @@ __device__ __forceinline__ AttnRequest attn_request(const AttnParams& p, int i)
     return attn_request(p.starts[i], p.starts[i + 1], p.tokens, p.lens != nullptr, p.lens ? p.lens[i] : 0, p.width << p.page_shift);
 }
 
-// a CTA's place in the order of all tiles
-struct AttnPlace {
-    int64_t total, unit;                    // all tiles; first tile of the unit
-    int block, request, head;
-};
-
-// How a kernel cuts its work: rows of a block, keys of a tile, what a unit costs beside its tiles, and whether a warp (of WARPS) adds up
-// a request's blocks (many of them), while there are few requests
-template <int ROWS_, int TILE_, int EXTRA_, int WARPS_>
+// How a kernel cuts its work: rows of a block, keys of a tile, what a unit costs beside its tiles, and whether a request may have many blocks
+template <int ROWS_, int TILE_, int EXTRA_, bool MANY_>
 struct AttnCut {
-    static constexpr int ROWS = ROWS_, TILE = TILE_, EXTRA = EXTRA_, WARPS = WARPS_;
+    static constexpr int ROWS = ROWS_, TILE = TILE_, EXTRA = EXTRA_;
+    static constexpr bool MANY = MANY_;
 };
 template <class Cut>
 __device__ __forceinline__ int attn_unit_cost(const AttnParams& p, const AttnRequest& r, int b, bool whole)
 {
     return whole ? 1 : attn_block_tiles(r, p.group, b, Cut::ROWS, Cut::TILE) + Cut::EXTRA;
 }
-
-struct AttnShared {
-    long long sums[32], total, before;
-    AttnPlace place;
-    int request;
-};
-// Where the CTA's run begins: every CTA adds up all requests.  By all threads, with barriers in it; `room` is shared memory of 4 bytes per thread.
+// tiles of a request in one head, by a warp
 template <class Cut>
-__device__ __forceinline__ AttnPlace attn_locate(const AttnParams& p, bool whole, AttnShared& sh, uint32_t* room)
+__device__ __forceinline__ uint32_t attn_request_cost(const AttnParams& p, const AttnRequest& r, bool whole)
 {
-    const int threads = blockDim.x, warps = threads >> 5, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const bool by_warps = Cut::WARPS && p.n <= threads;
-    const int per = (p.n + threads - 1) / threads, i0 = min(p.n, (int)threadIdx.x * per), i1 = min(p.n, i0 + per);
-    long long mine = 0;
+    const int blocks = attn_blocks(r, p.group.d, Cut::ROWS);
+    uint32_t sum = 0;
+    for (int b = threadIdx.x & 31; b < blocks; b += 32) sum += attn_unit_cost<Cut>(p, r, b, whole);
+    return __reduce_add_sync(~0u, sum);
+}
+
+constexpr int ATTN_ENTRIES = 160;
+struct AttnShared {
+    uint32_t cost[ATTN_ENTRIES];            // tiles of a head, of `per` requests each
+    long long total[5], keys[5];            // of 32 entries each
+};
+struct AttnTotals {
+    int64_t total;                          // tiles, of all heads
+    int per, runs;                          // requests of an entry; runs of all CTAs
+    bool whole;
+};
+// What there is to do: every CTA adds up all requests.  By all threads (at least ATTN_ENTRIES), with barriers in it.
+template <class Cut>
+__device__ __forceinline__ AttnTotals attn_totals(const AttnParams& p, AttnShared& sh)
+{
+    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    AttnTotals t;
+    t.whole = !p.partial;
+    t.per = (p.n + ATTN_ENTRIES - 1) / ATTN_ENTRIES;
+    long long keys = 0;
+    uint32_t cost = 0;
+    const bool by_warps = Cut::MANY && t.per == 1;
+    if ((int)threadIdx.x < ATTN_ENTRIES) {
+        const int i0 = min(p.n, (int)threadIdx.x * t.per), i1 = min(p.n, i0 + t.per);
+        for (int i = i0; i < i1; ++i) {
+            const AttnRequest r = attn_request(p, i);
+            keys += r.keys;
+            const int blocks = by_warps ? 0 : attn_blocks(r, p.group.d, Cut::ROWS);
+            for (int b = 0; b < blocks; ++b) cost += attn_unit_cost<Cut>(p, r, b, t.whole);
+        }
+        if (!by_warps) sh.cost[threadIdx.x] = cost;
+    }
     if (by_warps) {
         // the warp's requests, a lane each, then one after the other with a lane per block
         AttnRequest all = {};
         if (warp + warps * lane < p.n) all = attn_request(p, warp + warps * lane);
-        for (int k = 0; warp + warps * k < p.n; ++k) {
+        for (int k = 0; warp + warps * k < ATTN_ENTRIES; ++k) {
             AttnRequest r;
             r.first = __shfl_sync(~0u, all.first, k); r.rows = __shfl_sync(~0u, all.rows, k); r.keys = __shfl_sync(~0u, all.keys, k);
-            const int blocks = attn_blocks(r, p.group.d, Cut::ROWS);
-            uint32_t sum = 0;
-            for (int b = lane; b < blocks; b += 32) sum += attn_unit_cost<Cut>(p, r, b, whole);
-            sum = __reduce_add_sync(~0u, sum);
-            if (lane == 0) room[warp + warps * k] = sum;
-        }
-        __syncthreads();
-        if ((int)threadIdx.x < p.n) mine = room[threadIdx.x];
-    } else {
-        for (int i = i0; i < i1; ++i) {
-            const AttnRequest r = attn_request(p, i);
-            const int blocks = attn_blocks(r, p.group.d, Cut::ROWS);
-            for (int b = 0; b < blocks; ++b) mine += attn_unit_cost<Cut>(p, r, b, whole);
+            const uint32_t sum = attn_request_cost<Cut>(p, r, t.whole);
+            if (lane == 0) sh.cost[warp + warps * k] = sum;
         }
     }
-    mine *= p.kv_heads;
-    long long run = mine;
+    __syncthreads();
+    if (warp < ATTN_ENTRIES / 32) {
+        long long sum = sh.cost[threadIdx.x];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long up = __shfl_up_sync(~0u, run, o);
-        if (lane >= o) run += up;
-    }
-    if (lane == 31) sh.sums[warp] = run;
-    if (threadIdx.x == 0) sh.request = -1;
-    __syncthreads();
-    long long before = run - mine, total = 0;
-    for (int w = 0; w < warps; ++w) {
-        if (w < warp) before += sh.sums[w];
-        total += sh.sums[w];
-    }
-    if (threadIdx.x == 0) sh.total = total;
-    const int64_t ctas = min((int64_t)gridDim.x, (int64_t)total), lo = blockIdx.x < ctas ? attn_run(blockIdx.x, total, ctas) : total;
-    if (mine && before <= lo && lo < before + mine) {
-        if (by_warps) {
-            sh.request = threadIdx.x;
-            sh.before = before;
-        } else {
-            int64_t at = before;
-            for (int i = i0; i < i1; ++i) {
-                const AttnRequest r = attn_request(p, i);
-                const int blocks = attn_blocks(r, p.group.d, Cut::ROWS);
-                for (int b = 0; b < blocks; ++b) {
-                    const int cost = attn_unit_cost<Cut>(p, r, b, whole);
-                    const int64_t all = (int64_t)cost * p.kv_heads;
-                    if (lo < at + all) {
-                        const int head = (int)(lo - at) / cost;
-                        sh.place = AttnPlace{0, at + (int64_t)head * cost, b, i, head};
-                        b = blocks;
-                        i = i1;
-                    }
-                    at += all;
-                }
-            }
+        for (int o = 16; o; o >>= 1) {
+            sum += __shfl_xor_sync(~0u, sum, o);
+            keys += __shfl_xor_sync(~0u, keys, o);
         }
+        if (lane == 0) { sh.total[warp] = sum; sh.keys[warp] = keys; }
     }
     __syncthreads();
-    if (by_warps && sh.request >= 0 && warp == 0) {
-        const AttnRequest r = attn_request(p, sh.request);
-        const int blocks = attn_blocks(r, p.group.d, Cut::ROWS);
-        long long at = sh.before;
-        for (int b0 = 0; b0 < blocks; b0 += 32) {
-            const int cost = b0 + lane < blocks ? attn_unit_cost<Cut>(p, r, b0 + lane, whole) : 0;
-            long long sum = (long long)cost * p.kv_heads;
-            const long long own = sum;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long up = __shfl_up_sync(~0u, sum, o);
-                if (lane >= o) sum += up;
-            }
-            const long long from = at + sum - own;
-            if (own && from <= lo && lo < from + own) {
-                const int head = (int)(lo - from) / cost;
-                sh.place = AttnPlace{0, from + (long long)head * cost, b0 + lane, sh.request, head};
-            }
-            at += __shfl_sync(~0u, sum, 31);
-            if (at > lo) break;
-        }
-    }
-    __syncthreads();
-    AttnPlace place = sh.place;
-    place.total = sh.total;
-    return place;
+    t.total = keys = 0;
+    for (int w = 0; w < ATTN_ENTRIES / 32; ++w) { t.total += sh.total[w]; keys += sh.keys[w]; }
+    t.total *= p.kv_heads;
+    const int ctas = gridDim.x;
+    t.runs = (int)min((int64_t)ctas * (t.whole ? 1 : attn_parts(t.total, ctas, keys * p.kv_bytes, p.most_parts)), t.total);
+    return t;
 }
 
-// The units of a CTA's run, one after the other.  The next request's lengths are fetched when this one's are first used.
+// The units of a run, one after the other, for a whole warp.  The next request's lengths are fetched when this one's are first used.
 template <class Cut>
 struct AttnWalk {
     AttnRequest r, next;
-    int64_t lo, hi, unit, total;
-    int block, blocks, request, head, tiles, ctas;
-    bool whole;
+    int64_t lo, hi, unit;
+    int run, block, blocks, request, head, tiles;
 
     __device__ __forceinline__ void fetch(const AttnParams& p, int i)
     {
@@ -189,44 +150,95 @@ struct AttnWalk {
     }
     __device__ __forceinline__ void size(const AttnParams& p) { tiles = attn_block_tiles(r, p.group, block, Cut::ROWS, Cut::TILE); }
 
-    __device__ __forceinline__ void begin(const AttnParams& p, const AttnPlace& at, bool whole_units)
+    // the CTA's first run, or its next: false behind the last
+    __device__ __forceinline__ bool begin(const AttnParams& p, const AttnTotals& t, const AttnShared& sh) { return seek(p, t, sh, blockIdx.x); }
+    __device__ __forceinline__ bool next_run(const AttnParams& p, const AttnTotals& t, const AttnShared& sh) { return seek(p, t, sh, run + gridDim.x); }
+    __device__ __forceinline__ bool seek(const AttnParams& p, const AttnTotals& t, const AttnShared& sh, int which)
     {
-        whole = whole_units;
-        total = at.total;
-        ctas = (int)min((int64_t)gridDim.x, total);
-        lo = (int)blockIdx.x < ctas ? attn_run(blockIdx.x, total, ctas) : total;
-        hi = (int)blockIdx.x < ctas ? attn_run(blockIdx.x + 1, total, ctas) : total;
-        unit = hi;
-        if (lo >= hi) return;
-        unit = at.unit; block = at.block; request = at.request; head = at.head;
-        fetch(p, request);
-        enter(p);
+        run = which;
+        if (run >= t.runs) return false;
+        lo = attn_run(run, t.total, t.runs);
+        hi = attn_run(run + 1, t.total, t.runs);
+        const int lane = threadIdx.x & 31;
+        // the entry with tile lo, then its request, head and block; everything in front of `at` has been passed
+        long long at = 0;
+        int entry = 0;
+        for (int e0 = 0; e0 < ATTN_ENTRIES; e0 += 32) {
+            const long long own = (long long)sh.cost[e0 + lane] * p.kv_heads;
+            long long sum = own;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long up = __shfl_up_sync(~0u, sum, o);
+                if (lane >= o) sum += up;
+            }
+            const uint32_t behind = __ballot_sync(~0u, at + sum > lo);
+            if (behind) {
+                const int l = __ffs(behind) - 1;
+                entry = e0 + l;
+                at += __shfl_sync(~0u, sum - own, l);
+                break;
+            }
+            at += __shfl_sync(~0u, sum, 31);
+        }
+        uint32_t cost = 0;                                       // of the request in one head
+        for (request = entry * t.per;; ++request) {
+            r = attn_request(p, request);
+            cost = t.per == 1 ? sh.cost[request] : attn_request_cost<Cut>(p, r, t.whole);
+            const long long all = (long long)cost * p.kv_heads;
+            if (at + all > lo || request + 1 >= p.n) break;
+            at += all;
+        }
+        blocks = attn_blocks(r, p.group.d, Cut::ROWS);
+        head = (int)((uint32_t)(lo - at) / cost);
+        at += (long long)head * cost;
+        block = 0;
+        for (int b0 = 0; b0 < blocks; b0 += 32) {
+            const int own = b0 + lane < blocks ? attn_unit_cost<Cut>(p, r, b0 + lane, t.whole) : 0;
+            int sum = own;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int up = __shfl_up_sync(~0u, sum, o);
+                if (lane >= o) sum += up;
+            }
+            const uint32_t behind = __ballot_sync(~0u, at + sum > lo);
+            if (behind) {
+                const int l = __ffs(behind) - 1;
+                block = b0 + l;
+                at += __shfl_sync(~0u, sum - own, l);
+                break;
+            }
+            at += __shfl_sync(~0u, sum, 31);
+        }
+        unit = at;
+        fetch(p, request + 1);
         size(p);
-        if (!whole && lo >= unit + tiles) step(p);             // (what is left of the unit is what it costs beside its tiles)
+        if (!t.whole && lo >= unit + tiles) step(p, t);         // (what is left of the unit is what it costs beside its tiles)
+        return true;
     }
     __device__ __forceinline__ bool more() const { return unit < hi; }
-    __device__ __forceinline__ int cost() const { return whole ? 1 : tiles + Cut::EXTRA; }
-    // tiles of the unit that are this CTA's: [first, end)
-    __device__ __forceinline__ int first() const { return whole || lo <= unit ? 0 : (int)(lo - unit); }
-    __device__ __forceinline__ int end() const { return whole || unit + tiles <= hi ? tiles : (int)(hi - unit); }
-    __device__ __forceinline__ void step(const AttnParams& p)
+    // tiles of the unit that are this run's: [first, end)
+    __device__ __forceinline__ int first() const { return lo <= unit ? 0 : (int)(lo - unit); }
+    __device__ __forceinline__ int end(const AttnTotals& t) const { return t.whole || unit + tiles <= hi ? tiles : (int)(hi - unit); }
+    __device__ __forceinline__ void step(const AttnParams& p, const AttnTotals& t)
     {
-        unit += cost();
-        if (++head < p.kv_heads || unit >= hi) return;
-        head = 0;
+        unit += t.whole ? 1 : tiles + Cut::EXTRA;
+        if (unit >= hi) return;
         if (++block >= blocks) {
             block = 0;
-            do {
-                ++request;
-                enter(p);
-            } while (!blocks);                                 // (there is one: unit < hi)
+            if (++head >= p.kv_heads) {
+                head = 0;
+                do {
+                    ++request;
+                    enter(p);
+                } while (!blocks);                               // (there is one: unit < hi)
+            }
         }
         size(p);
     }
-    // whether other CTAs have tiles of the unit, and the CTAs that have some
-    __device__ __forceinline__ bool cut() const { return !whole && (unit < lo || unit + tiles > hi); }
-    __device__ __forceinline__ int opener() const { return attn_owner(unit, total, ctas); }
-    __device__ __forceinline__ int closer() const { return attn_owner(unit + tiles - 1, total, ctas); }
+    // whether other runs have tiles of the unit, and the runs that have some
+    __device__ __forceinline__ bool cut(const AttnTotals& t) const { return !t.whole && (unit < lo || unit + tiles > hi); }
+    __device__ __forceinline__ int opener(const AttnTotals& t) const { return attn_owner(unit, t.total, t.runs); }
+    __device__ __forceinline__ int closer(const AttnTotals& t) const { return attn_owner(unit + tiles - 1, t.total, t.runs); }
 };
 
 // Waits that give up: after that nothing is waited for any more, and the kernel runs to its end.  The first one is suspended, the second looks at the

@@ -12,16 +12,18 @@
 
 namespace mpq {
 
-constexpr int FEW_ROWS = 16, FEW_TILE = 128, FEW_WARPS = 4, FEW_KEYS = FEW_TILE / FEW_WARPS, FEW_THREADS = 32 * (FEW_WARPS + 1);
+constexpr int FEW_MOST_CTAS = 256, FEW_ROWS = 16, FEW_TILE = 128, FEW_WARPS = 4, FEW_KEYS = FEW_TILE / FEW_WARPS, FEW_THREADS = 32 * (FEW_WARPS + 1);
+static_assert(FEW_THREADS >= ATTN_ENTRIES, "an entry per thread");
 
-using FewCut = AttnCut<FEW_ROWS, FEW_TILE, 0, 0>;
+using FewCut = AttnCut<FEW_ROWS, FEW_TILE, 0, false>;
 
 template <int D>
 struct FewShape {
     static constexpr int WARP_BYTES = FEW_KEYS * D * 2;                      // keys (or values) of one warp
     static constexpr int STAGE_BYTES = 2 * FEW_WARPS * WARP_BYTES;           // [warp][k | v]
     static constexpr int STAGES = D == 128 ? 3 : 6;
-    static constexpr int JOIN_BYTES = FEW_WARPS * FEW_ROWS * D * 4;
+    // the warps' parts of o; the factors of a cut unit's pieces and up to sixteen rows of sums
+    static constexpr int JOIN_BYTES = 4 * (FEW_WARPS * FEW_ROWS * D > FEW_ROWS * FEW_MOST_CTAS + FEW_ROWS * D ? FEW_WARPS * FEW_ROWS * D : FEW_ROWS * FEW_MOST_CTAS + FEW_ROWS * D);
     static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + JOIN_BYTES;
     static constexpr int PIECE = FEW_ROWS * (D + 2);                         // floats of a piece in scratch: o, maxima, sums
 };
@@ -67,10 +69,8 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     }
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const bool whole = !p.partial;
-    const AttnPlace place = attn_locate<FewCut>(p, whole, s_shared, nullptr);       // (its barriers publish the mbarriers)
+    const AttnTotals totals = attn_totals<FewCut>(p, s_shared);              // (its barriers publish the mbarriers)
     AttnWalk<FewCut> u;
-    u.begin(p, place, whole);
 
     if (warp == FEW_WARPS) {
         // ---- producer: lane = (box of a tile, k or v); boxes behind the request's last key are not fetched
@@ -78,9 +78,10 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         const int box = lane % BOXES, what = lane / BOXES;                   // 0: k, 1: v
         int s = 0;
         uint32_t phase = 1;
-        for (; u.more(); u.step(p)) {
+        for (bool run = u.begin(p, totals, s_shared); run; run = u.next_run(p, totals, s_shared))
+            for (; u.more(); u.step(p, totals)) {
                 const int32_t* row = p.table + u.request * p.width;
-                const int end = u.end();
+                const int end = u.end(totals);
                 for (int t = u.first(); t < end; ++t) {
                     attn_wait(empty(s), phase, &s_abort, p.status, 41);
                     __syncwarp();
@@ -107,7 +108,8 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         const int km = lane >> 3, kr = lane & 7;
         int s = 0;
         uint32_t phase = 0;
-        for (; u.more(); u.step(p)) {
+        for (bool run = u.begin(p, totals, s_shared); run; run = u.next_run(p, totals, s_shared))
+        for (; u.more(); u.step(p, totals)) {
             const int rows = attn_block_rows(u.r, p.group.d, u.block, FEW_ROWS);
             const int row0 = u.block * FEW_ROWS;
             // keys that rows g and g + 8 see
@@ -134,7 +136,7 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
 #pragma unroll
                 for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
             float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-            const int end = u.end();
+            const int end = u.end(totals);
             for (int t = u.first(); t < end; ++t) {
                 attn_wait(full(s, warp), phase, &s_abort, p.status, 42);
                 const uint32_t kb = smem0 + s * S::STAGE_BYTES + warp * 2 * S::WARP_BYTES, vb = kb + S::WARP_BYTES;
@@ -241,10 +243,10 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                 *reinterpret_cast<float2*>(at + 8 * D) = make_float2(o[i][2] * f1, o[i][3] * f1);
             }
             few_sync();
-            const bool cut = u.cut();
-            const int opener = cut ? u.opener() : 0, closer = cut ? u.closer() : 0;
-            // a row's columns and what stands beside them; `slot` of scratch: what this CTA opened, or what it continues
-            auto slot = [&](int cta) { return p.partial + (int64_t)(2 * cta + (cta == opener ? 1 : 0)) * S::PIECE; };
+            const bool cut = u.cut(totals);
+            const int opener = cut ? u.opener(totals) : 0, closer = cut ? u.closer(totals) : 0;
+            // a row's columns and what stands beside them; `slot` of scratch: the unit that a run opened, or the one that it continues
+            auto slot = [&](int r) { return p.partial + (int64_t)(2 * r + (r == opener ? 1 : 0)) * S::PIECE; };
             auto store = [&](int r, int c, float v) {
                 const int at = row0 + r, tok = p.group.of(at);
                 const int64_t to = ((int64_t)(u.r.first + tok) * p.q_heads + (u.head - tok) * (int)p.group.d + at) * D + c;
@@ -262,7 +264,7 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                 }
                 if (!cut) store(r, c, l == 0.f ? 0.f : v / l);
                 else {
-                    float* mine = slot(blockIdx.x);
+                    float* mine = slot(u.run);
                     mine[r * D + c] = v;
                     if (c == 0) { mine[FEW_ROWS * D + r] = top; mine[FEW_ROWS * D + FEW_ROWS + r] = l; }
                 }
@@ -277,18 +279,56 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                     __threadfence();
                 }
                 few_sync();
-                if (s_last)
-                    for (int e = threadIdx.x; e < rows * D; e += 32 * FEW_WARPS) {
-                        const int r = e / D, c = e % D;
-                        float top = -INFINITY, l = 0.f, v = 0.f;
-                        for (int cta = opener; cta <= closer; ++cta) top = fmaxf(top, __ldcg(slot(cta) + FEW_ROWS * D + r));
-                        for (int cta = opener; cta <= closer; ++cta) {
-                            const float f = factor(__ldcg(slot(cta) + FEW_ROWS * D + r), top);
-                            l = fmaf(f, __ldcg(slot(cta) + FEW_ROWS * D + FEW_ROWS + r), l);
-                            v = fmaf(f, __ldcg(slot(cta) + r * D + c), v);
-                        }
-                        store(r, c, l == 0.f ? 0.f : v / l);
+                if (s_last) {
+                    // Factors of the pieces' rows; then one, two or four groups of threads add their part of the pieces each, in order, and the
+                    // groups' sums are added in order.
+                    const int pieces = closer - opener + 1;
+                    float *fac = join, *acc = join + FEW_ROWS * FEW_MOST_CTAS;
+                    for (int i = threadIdx.x; i < rows * pieces; i += 32 * FEW_WARPS) {
+                        const int q = i / rows, r = i - q * rows;
+                        fac[q * FEW_ROWS + r] = __ldcg(slot(opener + q) + FEW_ROWS * D + r);
                     }
+                    few_sync();
+                    if ((int)threadIdx.x < rows) {
+                        const int r = threadIdx.x;
+                        float top = -INFINITY, l = 0.f;
+                        for (int q = 0; q < pieces; ++q) top = fmaxf(top, fac[q * FEW_ROWS + r]);
+#pragma unroll 4
+                        for (int q = 0; q < pieces; ++q) {
+                            const float f = factor(fac[q * FEW_ROWS + r], top);
+                            fac[q * FEW_ROWS + r] = f;
+                            l = fmaf(f, __ldcg(slot(opener + q) + FEW_ROWS * D + FEW_ROWS + r), l);
+                        }
+                        s_sum[0][r] = l;
+                    }
+                    few_sync();
+                    const int groups = rows <= 4 ? 4 : rows <= 8 ? 2 : 1, each = 32 * FEW_WARPS / groups, group = threadIdx.x / each;
+                    const int q0 = pieces * group / groups, q1 = pieces * (group + 1) / groups;
+                    for (int e = threadIdx.x - group * each; e < rows * D / 4; e += each) {
+                        const int r = e / (D / 4);
+                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                        for (int q = q0; q < q1; q += 4) {
+                            float4 a[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                if (q + k < q1) a[k] = __ldcg(reinterpret_cast<const float4*>(slot(opener + q + k)) + e);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                if (q + k < q1) {
+                                    const float f = fac[(q + k) * FEW_ROWS + r];
+                                    v.x = fmaf(a[k].x, f, v.x); v.y = fmaf(a[k].y, f, v.y); v.z = fmaf(a[k].z, f, v.z); v.w = fmaf(a[k].w, f, v.w);
+                                }
+                        }
+                        reinterpret_cast<float4*>(acc)[group * (rows * D / 4) + e] = v;
+                    }
+                    few_sync();
+                    for (int e = threadIdx.x; e < rows * D; e += 32 * FEW_WARPS) {
+                        float v = 0.f;
+                        for (int w = 0; w < groups; ++w) v += acc[w * rows * D + e];
+                        const float l = s_sum[0][e / D];
+                        store(e / D, e % D, l == 0.f ? 0.f : v / l);
+                    }
+                }
             }
             few_sync();                                                      // the next unit writes what this one's threads read
         }

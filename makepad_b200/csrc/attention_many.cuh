@@ -25,7 +25,7 @@ namespace mpq {
 
 constexpr int MANY_ROWS = 256, MANY_TILE = 128, MANY_THREADS = 640;
 constexpr int MANY_REGS_WORK = 104, MANY_REGS_REST = 64;         // 4 x 104 + 64 = 5 x 96, what a thread is launched with
-using ManyCut = AttnCut<MANY_ROWS, MANY_TILE, 1, MANY_THREADS / 32>;
+using ManyCut = AttnCut<MANY_ROWS, MANY_TILE, 1, true>;
 constexpr int MANY_POWERS = 4;                                    // every so many pairs of weights by a polynomial: see power2
 constexpr float MANY_LATE = 8.f;                                  // log2 of how far a row's maximum runs ahead of the one in use
 
@@ -35,13 +35,12 @@ struct ManyUnit {
     int first, end, ends[2];                 // tiles of keys of this CTA: all, and up to where the row tiles want them
     int keys, new_rows, first_row;           // of the request
     int row0, rows, head, request;           // first packed row of the block, rows of it
-    int cut, opener, closer;                 // whether other CTAs have tiles of the unit, and which
+    int cut, opener, closer, run;            // whether other runs have tiles of the unit, and which; this one
 };
 struct ManyShared {
     uint64_t q_full[2], s_full[2], p_half[2], p_full[2], o_full[2], o_empty[2], kv_full[8], kv_empty[8], unit_full[MANY_UNITS], unit_empty[MANY_UNITS];
     ManyUnit units[MANY_UNITS];
-    float top[2][2][128];                    // a row's maximum over the keys of each team
-    AttnShared locate;
+    AttnShared totals;
     uint32_t tmem;
     int last[2];
     volatile int abort;
@@ -51,8 +50,9 @@ template <int D>
 struct ManyShape {
     static constexpr int HALVES = D / 64, HALF_BYTES = 128 * 128;            // 128 keys (or rows) of 64 elements, 128-byte swizzle
     static constexpr int TILE_BYTES = HALVES * HALF_BYTES;
-    static constexpr int STAGES = D == 128 ? 5 : 8;                          // K and V tiles in turn
-    static constexpr int SMEM = (2 + STAGES) * TILE_BYTES + sizeof(ManyShared);
+    static constexpr int STAGES = D == 128 ? 4 : 8;                          // K and V tiles in turn
+    static constexpr int STORE_BYTES = 16 * 2048;                            // per softmax warp: 64 bytes of 32 rows on their way out
+    static constexpr int SMEM = (2 + STAGES) * TILE_BYTES + STORE_BYTES + sizeof(ManyShared);
     static constexpr int PIECE = MANY_ROWS * (D + 2);                        // floats of a piece in scratch: o, maxima, sums
 };
 
@@ -162,7 +162,7 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     using S = ManyShape<D>;
     using Walk = AttnWalk<ManyCut>;
     extern __shared__ __align__(1024) unsigned char smem_many[];              // (no other shared memory: 227 KB are just enough)
-    ManyShared& sh = *reinterpret_cast<ManyShared*>(smem_many + (2 + S::STAGES) * S::TILE_BYTES);
+    ManyShared& sh = *reinterpret_cast<ManyShared*>(smem_many + (2 + S::STAGES) * S::TILE_BYTES + S::STORE_BYTES);
     const uint32_t smem0 = s2u(smem_many), smem_kv = smem0 + 2 * S::TILE_BYTES;
     const uint32_t q_full = s2u(sh.q_full), s_full = s2u(sh.s_full), p_half = s2u(sh.p_half), p_full = s2u(sh.p_full), o_full = s2u(sh.o_full),
                    o_empty = s2u(sh.o_empty), kv_full = s2u(sh.kv_full), kv_empty = s2u(sh.kv_empty), unit_full = s2u(sh.unit_full), unit_empty = s2u(sh.unit_empty);
@@ -201,8 +201,7 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     const uint32_t tmem = (uint32_t)uniform((int)sh.tmem);
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const bool whole = !p.partial;
-    const AttnPlace place = attn_locate<ManyCut>(p, whole, sh.locate, reinterpret_cast<uint32_t*>(smem_many));
+    const AttnTotals totals = attn_totals<ManyCut>(p, sh.totals);
     // the units, for the warps that are told of them: the next one, or false behind the last
     int unit_at = 0;
     uint32_t unit_phase = 0;
@@ -340,22 +339,22 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         } else {
             // ---- the units
             Walk w;
-            w.begin(p, place, whole);
             uint32_t phase = 1;
             int at = 0;
-            for (bool there = true; there && !sh.abort;) {
-                there = w.more();
+            bool there = w.begin(p, totals, sh.totals);
+            do {
+                while (there && !w.more()) there = w.next_run(p, totals, sh.totals);
                 attn_wait(unit_empty + 8 * at, phase, &sh.abort, p.status, 63);
                 if (lane == 0) {
                     ManyUnit n = {};
                     n.there = there;
                     if (there) {
-                        n.first = w.first(); n.end = w.end();
+                        n.first = w.first(); n.end = w.end(totals);
                         n.keys = w.r.keys; n.new_rows = w.r.rows; n.first_row = w.r.first;
                         n.row0 = w.block * MANY_ROWS; n.rows = attn_block_rows(w.r, p.group.d, w.block, MANY_ROWS);
                         n.head = w.head; n.request = w.request;
-                        n.cut = w.cut();
-                        if (n.cut) { n.opener = w.opener(); n.closer = w.closer(); }
+                        n.cut = w.cut(totals); n.run = w.run;
+                        if (n.cut) { n.opener = w.opener(totals); n.closer = w.closer(totals); }
 #pragma unroll
                         for (int t = 0; t < 2; ++t) {
                             const int rows = min(n.rows - 128 * t, 128);
@@ -367,8 +366,9 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 }
                 __syncwarp();
                 if (++at == MANY_UNITS) { at = 0; phase ^= 1u; }
-                if (there) w.step(p);
-            }
+                if (there) w.step(p, totals);
+                else break;
+            } while (!sh.abort);
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(MANY_REGS_WORK));
@@ -378,6 +378,10 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         const uint32_t ts = tmem + lanes + 128 * t, to = tmem + lanes + 256 + 128 * t + half * (D / 2);
         const int pair = 1 + 4 * t + quarter;                                  // barrier of the two warps with these rows
         uint32_t s_phase = 0, o_phase = 0;
+        // This warp's 2 KB, and those of the warp with the other half: a row's maximum or sum there (a float per lane) while a unit is worked on, at its
+        // end rows on their way out.
+        unsigned char* room = smem_many + (2 + S::STAGES) * S::TILE_BYTES + warp * 2048;
+        float *tell = reinterpret_cast<float*>(room) + lane, *told = reinterpret_cast<float*>(room + (half ? -4 : 4) * 2048) + lane;
         // The next unit's rows of Q, 16 bytes at a time into the swizzled tile: chunk c of every sixteenth (or thirty-second) row; token and head of
         // the row go on with it.  (The tile is free: this thread has seen the last S that was made of it.)
         auto fetch_q = [&] {
@@ -446,9 +450,9 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 }
                 float top = max_nan(y[0], y[1], y[1]);
                 // (the other team's reading of the last one is behind its arrival at p_full, which this S waited for)
-                sh.top[t][half][row] = top;
+                *tell = top;
                 team_sync<64>(pair);
-                top = max_nan(top, sh.top[t][half ^ 1][row], -INFINITY);
+                top = max_nan(top, *told, -INFINITY);
                 if (top == INFINITY) top = NAN;                                // (what inf - inf would make of the row)
                 if (j == first) m = top;
                 else if (__any_sync(~0u, !((top - m) * p.scale_log2 <= MANY_LATE))) {
@@ -501,31 +505,52 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 tc_fence_after();
             }
             if (fetched) q_there();
-            sh.top[t][half][row] = l;                                          // (behind o_full, so behind the other team's last reading, too)
+            *tell = l;                                                         // (behind o_full, so behind the other team's last reading, too)
             team_sync<64>(pair);
-            l += sh.top[t][half ^ 1][row];
-            team_sync<64>(pair);                                               // (the next unit's maxima go there)
+            l += *told;
+            team_sync<64>(pair);                                               // (rows go there now)
             const bool cut = u.cut;
             const int opener = u.opener, closer = u.closer;
-            const int64_t to_row = ((int64_t)(u.first_row + tok) * p.q_heads + (u.head - tok) * (int)p.group.d + at) * D + half * (D / 2);
-            auto store16 = [&](int c, const float* v) {                        // 16 columns from c on, of this thread's half
-                if (row >= rows) return;
-                if (p.out_f32) {
-                    float* out = static_cast<float*>(p.out) + to_row + c;
+            // 64 bytes of each of the warp's rows from column c of this thread's half on: through shared memory (16-byte chunks, their order turned so that neither
+            // side meets a bank twice), so that four lanes store 64 bytes of a row
+            const int64_t out0 = ((int64_t)u.first_row * p.q_heads + u.head * (int)p.group.d) * D + half * (D / 2);
+            auto send = [&](int c, const uint32_t (&w)[16]) {
+                const uint32_t mine = s2u(room) + lane * 64;
 #pragma unroll
-                    for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(out + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                for (int i = 0; i < 4; ++i)
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + ((i ^ ((lane >> 1) & 3)) << 4)), "r"(w[4 * i]), "r"(w[4 * i + 1]), "r"(w[4 * i + 2]), "r"(w[4 * i + 3]) : "memory");
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int q = 8 * i + (lane >> 2), to = u.row0 + 128 * t + quarter * 32 + q;
+                    uint4 v;
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(s2u(room) + q * 64 + (((lane & 3) ^ ((q >> 1) & 3)) << 4)) : "memory");
+                    if (quarter * 32 + q < rows) {
+                        const int token = p.group.of(to);
+                        const int64_t place = out0 + (int64_t)token * (p.q_heads - (int)p.group.d) * D + (int64_t)to * D + c;
+                        *reinterpret_cast<uint4*>(static_cast<char*>(p.out) + place * (p.out_f32 ? 4 : 2) + (lane & 3) * 16) = v;
+                    }
+                }
+                __syncwarp();
+            };
+            auto send16 = [&](int c, const float (&v)[16], uint32_t (&held)[16]) {      // sixteen columns, and (bf16) the sixteen before
+                if (p.out_f32) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) held[i] = __float_as_uint(v[i]);
+                    send(c, held);
                 } else {
-                    uint4* out = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + to_row + c);
-                    out[0] = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
-                    out[1] = make_uint4(pack_bf16(v[8], v[9]), pack_bf16(v[10], v[11]), pack_bf16(v[12], v[13]), pack_bf16(v[14], v[15]));
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) held[i + (c & 16 ? 8 : 0)] = pack_bf16(v[2 * i], v[2 * i + 1]);
+                    if (c & 16) send(c - 16, held);
                 }
             };
             // a piece: [column / 4][row][4], so that a warp's threads lie beside each other; then maxima, sums
             const int mine = 128 * t + row, col4 = half * (D / 8);
-            auto slot = [&](int cta) { return p.partial + (int64_t)(2 * cta + (cta == opener ? 1 : 0)) * S::PIECE; };
+            auto slot = [&](int r) { return p.partial + (int64_t)(2 * r + (r == opener ? 1 : 0)) * S::PIECE; };
+            uint32_t held[16];
             if (some) {
                 const float scale = cut ? 1.f : l == 0.f ? 0.f : 1.f / l;
-#pragma unroll 1
+#pragma unroll
                 for (int c = 0; c < D / 2; c += 16) {
                     uint32_t o[16];
                     tc_ld16(to + c, o);
@@ -533,9 +558,9 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     float v[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(o[i]) * scale;
-                    if (!cut) store16(c, v);
+                    if (!cut) send16(c, v, held);
                     else {
-                        float4* to4 = reinterpret_cast<float4*>(slot(blockIdx.x)) + (col4 + (c >> 2)) * MANY_ROWS + mine;
+                        float4* to4 = reinterpret_cast<float4*>(slot(u.run)) + (col4 + (c >> 2)) * MANY_ROWS + mine;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) to4[i * MANY_ROWS] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
                     }
@@ -545,7 +570,7 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             }
             if (cut) {
                 if (half == 0) {
-                    float* head = slot(blockIdx.x) + MANY_ROWS * D;
+                    float* head = slot(u.run) + MANY_ROWS * D;
                     head[mine] = m == -INFINITY ? m : m * p.scale_log2;
                     head[MANY_ROWS + mine] = l;
                 }
@@ -559,31 +584,36 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 }
                 team_sync<256>(9 + t);
                 if (sh.last[t]) {
-                    float top = -INFINITY, sum = 0.f;
-                    for (int cta = opener; cta <= closer; ++cta) top = max_nan(top, __ldcg(slot(cta) + MANY_ROWS * D + mine), -INFINITY);
-                    for (int cta = opener; cta <= closer; ++cta) {
-                        const float mm = __ldcg(slot(cta) + MANY_ROWS * D + mine);
-                        if (mm != -INFINITY) sum = fmaf(exp2f(mm - top), __ldcg(slot(cta) + MANY_ROWS * D + MANY_ROWS + mine), sum);
-                    }
-                    const float scale = sum == 0.f ? 0.f : 1.f / sum;
+                    // the pieces in order, rescaled when a larger maximum comes; 32 columns at a time
+                    float sum = 0.f;
 #pragma unroll 1
-                    for (int c = 0; c < D / 2; c += 16) {
-                        float v[16];
+                    for (int c = 0; c < D / 2; c += 32) {
+                        float v[2][16], top = -INFINITY;
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) v[i] = 0.f;
-                        for (int cta = opener; cta <= closer; ++cta) {
-                            const float mm = __ldcg(slot(cta) + MANY_ROWS * D + mine);
+                        for (int i = 0; i < 32; ++i) v[i >> 4][i & 15] = 0.f;
+                        sum = 0.f;
+                        for (int r = opener; r <= closer; ++r) {
+                            const float* head = slot(r) + MANY_ROWS * D + mine;
+                            const float4* from = reinterpret_cast<const float4*>(slot(r)) + (col4 + (c >> 2)) * MANY_ROWS + mine;
+                            float4 a[8];
+                            const float mm = __ldcg(head), ll = __ldcg(head + MANY_ROWS);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) a[i] = __ldcg(from + i * MANY_ROWS);
                             if (mm == -INFINITY) continue;                     // (nothing of this piece is seen: its o need not be there)
-                            const float f = exp2f(mm - top) * scale;
-                            const float4* from = reinterpret_cast<const float4*>(slot(cta)) + (col4 + (c >> 2)) * MANY_ROWS + mine;
+                            const float both = max_nan(top, mm, mm), f = top == -INFINITY ? 0.f : ex2(top - both), g = ex2(mm - both);
+                            top = both;
+                            sum = fmaf(sum, f, ll * g);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const float4 a = __ldcg(from + i * MANY_ROWS);
-                                v[4 * i] = fmaf(a.x, f, v[4 * i]); v[4 * i + 1] = fmaf(a.y, f, v[4 * i + 1]);
-                                v[4 * i + 2] = fmaf(a.z, f, v[4 * i + 2]); v[4 * i + 3] = fmaf(a.w, f, v[4 * i + 3]);
+                            for (int i = 0; i < 8; ++i) {
+                                float* w = &v[i >> 2][4 * (i & 3)];
+                                w[0] = fmaf(a[i].x, g, w[0] * f); w[1] = fmaf(a[i].y, g, w[1] * f); w[2] = fmaf(a[i].z, g, w[2] * f); w[3] = fmaf(a[i].w, g, w[3] * f);
                             }
                         }
-                        store16(c, v);
+                        const float scale = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i >> 4][i & 15] *= scale;
+                        send16(c, v[0], held);
+                        send16(c + 16, v[1], held);
                     }
                 }
                 team_sync<256>(9 + t);                                         // (sh.last is the next unit's then)

@@ -3,9 +3,9 @@
 // The new tokens of a request and the query heads that share a head of keys are its rows, packed token by token: row = token * group +
 // head in the group.  A block is up to ROWS consecutive rows; a unit is a block and a head of keys; its tiles are the TILE keys at a time that
 // its last row sees (one, empty, where it sees none: its rows of zeros are written all the same).  The tiles of all units in order
-// (request, block, head) are cut into equal runs, one per CTA, wherever that falls: no shape leaves SMs idle.  What a unit costs beside its tiles (its
-// queries, its end) counts as `extra` tiles behind them that nobody works on.  A unit that a cut falls into has a piece in each CTA from the one with its
-// first tile to the one with its last.  A CTA opens at most one such unit (its last) and continues at most one (its first).
+// (request, head, block) are cut into equal runs, one per CTA (or a few: attn_parts), wherever that falls: no shape leaves SMs idle.  What a unit
+// costs beside its tiles (its queries, its end) counts as `extra` tiles behind them that nobody works on.  A unit that a cut falls into has a piece in each
+// run from the one with its first tile to the one with its last.  A run opens at most one such unit (its last) and continues at most one (its first).
 #pragma once
 #include <stdint.h>
 
@@ -72,8 +72,32 @@ MPQ_BOTH int attn_block_tiles(const AttnRequest& r, const AttnDivisor& group, in
     return attn_tiles(attn_seen(r, group.of(b * block_rows + attn_block_rows(r, (int)group.d, b, block_rows) - 1)), tile);
 }
 
-// run of CTA c of `ctas` (at most `total` of them have one), and the CTA that has tile t
-MPQ_BOTH int64_t attn_run(int64_t c, int64_t total, int64_t ctas) { return c * total / ctas; }
-MPQ_BOTH int attn_owner(int64_t t, int64_t total, int64_t ctas) { return (int)(((t + 1) * ctas - 1) / total); }
+// First tile of run v of `runs` (at most `total`), and the run that has tile t.  v * (total % runs) stays below 2^31: there are few runs.
+MPQ_BOTH int64_t attn_run(int v, int64_t total, int runs)
+{
+    if (total < (1ll << 32)) {
+        const uint32_t q = (uint32_t)total / (uint32_t)runs, r = (uint32_t)total - q * runs;
+        return (int64_t)v * q + (uint32_t)v * r / (uint32_t)runs;
+    }
+    const int64_t q = total / runs;
+    return v * q + (int64_t)((uint32_t)v * (uint32_t)(total - q * runs) / (uint32_t)runs);
+}
+MPQ_BOTH int attn_owner(int64_t t, int64_t total, int runs)
+{
+    if (total < (1ll << 20)) return (int)(((uint32_t)(t + 1) * (uint32_t)runs - 1) / (uint32_t)total);
+    return (int)(((t + 1) * runs - 1) / total);
+}
+constexpr int ATTN_MOST_RUNS = 2048;
+
+// Into how many parts, one after the other, all tiles are cut before each part is cut into a run per CTA: so many that the keys and values of a part
+// (in a part are the heads of few requests) stay in L2, but no runs of fewer than ATTN_LEAST_RUN tiles.
+constexpr int64_t ATTN_PART_BYTES = 40 << 20;
+constexpr int ATTN_LEAST_RUN = 48;
+MPQ_BOTH int attn_parts(int64_t total, int ctas, int64_t kv_bytes, int most)
+{
+    int64_t parts = (kv_bytes + ATTN_PART_BYTES - 1) / ATTN_PART_BYTES;
+    if (parts > total / ((int64_t)ctas * ATTN_LEAST_RUN)) parts = total / ((int64_t)ctas * ATTN_LEAST_RUN);
+    return parts < 1 ? 1 : parts > most ? most : (int)parts;
+}
 
 }  // namespace mpq

@@ -199,12 +199,14 @@ static void attention_params(AttnParams* p, const uint16_t* q, int64_t q_stride,
     p->out = out; p->out_f32 = out_is_f32 != 0;
 }
 
-// The pieces of cut units: as much as the kernel with the largest wants, by the first call outside a capture.  Without it units stay whole.
-static void attention_scratch(mpq_context* ctx, AttnParams* p, cudaStream_t s)
+// Room for the pieces of cut units (two per run), by the first call outside a capture that wants so much: of `parts` runs per CTA, or of one where
+// there is no more.  Without any units stay whole.
+static void attention_scratch(mpq_context* ctx, AttnParams* p, int ctas, size_t piece, int parts, cudaStream_t s)
 {
-    const size_t need = 2 * (size_t)ctx->prop.multiProcessorCount * ManyShape<128>::PIECE * sizeof(float);
-    if (ctx->attn_partial.bytes() < need && !stream_captures(s)) ctx->attn_partial.reserve(need);
-    p->partial = ctx->attn_partial.bytes() >= need ? ctx->attn_partial.as<float>() : nullptr;
+    const size_t each = 2 * (size_t)ctas * piece * sizeof(float);
+    if (ctx->attn_partial.bytes() < each * parts && !stream_captures(s) && ctx->attn_partial.reserve(each * parts) != cudaSuccess && parts > 1) ctx->attn_partial.reserve(each);
+    p->most_parts = (int)std::min<size_t>(parts, ctx->attn_partial.bytes() / each);
+    p->partial = p->most_parts ? ctx->attn_partial.as<float>() : nullptr;
     p->arrived = ctx->attn_arrived;
     p->status = ctx->attn_status;
 }
@@ -228,8 +230,10 @@ static bool rows_map(CUtensorMap* map, const void* base, int64_t tokens, int64_t
 }
 
 template <int D, int BOX>
-static int32_t attention_few(mpq_context* ctx, const AttnParams& p, const AttnKeys& kv, cudaStream_t s)
+static int32_t attention_few(mpq_context* ctx, AttnParams p, const AttnKeys& kv, cudaStream_t s)
 {
+    const int ctas = std::min(ctx->prop.multiProcessorCount, FEW_MOST_CTAS);
+    attention_scratch(ctx, &p, ctas, FewShape<D>::PIECE, 1, s);
     static PerDeviceOnce raised;
     if (raised.needs(ctx->device)) {
         CU_TRY(ctx, cudaFuncSetAttribute(attention_few_kernel<D, BOX>, cudaFuncAttributeMaxDynamicSharedMemorySize, FewShape<D>::SMEM));
@@ -238,13 +242,19 @@ static int32_t attention_few(mpq_context* ctx, const AttnParams& p, const AttnKe
     CUtensorMap map_k, map_v;
     if (!cache_map(&map_k, kv.k, kv, p.kv_heads, D, BOX, D / 64) || !cache_map(&map_v, kv.v, kv, p.kv_heads, D, BOX, D / 64)) return fail(ctx, MPQ_ERR_CUDA, "cuTensorMapEncodeTiled failed for the cache");
     ctx->launches += 1;
-    CU_TRY(ctx, launch_beside(ctx, attention_few_kernel<D, BOX>, dim3(std::min(ctx->prop.multiProcessorCount, ATTN_COUNTERS)), FEW_THREADS, FewShape<D>::SMEM, 1, s, map_k, map_v, p));
+    CU_TRY(ctx, launch_beside(ctx, attention_few_kernel<D, BOX>, dim3(ctas), FEW_THREADS, FewShape<D>::SMEM, 1, s, map_k, map_v, p));
     return MPQ_OK;
 }
 
 template <int D, bool PAGED>
-static int32_t attention_many(mpq_context* ctx, const AttnParams& p, const AttnKeys& kv, cudaStream_t s)
+static int32_t attention_many(mpq_context* ctx, AttnParams p, const AttnKeys& kv, cudaStream_t s)
 {
+    constexpr int PARTS = 4;
+    static_assert(2 * PARTS * FEW_MOST_CTAS <= ATTN_COUNTERS && PARTS * FEW_MOST_CTAS <= ATTN_MOST_RUNS, "a counter per run and row tile");
+    const int ctas = std::min(ctx->prop.multiProcessorCount, FEW_MOST_CTAS);
+    p.kv_bytes = 4ll * p.kv_heads * D;
+    const int64_t keys = PAGED ? kv.pages * kv.page_size : p.tokens;
+    attention_scratch(ctx, &p, ctas, ManyShape<D>::PIECE, attn_parts(MOST, ctas, keys * p.kv_bytes, PARTS), s);
     static PerDeviceOnce raised;
     if (raised.needs(ctx->device)) {
         CU_TRY(ctx, cudaFuncSetAttribute(attention_many_kernel<D, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, ManyShape<D>::SMEM));
@@ -258,15 +268,14 @@ static int32_t attention_many(mpq_context* ctx, const AttnParams& p, const AttnK
         if (!made) return fail(ctx, MPQ_ERR_CUDA, "cuTensorMapEncodeTiled failed for the keys or values");
     }
     ctx->launches += 1;
-    CU_TRY(ctx, launch_beside(ctx, attention_many_kernel<D, PAGED>, dim3(std::min(ctx->prop.multiProcessorCount, ATTN_COUNTERS / 2)), MANY_THREADS, ManyShape<D>::SMEM, 1, s, maps[0], maps[1], p));
+    CU_TRY(ctx, launch_beside(ctx, attention_many_kernel<D, PAGED>, dim3(ctas), MANY_THREADS, ManyShape<D>::SMEM, 1, s, maps[0], maps[1], p));
     return MPQ_OK;
 }
 
-static int32_t attention_launch(mpq_context* ctx, AttnParams p, const AttnKeys& kv, int32_t head_dim, cudaStream_t s)
+static int32_t attention_launch(mpq_context* ctx, const AttnParams& p, const AttnKeys& kv, int32_t head_dim, cudaStream_t s)
 {
     const OnDevice on(ctx->device);
     CU_TRY(ctx, on.error);
-    attention_scratch(ctx, &p, s);
     const int64_t most_new = kv.max_new > 0 ? std::min(kv.max_new, p.tokens) : p.tokens;
     if (p.table && most_new * p.group.d <= FEW_ROWS) {
         if (head_dim == 64) return kv.page_size == 16 ? attention_few<64, 16>(ctx, p, kv, s) : attention_few<64, 32>(ctx, p, kv, s);
