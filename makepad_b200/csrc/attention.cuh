@@ -265,6 +265,12 @@ __device__ __forceinline__ void attn_spin(uint32_t bar, uint32_t parity, volatil
     }
 }
 
+// looked at once, then suspended: for a wait that is long as a rule, beside warps that need the issue slots
+__device__ __forceinline__ void attn_look(uint32_t bar, uint32_t parity, volatile int* abort, int* status, int code)
+{
+    if (!bar_test(bar, parity)) attn_wait(bar, parity, abort, status, code);
+}
+
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int a, int b, int c, int d, uint32_t bar)
 {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"

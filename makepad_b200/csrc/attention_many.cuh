@@ -38,7 +38,7 @@ struct ManyUnit {
     int cut, opener, closer, run;            // whether other runs have tiles of the unit, and which; this one
 };
 struct ManyShared {
-    uint64_t q_full[2], s_full[2], p_half[2], p_full[2], o_full[2], o_empty[2], kv_full[8], kv_empty[8], unit_full[MANY_UNITS], unit_empty[MANY_UNITS];
+    uint64_t q_full[2], s_full[2], p_half[2], p_full[2], o_full[2], o_empty[2], kv_full[8], kv_empty[8], unit_full[MANY_UNITS], unit_empty[MANY_UNITS], told[16], turn[2];
     ManyUnit units[MANY_UNITS];
     AttnShared totals;
     uint32_t tmem;
@@ -174,6 +174,7 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     if (threadIdx.x == 0) {
         sh.abort = 0;
         for (int t = 0; t < 2; ++t) {
+            bar_init(s2u(&sh.turn[t]), 1);
             bar_init(q_full + 8 * t, 256);
             bar_init(s_full + 8 * t, 1);
             bar_init(p_half + 8 * t, 256);
@@ -185,6 +186,7 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             bar_init(kv_full + 8 * s, 1);
             bar_init(kv_empty + 8 * s, 2);
         }
+        for (int i = 0; i < 16; ++i) bar_init(s2u(&sh.told[i]), 1);
         for (int i = 0; i < MANY_UNITS; ++i) {
             bar_init(unit_full + 8 * i, 1);
             bar_init(unit_empty + 8 * i, 19);
@@ -226,7 +228,10 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             const uint32_t ts = tmem + 128 * t, to = tmem + 256 + 128 * t, mine = 8 * t;
             const uint64_t a = smem_desc_sw128(smem0 + t * S::TILE_BYTES);
             int s = 0;
-            uint32_t kv_phase = 0, q_phase = 0, p_phase = 0, oe_phase = 1;
+            uint32_t kv_phase = 0, q_phase = 0, p_phase = 0, oe_phase = 1, turn_phase = 1 - t;
+            // The tiles take turns at the end of a product and the next scores: else their softmaxes fall into step, contend for the exponentials at one
+            // time and for the tensor core at the other (4200 cycles per 128 keys)
+            const uint32_t my_turn = s2u(&sh.turn[t ^ 1]), turn_over = s2u(&sh.turn[t]);
             auto advance = [&] { if (++s == S::STAGES) { s = 0; kv_phase ^= 1u; } };
             while (next_unit(u)) {
                 const int first = u.first, end = u.end, e = t ? u.ends[1] : u.ends[0], keys = u.keys;
@@ -234,10 +239,11 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     attn_spin(q_full + mine, q_phase, &sh.abort, p.status, 51);
                     q_phase ^= 1u;
                 }
-                // j: the keys whose scores are made; then (and before the next ones) the product with the values of those before
+                // j: the keys whose scores are made; in front of them the product with the values of those before
                 for (int j = first; j <= end; ++j) {
+                    int v = 0, k0 = 0;
                     if (j > first) {
-                        const int v = uniform(s);
+                        v = uniform(s);
                         attn_spin(kv_full + 8 * v, kv_phase, &sh.abort, p.status, 53);
                         advance();
                         const int from = max(keys - (j - 1) * MANY_TILE, 0);
@@ -251,55 +257,56 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                             __syncwarp();
                         }
-                        if (j <= e) {
-                            const uint64_t b = smem_desc_sw128_mn(smem_kv + v * S::TILE_BYTES);
-                            const uint32_t go_on = j > first + 1 ? 1u : 0u;
-                            // (the first 32 keys of each team, then the others)
-                            auto product = [&](int part) {
-#pragma unroll
-                                for (int q = 0; q < 4; ++q) {
-                                    const int k = (q >> 1) * 4 + 2 * part + (q & 1);
-                                    tc_mma_f16_ts(to, ts + 8 * k, b + (uint64_t)((k * 16 * 128) >> 4), idesc_o, part || q ? 1u : go_on);
-                                }
-                            };
-                            if (j == first + 1) {
-                                attn_spin(o_empty + mine, oe_phase, &sh.abort, p.status, 54);
-                                oe_phase ^= 1u;
-                            }
-                            attn_spin(p_half + mine, p_phase, &sh.abort, p.status, 61);
-                            tc_fence_after();
-                            if (elect_one()) product(0);
-                            __syncwarp();
-                            attn_spin(p_full + mine, p_phase, &sh.abort, p.status, 55);
-                            p_phase ^= 1u;
-                            tc_fence_after();
-                            if (elect_one()) {
-                                product(1);
-                                if (j == e) tc_commit(o_full + mine);
-                                tc_commit(kv_empty + 8 * v);
-                            }
-                            __syncwarp();
-                        } else if (elect_one()) tc_commit(kv_empty + 8 * v);
                     }
+                    // (the next keys are waited for here, and not between the product and the scores)
                     if (j < end) {
-                        const int k0 = uniform(s);
+                        k0 = uniform(s);
                         attn_spin(kv_full + 8 * k0, kv_phase, &sh.abort, p.status, 56);
                         advance();
-                        tc_fence_after();
-                        const uint64_t b = smem_desc_sw128(smem_kv + k0 * S::TILE_BYTES);
-                        if (elect_one()) {
-                            if (j < e) {
-#pragma unroll
-                                for (int k = 0; k < D / 16; ++k) {
-                                    const uint64_t off = (uint64_t)(((k >> 2) * S::HALF_BYTES + (k & 3) * 32) >> 4);
-                                    tc_mma_f16_ss(ts, a + off, b + off, idesc_s, k ? 1u : 0u);
-                                }
-                                tc_commit(s_full + mine);
-                            }
-                            tc_commit(kv_empty + 8 * k0);
-                        }
-                        __syncwarp();
                     }
+                    const uint64_t bv = smem_desc_sw128_mn(smem_kv + v * S::TILE_BYTES), bk = smem_desc_sw128(smem_kv + k0 * S::TILE_BYTES);
+                    const bool multiply = j > first && j <= e;
+                    // (the first 32 keys of each team, then the others)
+                    auto product = [&](int part) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const int k = (q >> 1) * 4 + 2 * part + (q & 1);
+                            tc_mma_f16_ts(to, ts + 8 * k, bv + (uint64_t)((k * 16 * 128) >> 4), idesc_o, part || q || j > first + 1 ? 1u : 0u);
+                        }
+                    };
+                    if (multiply) {
+                        if (j == first + 1) {
+                            attn_spin(o_empty + mine, oe_phase, &sh.abort, p.status, 54);
+                            oe_phase ^= 1u;
+                        }
+                        attn_spin(p_half + mine, p_phase, &sh.abort, p.status, 61);
+                        tc_fence_after();
+                        if (elect_one()) product(0);
+                        __syncwarp();
+                        attn_spin(p_full + mine, p_phase, &sh.abort, p.status, 55);
+                        p_phase ^= 1u;
+                    }
+                    attn_spin(my_turn, turn_phase, &sh.abort, p.status, 66);
+                    turn_phase ^= 1u;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        if (multiply) {
+                            product(1);
+                            if (j == e) tc_commit(o_full + mine);
+                        }
+                        if (j < e) {
+#pragma unroll
+                            for (int k = 0; k < D / 16; ++k) {
+                                const uint64_t off = (uint64_t)(((k >> 2) * S::HALF_BYTES + (k & 3) * 32) >> 4);
+                                tc_mma_f16_ss(ts, a + off, bk + off, idesc_s, k ? 1u : 0u);
+                            }
+                            tc_commit(s_full + mine);
+                        }
+                        bar_arrive(turn_over);
+                        if (j > first) tc_commit(kv_empty + 8 * v);
+                        if (j < end) tc_commit(kv_empty + 8 * k0);
+                    }
+                    __syncwarp();
                 }
             }
         } else if (warp == 18) {
@@ -382,6 +389,24 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         // end rows on their way out.
         unsigned char* room = smem_many + (2 + S::STAGES) * S::TILE_BYTES + warp * 2048;
         float *tell = reinterpret_cast<float*>(room) + lane, *told = reinterpret_cast<float*>(room + (half ? -4 : 4) * 2048) + lane;
+        const uint32_t tell_bar = s2u(&sh.told[warp]), told_bar = s2u(&sh.told[warp ^ 4]);
+        uint32_t told_phase = 0;
+        // the larger of this thread's and the other half's
+        auto say = [&](float v) {
+            *tell = v;
+            __syncwarp();
+            if (lane == 0) bar_arrive(tell_bar);
+        };
+        auto hear = [&] {
+            attn_spin(told_bar, told_phase, &sh.abort, p.status, 65);
+            told_phase ^= 1u;
+            return *told;
+        };
+        auto hide = [](uint32_t (&x)[32], int from) {                          // scores of keys that the row does not see
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (i >= from) x[i] = 0xFF800000u;
+        };
         // The next unit's rows of Q, 16 bytes at a time into the swizzled tile: chunk c of every sixteenth (or thirty-second) row; token and head of
         // the row go on with it.  (The tile is free: this thread has seen the last S that was made of it.)
         auto fetch_q = [&] {
@@ -434,66 +459,87 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 for (int c = 0; c < 2; ++c) tc_ld_wait_for(x[c]);
                 const bool ragged = left_all < 64;
                 if (ragged) {
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (32 * c + i >= left) x[c][i] = 0xFF800000u;
+                    hide(x[0], left);
+                    hide(x[1], left - 32);
                 }
-                float y[2];
+                float y[4];
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    y[c] = max_nan(__uint_as_float(x[c][0]), __uint_as_float(x[c][1]), __uint_as_float(x[c][2]));
+                for (int c = 0; c < 4; ++c) {
+                    const uint32_t* z = &x[c >> 1][16 * (c & 1)];
+                    y[c] = max_nan(__uint_as_float(z[0]), __uint_as_float(z[1]), __uint_as_float(z[2]));
 #pragma unroll
-                    for (int i = 3; i < 31; i += 2) y[c] = max_nan(y[c], __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]));
-                    y[c] = max_nan(y[c], y[c], __uint_as_float(x[c][31]));
+                    for (int i = 3; i < 15; i += 2) y[c] = max_nan(y[c], __uint_as_float(z[i]), __uint_as_float(z[i + 1]));
                 }
-                float top = max_nan(y[0], y[1], y[1]);
+                float top = max_nan(max_nan(y[0], y[1], __uint_as_float(x[0][15])), max_nan(y[2], y[3], __uint_as_float(x[0][31])), max_nan(__uint_as_float(x[1][15]), __uint_as_float(x[1][31]), -INFINITY));
                 // (the other team's reading of the last one is behind its arrival at p_full, which this S waited for)
-                *tell = top;
-                team_sync<64>(pair);
-                top = max_nan(top, *told, -INFINITY);
-                if (top == INFINITY) top = NAN;                                // (what inf - inf would make of the row)
-                if (j == first) m = top;
-                else if (__any_sync(~0u, !((top - m) * p.scale_log2 <= MANY_LATE))) {
-                    // (this S came behind the last product into O)
-                    const float m2 = max_nan(m, top, top), f = m2 == -INFINITY ? 1.f : ex2((m - m2) * p.scale_log2);
-                    m = m2;
-                    l *= f;
-#pragma unroll 1
-                    for (int c = 0; c < D / 2; c += 16) {
-                        uint32_t o[16];
-                        tc_ld16(to + c, o);
-                        tc_ld_wait_for(o);
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                        tc_st16(to + c, o);
-                    }
+                // (the other team's reading of the last one is behind its arrival at p_full, which this S waited for)
+                say(top);
+                // The weights against the maximum in use, beside the exchange of this tile's: only then is it looked at whether they stand (the first
+                // tile of a unit has none to begin with).
+                if (j == first) {
+                    m = max_nan(top, hear(), -INFINITY);
+                    if (m == INFINITY) m = NAN;                                // (what inf - inf would make of the row)
                 }
-                const float base = m == -INFINITY ? 0.f : m * p.scale_log2;
-                const uint64_t scale2 = pair_of(p.scale_log2, p.scale_log2), base2 = pair_of(-base, -base);
-                uint64_t sum[2] = {0, 0};
-                auto weights = [&](auto with_powers) {
+                uint64_t sum[2];
+                // group g: sixteen of a block's 32 keys
+                auto weights = [&](const uint32_t (&x)[32], uint32_t (&w)[16], int g, auto with_powers) {
                     constexpr bool POWERS = decltype(with_powers)::value;
+                    const float base = m == -INFINITY ? 0.f : m * p.scale_log2;
+                    const uint64_t scale2 = pair_of(p.scale_log2, p.scale_log2), base2 = pair_of(-base, -base);
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        uint32_t w[16];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const uint64_t a = fma2(pair_of(x[c][2 * i], x[c][2 * i + 1]), scale2, base2);
-                            const uint64_t e = POWERS && i % MANY_POWERS == MANY_POWERS - 1 ? power2(a) : ex2_pair(a);
-                            sum[i & 1] = add2(sum[i & 1], e);
-                            // bf16 is what the tensor cores take beside bf16 values; the sum keeps the weights as they were
-                            w[i] = bf16_pair(e);
-                        }
-                        tc_st16(ts + 32 * half + 16 * c, w);
-                        tc_st_wait();
-                        tc_fence_before();
-                        bar_arrive((c ? p_full : p_half) + 8 * t);
+                    for (int i = 8 * g; i < 8 * g + 8; ++i) {
+                        const uint64_t a = fma2(pair_of(x[2 * i], x[2 * i + 1]), scale2, base2);
+                        const uint64_t e = POWERS && i % MANY_POWERS == MANY_POWERS - 1 ? power2(a) : ex2_pair(a);
+                        sum[i & 1] = add2(sum[i & 1], e);
+                        // bf16 is what the tensor cores take beside bf16 values; the sum keeps the weights as they were
+                        w[i] = bf16_pair(e);
                     }
                 };
-                if (ragged) weights(std::false_type{});
-                else weights(std::true_type{});
+                auto hand_over = [&](uint32_t bar) {
+                    tc_st_wait();
+                    tc_fence_before();
+                    bar_arrive(bar + 8 * t);
+                };
+                // What is waited for (the other team's maximum, stores into tensor memory) has a group of weights in front of it
+                auto all_weights = [&](auto with_powers) {
+                    uint32_t w[16];
+                    sum[0] = sum[1] = 0;
+                    weights(x[0], w, 0, with_powers);
+                    if (j > first) top = max_nan(top, hear(), -INFINITY);
+                    weights(x[0], w, 1, with_powers);
+                    if (j > first) {
+                        if (top == INFINITY) top = NAN;
+                        if (__any_sync(~0u, !((top - m) * p.scale_log2 <= MANY_LATE))) {
+                            // the maximum moves (this S came behind the last product into O), and the weights are made once more: the scores are still there
+                            const float m2 = max_nan(m, top, top), f = m2 == -INFINITY ? 1.f : ex2((m - m2) * p.scale_log2);
+                            m = m2;
+                            l *= f;
+#pragma unroll 1
+                            for (int c = 0; c < D / 2; c += 16) {
+                                uint32_t o[16];
+                                tc_ld16(to + c, o);
+                                tc_ld_wait_for(o);
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                                tc_st16(to + c, o);
+                            }
+                            tc_ld32(ts + 64 * half, x[0]);
+                            tc_ld_wait_for(x[0]);
+                            if (ragged) hide(x[0], left);
+                            sum[0] = sum[1] = 0;
+                            weights(x[0], w, 0, std::false_type{});
+                            weights(x[0], w, 1, std::false_type{});
+                        }
+                    }
+                    tc_st16(ts + 32 * half, w);
+                    weights(x[1], w, 0, with_powers);
+                    hand_over(p_half);
+                    weights(x[1], w, 1, with_powers);
+                    tc_st16(ts + 32 * half + 16, w);
+                    hand_over(p_full);
+                };
+                if (ragged) all_weights(std::false_type{});
+                else all_weights(std::true_type{});
                 const uint64_t both = add2(sum[0], sum[1]);
                 l += __uint_as_float((uint32_t)both) + __uint_as_float((uint32_t)(both >> 32));
             }
@@ -505,9 +551,8 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 tc_fence_after();
             }
             if (fetched) q_there();
-            *tell = l;                                                         // (behind o_full, so behind the other team's last reading, too)
-            team_sync<64>(pair);
-            l += *told;
+            say(l);                                                            // (behind o_full, so behind the other team's last reading, too)
+            l += hear();
             team_sync<64>(pair);                                               // (rows go there now)
             const bool cut = u.cut;
             const int opener = u.opener, closer = u.closer;
