@@ -76,7 +76,7 @@ struct AttnShared {
     long long total[5], keys[5];            // of 32 entries each
 };
 struct AttnTotals {
-    int64_t total;                          // tiles, of all heads
+    int total;                              // tiles, of all heads
     int per, runs;                          // requests of an entry; runs of all CTAs
     bool whole;
 };
@@ -114,20 +114,25 @@ __device__ __forceinline__ AttnTotals attn_totals(const AttnParams& p, AttnShare
     }
     __syncthreads();
     if (warp < ATTN_ENTRIES / 32) {
-        long long sum = sh.cost[threadIdx.x];
+        const uint32_t own = sh.cost[threadIdx.x];
+        const uint32_t low = __reduce_add_sync(~0u, own & 0xFFFFu), high = __reduce_add_sync(~0u, own >> 16);
+        if (p.most_parts > 1)
 #pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            sum += __shfl_xor_sync(~0u, sum, o);
-            keys += __shfl_xor_sync(~0u, keys, o);
-        }
-        if (lane == 0) { sh.total[warp] = sum; sh.keys[warp] = keys; }
+            for (int o = 16; o; o >>= 1) keys += __shfl_xor_sync(~0u, keys, o);
+        if (lane == 0) { sh.total[warp] = ((long long)high << 16) + low; sh.keys[warp] = keys; }
     }
     __syncthreads();
-    t.total = keys = 0;
-    for (int w = 0; w < ATTN_ENTRIES / 32; ++w) { t.total += sh.total[w]; keys += sh.keys[w]; }
-    t.total *= p.kv_heads;
+    long long total = keys = 0;
+#pragma unroll
+    for (int w = 0; w < ATTN_ENTRIES / 32; ++w) { total += sh.total[w]; keys += sh.keys[w]; }
+    total *= p.kv_heads;
+    if (total > ATTN_MOST_TILES) {
+        if (threadIdx.x == 0) atomicExch(p.status, 40);
+        total = 0;
+    }
+    t.total = (int)total;
     const int ctas = gridDim.x;
-    t.runs = (int)min((int64_t)ctas * (t.whole ? 1 : attn_parts(t.total, ctas, keys * p.kv_bytes, p.most_parts)), t.total);
+    t.runs = min(t.whole || p.most_parts == 1 ? ctas : ctas * attn_parts(t.total, ctas, keys * p.kv_bytes, p.most_parts), t.total);
     return t;
 }
 
@@ -135,7 +140,7 @@ __device__ __forceinline__ AttnTotals attn_totals(const AttnParams& p, AttnShare
 template <class Cut>
 struct AttnWalk {
     AttnRequest r, next;
-    int64_t lo, hi, unit;
+    int lo, hi, unit;
     int run, block, blocks, request, head, tiles;
 
     __device__ __forceinline__ void fetch(const AttnParams& p, int i)
@@ -150,6 +155,26 @@ struct AttnWalk {
     }
     __device__ __forceinline__ void size(const AttnParams& p) { tiles = attn_block_tiles(r, p.group, block, Cut::ROWS, Cut::TILE); }
 
+    // a lane's `own` tiles behind all lanes in front of it and `at`: the lane with tile lo, and everything in front of it passed
+    __device__ __forceinline__ bool pass(int own, int& at, int& which, int base) const
+    {
+        const int lane = threadIdx.x & 31;
+        int sum = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(~0u, sum, o);
+            if (lane >= o) sum += up;
+        }
+        const uint32_t behind = __ballot_sync(~0u, at + sum > lo);
+        if (behind) {
+            const int l = __ffs(behind) - 1;
+            which = base + l;
+            at += __shfl_sync(~0u, sum - own, l);
+            return true;
+        }
+        at += __shfl_sync(~0u, sum, 31);
+        return false;
+    }
     // the CTA's first run, or its next: false behind the last
     __device__ __forceinline__ bool begin(const AttnParams& p, const AttnTotals& t, const AttnShared& sh) { return seek(p, t, sh, blockIdx.x); }
     __device__ __forceinline__ bool next_run(const AttnParams& p, const AttnTotals& t, const AttnShared& sh) { return seek(p, t, sh, run + gridDim.x); }
@@ -161,64 +186,37 @@ struct AttnWalk {
         hi = attn_run(run + 1, t.total, t.runs);
         const int lane = threadIdx.x & 31;
         // the entry with tile lo, then its request, head and block; everything in front of `at` has been passed
-        long long at = 0;
-        int entry = 0;
+        int at = 0, entry = 0;
         for (int e0 = 0; e0 < ATTN_ENTRIES; e0 += 32) {
-            const long long own = (long long)sh.cost[e0 + lane] * p.kv_heads;
-            long long sum = own;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long up = __shfl_up_sync(~0u, sum, o);
-                if (lane >= o) sum += up;
-            }
-            const uint32_t behind = __ballot_sync(~0u, at + sum > lo);
-            if (behind) {
-                const int l = __ffs(behind) - 1;
-                entry = e0 + l;
-                at += __shfl_sync(~0u, sum - own, l);
-                break;
-            }
-            at += __shfl_sync(~0u, sum, 31);
+            const int own = (int)sh.cost[e0 + lane] * p.kv_heads;
+            if (pass(own, at, entry, e0)) break;
         }
-        uint32_t cost = 0;                                       // of the request in one head
+        int cost = 0;                                            // of the request in one head
         for (request = entry * t.per;; ++request) {
             r = attn_request(p, request);
-            cost = t.per == 1 ? sh.cost[request] : attn_request_cost<Cut>(p, r, t.whole);
-            const long long all = (long long)cost * p.kv_heads;
-            if (at + all > lo || request + 1 >= p.n) break;
-            at += all;
+            cost = t.per == 1 ? (int)sh.cost[request] : (int)attn_request_cost<Cut>(p, r, t.whole);
+            if (at + cost * p.kv_heads > lo || request + 1 >= p.n) break;
+            at += cost * p.kv_heads;
         }
-        blocks = attn_blocks(r, p.group.d, Cut::ROWS);
-        head = (int)((uint32_t)(lo - at) / cost);
-        at += (long long)head * cost;
-        block = 0;
-        for (int b0 = 0; b0 < blocks; b0 += 32) {
-            const int own = b0 + lane < blocks ? attn_unit_cost<Cut>(p, r, b0 + lane, t.whole) : 0;
-            int sum = own;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int up = __shfl_up_sync(~0u, sum, o);
-                if (lane >= o) sum += up;
-            }
-            const uint32_t behind = __ballot_sync(~0u, at + sum > lo);
-            if (behind) {
-                const int l = __ffs(behind) - 1;
-                block = b0 + l;
-                at += __shfl_sync(~0u, sum - own, l);
-                break;
-            }
-            at += __shfl_sync(~0u, sum, 31);
-        }
-        unit = at;
         fetch(p, request + 1);
+        blocks = attn_blocks(r, p.group.d, Cut::ROWS);
+        head = (lo - at) / cost;
+        at += head * cost;
+        block = 0;
+        if (blocks > 1)
+            for (int b0 = 0; b0 < blocks; b0 += 32) {
+                const int own = b0 + lane < blocks ? attn_unit_cost<Cut>(p, r, b0 + lane, t.whole) : 0;
+                if (pass(own, at, block, b0)) break;
+            }
+        unit = at;
         size(p);
         if (!t.whole && lo >= unit + tiles) step(p, t);         // (what is left of the unit is what it costs beside its tiles)
         return true;
     }
     __device__ __forceinline__ bool more() const { return unit < hi; }
     // tiles of the unit that are this run's: [first, end)
-    __device__ __forceinline__ int first() const { return lo <= unit ? 0 : (int)(lo - unit); }
-    __device__ __forceinline__ int end(const AttnTotals& t) const { return t.whole || unit + tiles <= hi ? tiles : (int)(hi - unit); }
+    __device__ __forceinline__ int first() const { return lo <= unit ? 0 : lo - unit; }
+    __device__ __forceinline__ int end(const AttnTotals& t) const { return t.whole || unit + tiles <= hi ? tiles : hi - unit; }
     __device__ __forceinline__ void step(const AttnParams& p, const AttnTotals& t)
     {
         unit += t.whole ? 1 : tiles + Cut::EXTRA;
@@ -265,10 +263,13 @@ __device__ __forceinline__ void attn_spin(uint32_t bar, uint32_t parity, volatil
     }
 }
 
-// looked at once, then suspended: for a wait that is long as a rule, beside warps that need the issue slots
-__device__ __forceinline__ void attn_look(uint32_t bar, uint32_t parity, volatile int* abort, int* status, int code)
+// One more of `counter`, behind everything that the threads of this barrier's sides have stored, and in front of what they read of the others' (the thread
+// that says it releases and acquires for all of them)
+__device__ __forceinline__ uint32_t attn_arrive(uint32_t* counter)
 {
-    if (!bar_test(bar, parity)) attn_wait(bar, parity, abort, status, code);
+    uint32_t before;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+    return before;
 }
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int a, int b, int c, int d, uint32_t bar)

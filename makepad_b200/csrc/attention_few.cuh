@@ -80,24 +80,32 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         uint32_t phase = 1;
         for (bool run = u.begin(p, totals, s_shared); run; run = u.next_run(p, totals, s_shared))
             for (; u.more(); u.step(p, totals)) {
+                // (a tile's pages are looked up while the one before waits for its room)
                 const int32_t* row = p.table + u.request * p.width;
                 const int end = u.end(totals);
+                auto page_of = [&](int t) {
+                    const int key = t * FEW_TILE + box * BOX;
+                    if (what > 1 || t >= end || key >= u.r.keys) return -1;
+                    const int page = row[key >> p.page_shift];
+                    return page < 0 || page >= p.pages ? (int)p.pages : page;                    // (beyond the cache: zeros)
+                };
+                int page = page_of(u.first());
                 for (int t = u.first(); t < end; ++t) {
+                    const int next = page_of(t + 1);
                     attn_wait(empty(s), phase, &s_abort, p.status, 41);
                     __syncwarp();
-                    const int key = t * FEW_TILE + box * BOX;
-                    // what this warp of the tile gets: whole boxes up to the last key
+                    // what a warp of the tile gets: whole boxes up to the last key
                     if (lane < FEW_WARPS) {
-                        const int left = (min(u.r.keys, (t + 1) * FEW_TILE) - t * FEW_TILE - lane * FEW_KEYS + BOX - 1) / BOX;
+                        const int left = (min(u.r.keys - t * FEW_TILE, FEW_TILE) - lane * FEW_KEYS + BOX - 1) / BOX;
                         bar_expect_tx(full(s, lane), 2 * BOX_BYTES * max(0, min(left, PER_WARP)));
                     }
                     __syncwarp();
-                    if (what < 2 && key < u.r.keys) {
-                        const int page = row[key >> p.page_shift], w = box / PER_WARP;
+                    if (page >= 0) {
+                        const int key = t * FEW_TILE + box * BOX, w = box / PER_WARP;
                         const uint32_t dst = smem0 + s * S::STAGE_BYTES + w * 2 * S::WARP_BYTES + what * S::WARP_BYTES + (box % PER_WARP) * BOX_BYTES;
-                        const int at = page < 0 || page >= p.pages ? (int)p.pages : page;        // (beyond the cache: zeros)
-                        tma_load_4d(dst, what ? &map_v : &map_k, 0, key & ((1 << p.page_shift) - 1), 0, at * p.kv_heads + u.head, full(s, w));
+                        tma_load_4d(dst, what ? &map_v : &map_k, 0, key & ((1 << p.page_shift) - 1), 0, page * p.kv_heads + u.head, full(s, w));
                     }
+                    page = next;
                     if (++s == S::STAGES) { s = 0; phase ^= 1u; }
                 }
             }
@@ -270,13 +278,11 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                 }
             }
             if (cut) {
-                __threadfence();
                 few_sync();
                 if (threadIdx.x == 0) {
-                    const uint32_t before = atomicAdd(p.arrived + opener, 1u);
+                    const uint32_t before = attn_arrive(p.arrived + opener);
                     s_last = before == (uint32_t)(closer - opener);
                     if (s_last) p.arrived[opener] = 0;
-                    __threadfence();
                 }
                 few_sync();
                 if (s_last) {

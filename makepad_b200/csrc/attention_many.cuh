@@ -123,13 +123,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
     return v;
 }
-__device__ __forceinline__ uint32_t bf16_pair(uint64_t v)
-{
-    uint32_t w;
-    asm("{\n\t.reg .f32 a, b;\n\tmov.b64 {a, b}, %1;\n\tcvt.rn.bf16x2.f32 %0, b, a;\n\t}" : "=r"(w) : "l"(v));
-    return w;
-}
-__device__ __forceinline__ uint64_t ex2_pair(uint64_t t) { return pair_of(ex2(__uint_as_float((uint32_t)t)), ex2(__uint_as_float((uint32_t)(t >> 32)))); }
 // 2^t of both by multiplications and additions, for t <= 8 (below -126: 2^-126): t = n + f with |f| <= 1/2, by adding and taking away 1.5 * 2^23,
 // whose low bits are then n; 2^f by the polynomial of degree 3 with the least relative error there, 7.5e-5 (a linear programme over 4001
 // points), a twentieth of what bf16 rounds off; n goes into the exponent.
@@ -317,22 +310,25 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             const int h = lane % S::HALVES, box = lane / S::HALVES;
             const uint32_t box_bytes = 128u << shift;                          // of one half
             while (next_unit(u)) {
+                // (a tile's pages are looked up while the one before waits for its room)
                 const int32_t* row = PAGED ? p.table + u.request * p.width : nullptr;
-                for (int j = u.first; j < u.end; ++j) {
+                auto page_of = [&](int j) {
                     const int key = j * MANY_TILE + (box << shift);
-                    const bool mine = box < boxes && key < u.keys;
+                    if (box >= boxes || j >= u.end || key >= u.keys) return -1;
+                    if (!PAGED) return 0;
+                    const int page = row[key >> p.page_shift];
+                    return page < 0 || page >= p.pages ? (int)p.pages : page;  // (beyond the cache: zeros)
+                };
+                int page = page_of(u.first);
+                for (int j = u.first; j < u.end; ++j) {
+                    const int key = j * MANY_TILE + (box << shift), next = page_of(j + 1);
                     const int there = (max(min(u.keys - j * MANY_TILE, MANY_TILE), 0) + (1 << shift) - 1) >> shift;
-                    int page = 0;
-                    if (PAGED && mine) {
-                        page = row[key >> p.page_shift];
-                        if (page < 0 || page >= p.pages) page = (int)p.pages;  // (beyond the cache: zeros)
-                    }
 #pragma unroll
                     for (int what = 0; what < 2; ++what) {
                         attn_wait(kv_empty + 8 * s, phase, &sh.abort, p.status, 57);
                         if (lane == 0) bar_expect_tx(kv_full + 8 * s, there * S::HALVES * box_bytes);
                         __syncwarp();
-                        if (mine) {
+                        if (page >= 0) {
                             const uint32_t dst = smem_kv + s * S::TILE_BYTES + h * S::HALF_BYTES + box * box_bytes;
                             const CUtensorMap* map = what ? &map_v : &map_k;
                             if (PAGED) tma_load_4d(dst, map, 0, key & ((1 << p.page_shift) - 1), h, page * p.kv_heads + u.head, kv_full + 8 * s);
@@ -341,6 +337,7 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                         __syncwarp();
                         if (++s == S::STAGES) { s = 0; phase ^= 1u; }
                     }
+                    page = next;
                 }
             }
         } else {
@@ -480,7 +477,7 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     m = max_nan(top, hear(), -INFINITY);
                     if (m == INFINITY) m = NAN;                                // (what inf - inf would make of the row)
                 }
-                uint64_t sum[2];
+                float sum[2];
                 // group g: sixteen of a block's 32 keys
                 auto weights = [&](const uint32_t (&x)[32], uint32_t (&w)[16], int g, auto with_powers) {
                     constexpr bool POWERS = decltype(with_powers)::value;
@@ -489,10 +486,19 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 #pragma unroll
                     for (int i = 8 * g; i < 8 * g + 8; ++i) {
                         const uint64_t a = fma2(pair_of(x[2 * i], x[2 * i + 1]), scale2, base2);
-                        const uint64_t e = POWERS && i % MANY_POWERS == MANY_POWERS - 1 ? power2(a) : ex2_pair(a);
-                        sum[i & 1] = add2(sum[i & 1], e);
-                        // bf16 is what the tensor cores take beside bf16 values; the sum keeps the weights as they were
-                        w[i] = bf16_pair(e);
+                        float e0, e1;
+                        if (POWERS && i % MANY_POWERS == MANY_POWERS - 1) {
+                            const uint64_t e = power2(a);
+                            e0 = __uint_as_float((uint32_t)e);
+                            e1 = __uint_as_float((uint32_t)(e >> 32));
+                        } else {
+                            e0 = ex2(__uint_as_float((uint32_t)a));
+                            e1 = ex2(__uint_as_float((uint32_t)(a >> 32)));
+                        }
+                        // bf16 is what the tensor cores take beside bf16 values; the sums keep the weights as they were
+                        sum[0] += e0;
+                        sum[1] += e1;
+                        w[i] = pack_bf16(e0, e1);
                     }
                 };
                 auto hand_over = [&](uint32_t bar) {
@@ -503,7 +509,7 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 // What is waited for (the other team's maximum, stores into tensor memory) has a group of weights in front of it
                 auto all_weights = [&](auto with_powers) {
                     uint32_t w[16];
-                    sum[0] = sum[1] = 0;
+                    sum[0] = sum[1] = 0.f;
                     weights(x[0], w, 0, with_powers);
                     if (j > first) top = max_nan(top, hear(), -INFINITY);
                     weights(x[0], w, 1, with_powers);
@@ -526,7 +532,7 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                             tc_ld32(ts + 64 * half, x[0]);
                             tc_ld_wait_for(x[0]);
                             if (ragged) hide(x[0], left);
-                            sum[0] = sum[1] = 0;
+                            sum[0] = sum[1] = 0.f;
                             weights(x[0], w, 0, std::false_type{});
                             weights(x[0], w, 1, std::false_type{});
                         }
@@ -540,8 +546,7 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 };
                 if (ragged) all_weights(std::false_type{});
                 else all_weights(std::true_type{});
-                const uint64_t both = add2(sum[0], sum[1]);
-                l += __uint_as_float((uint32_t)both) + __uint_as_float((uint32_t)(both >> 32));
+                l += sum[0] + sum[1];
             }
             // ---- the unit's end: O, unscaled, and the sums of both halves
             const bool some = first < end, fetched = fetch_q();
@@ -619,13 +624,11 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     head[mine] = m == -INFINITY ? m : m * p.scale_log2;
                     head[MANY_ROWS + mine] = l;
                 }
-                __threadfence();
                 team_sync<256>(9 + t);
                 if ((threadIdx.x & 255) == 0) {
-                    const uint32_t before = atomicAdd(p.arrived + 2 * opener + t, 1u);
+                    const uint32_t before = attn_arrive(p.arrived + 2 * opener + t);
                     sh.last[t] = before == (uint32_t)(closer - opener);
                     if (sh.last[t]) p.arrived[2 * opener + t] = 0;
-                    __threadfence();
                 }
                 team_sync<256>(9 + t);
                 if (sh.last[t]) {

@@ -72,32 +72,30 @@ MPQ_BOTH int attn_block_tiles(const AttnRequest& r, const AttnDivisor& group, in
     return attn_tiles(attn_seen(r, group.of(b * block_rows + attn_block_rows(r, (int)group.d, b, block_rows) - 1)), tile);
 }
 
-// First tile of run v of `runs` (at most `total`), and the run that has tile t.  v * (total % runs) stays below 2^31: there are few runs.
-MPQ_BOTH int64_t attn_run(int v, int64_t total, int runs)
+// First tile of run v of `runs` (at most `total`, and at most ATTN_MOST_RUNS), and the run that has tile t.
+MPQ_BOTH int attn_run(int v, int total, int runs)
 {
-    if (total < (1ll << 32)) {
-        const uint32_t q = (uint32_t)total / (uint32_t)runs, r = (uint32_t)total - q * runs;
-        return (int64_t)v * q + (uint32_t)v * r / (uint32_t)runs;
-    }
-    const int64_t q = total / runs;
-    return v * q + (int64_t)((uint32_t)v * (uint32_t)(total - q * runs) / (uint32_t)runs);
+    const uint32_t q = (uint32_t)total / (uint32_t)runs, r = (uint32_t)total - q * runs;
+    return (int)(v * q + (uint32_t)v * r / (uint32_t)runs);
 }
-MPQ_BOTH int attn_owner(int64_t t, int64_t total, int runs)
+MPQ_BOTH int attn_owner(int t, int total, int runs)
 {
-    if (total < (1ll << 20)) return (int)(((uint32_t)(t + 1) * (uint32_t)runs - 1) / (uint32_t)total);
-    return (int)(((t + 1) * runs - 1) / total);
+    if (total < (1 << 20)) return (int)(((uint32_t)(t + 1) * (uint32_t)runs - 1) / (uint32_t)total);
+    return (int)((((uint64_t)t + 1) * runs - 1) / (uint32_t)total);
 }
 constexpr int ATTN_MOST_RUNS = 2048;
+constexpr int64_t ATTN_MOST_TILES = 1ll << 30;         // of a call: what has more (hours of work) is not begun, and says so in the status word
 
 // Into how many parts, one after the other, all tiles are cut before each part is cut into a run per CTA: so many that the keys and values of a part
 // (in a part are the heads of few requests) stay in L2, but no runs of fewer than ATTN_LEAST_RUN tiles.
 constexpr int64_t ATTN_PART_BYTES = 40 << 20;
 constexpr int ATTN_LEAST_RUN = 48;
-MPQ_BOTH int attn_parts(int64_t total, int ctas, int64_t kv_bytes, int most)
+MPQ_BOTH int attn_parts(int total, int ctas, int64_t kv_bytes, int most)
 {
-    int64_t parts = (kv_bytes + ATTN_PART_BYTES - 1) / ATTN_PART_BYTES;
-    if (parts > total / ((int64_t)ctas * ATTN_LEAST_RUN)) parts = total / ((int64_t)ctas * ATTN_LEAST_RUN);
-    return parts < 1 ? 1 : parts > most ? most : (int)parts;
+    int parts = total / (ctas * ATTN_LEAST_RUN);
+    if (parts > most) parts = most;
+    for (; parts > 1 && (parts - 1) * ATTN_PART_BYTES >= kv_bytes;) --parts;
+    return parts < 1 ? 1 : parts;
 }
 
 }  // namespace mpq

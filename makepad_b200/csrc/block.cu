@@ -254,7 +254,7 @@ static int32_t attention_many(mpq_context* ctx, AttnParams p, const AttnKeys& kv
     const int ctas = std::min(ctx->prop.multiProcessorCount, FEW_MOST_CTAS);
     p.kv_bytes = 4ll * p.kv_heads * D;
     const int64_t keys = PAGED ? kv.pages * kv.page_size : p.tokens;
-    attention_scratch(ctx, &p, ctas, ManyShape<D>::PIECE, attn_parts(MOST, ctas, keys * p.kv_bytes, PARTS), s);
+    attention_scratch(ctx, &p, ctas, ManyShape<D>::PIECE, attn_parts((int)MOST, ctas, keys * p.kv_bytes, PARTS), s);
     static PerDeviceOnce raised;
     if (raised.needs(ctx->device)) {
         CU_TRY(ctx, cudaFuncSetAttribute(attention_many_kernel<D, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, ManyShape<D>::SMEM));

@@ -19,19 +19,20 @@ int main()
     long bad = 0;
     for (int trial = 0; trial < 4000; ++trial) {
         // owners of tiles agree with the runs, for fewer and for more tiles than CTAs
-        const int64_t total = trial % 5 == 0 ? (int64_t)pick(1, 1000000) * pick(1, 1000000) : pick(1, trial % 2 ? 300 : 100000);
+        const int total = trial % 5 == 0 ? pick(1, 1 << 30) : pick(1, trial % 2 ? 300 : 100000);
         const int ctas0 = pick(1, trial % 3 ? 160 : 1024), ctas = (int)(ctas0 < total ? ctas0 : total);
         if (attn_run(0, total, ctas) != 0 || attn_run(ctas, total, ctas) != total) ++bad;
         for (int c = 0; c < ctas; ++c) {
-            const int64_t lo = attn_run(c, total, ctas), hi = attn_run(c + 1, total, ctas);
+            const int lo = attn_run(c, total, ctas), hi = attn_run(c + 1, total, ctas);
             if (lo >= hi) ++bad;
             if (attn_owner(lo, total, ctas) != c || attn_owner(hi - 1, total, ctas) != c) ++bad;
         }
     }
-    if (attn_owner((1ll << 46) - 1, 1ll << 46, 148) != 147) ++bad;
+    if (attn_owner((1 << 30) - 1, 1 << 30, ATTN_MOST_RUNS) != ATTN_MOST_RUNS - 1) ++bad;
     // parts: one for little work or few keys, never runs of fewer tiles than ATTN_LEAST_RUN unless there is one part
     for (int trial = 0; trial < 2000; ++trial) {
-        const int64_t total = pick(1, 1 << 20), bytes = (int64_t)pick(0, 1 << 20) << 10;
+        const int total = pick(1, 1 << 20);
+        const int64_t bytes = (int64_t)pick(0, 1 << 20) << 10;
         const int ctas = pick(1, 256), parts = attn_parts(total, ctas, bytes, 4);
         if (parts < 1 || parts > 4 || (parts > 1 && (total / parts / ctas < ATTN_LEAST_RUN || (parts - 1) * ATTN_PART_BYTES >= bytes))) ++bad;
     }
