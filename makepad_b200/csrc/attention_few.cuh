@@ -1,31 +1,33 @@
 // Attention of few rows (one token, or a handful, per request and head of keys) over the pages of a cache: the cache is read once, at HBM's rate.
 //
-// A block is 16 rows, the M of mma.sync.m16n8k16; with one row a head the other fifteen are idle, and still the tensor work of 32 keys (64 MMAs) is
-// under a fifth of the time that their 16 KB take to arrive at an SM's share of the memory bandwidth.  (tcgen05 wants 128 rows, or the keys as its M operand and
-// the weights through shared memory, for nothing that is missing here.)
+// The KEYS are the M of mma.sync.m16n8k16 and up to 8 (or 16) rows its N: S^T = K Q^T, O^T += V^T P^T.  A tile of 128 keys is 256 MMAs (512 with 16 rows) for the
+// 64 KB (D = 128) that take an SM 2700 cycles of its share of the memory bandwidth.  With the rows as M, most of them idle, twice
+// the MMAs took 2150 cycles a tile, and no stall of the memory was ever caught up.  (tcgen05 wants 128 rows, or the weights
+// through shared memory, for nothing that is missing here.)
 //
 // A CTA has one producer warp and four warps that compute, 32 of a tile's 128 keys each.  The producer looks up the pages and keeps a ring of tiles full
-// (TMA, 128-byte swizzle; it runs ahead into the next unit), each warp waits for its own keys only.  Scores stay in registers: the accumulators of q k^T are the
-// A operand of the product with v.  At a unit's end the four warps' (maximum, sum, o) are joined through shared memory.
+// (TMA, 128-byte swizzle; it runs ahead into the next unit), each warp waits for its own keys only.  Weights stay in registers: transposed 8 x 8 at a
+// time (movmatrix), the accumulators of K Q^T are the B operand of the product with V^T.  At a unit's end the four warps' (maximum, sum, o) are
+// joined through shared memory.
 #pragma once
 #include "attention.cuh"
 
 namespace mpq {
 
-constexpr int FEW_MOST_CTAS = 256, FEW_ROWS = 16, FEW_TILE = 128, FEW_WARPS = 4, FEW_KEYS = FEW_TILE / FEW_WARPS, FEW_THREADS = 32 * (FEW_WARPS + 1);
+constexpr int FEW_MOST_CTAS = 256, FEW_TILE = 128, FEW_WARPS = 4, FEW_KEYS = FEW_TILE / FEW_WARPS, FEW_THREADS = 32 * (FEW_WARPS + 1);
+// a unit's end (sums joined, pieces stored and counted) takes a CTA about as long as two tiles
+template <int NT>
+using FewCut = AttnCut<8 * NT, FEW_TILE, 2, false>;
 static_assert(FEW_THREADS >= ATTN_ENTRIES, "an entry per thread");
 
-using FewCut = AttnCut<FEW_ROWS, FEW_TILE, 0, false>;
-
-template <int D>
+template <int D, int NT>
 struct FewShape {
+    static constexpr int ROWS = 8 * NT;
     static constexpr int WARP_BYTES = FEW_KEYS * D * 2;                      // keys (or values) of one warp
     static constexpr int STAGE_BYTES = 2 * FEW_WARPS * WARP_BYTES;           // [warp][k | v]
     static constexpr int STAGES = D == 128 ? 3 : 6;
-    // the warps' parts of o; the factors of a cut unit's pieces and up to sixteen rows of sums
-    static constexpr int JOIN_BYTES = 4 * (FEW_WARPS * FEW_ROWS * D > FEW_ROWS * FEW_MOST_CTAS + FEW_ROWS * D ? FEW_WARPS * FEW_ROWS * D : FEW_ROWS * FEW_MOST_CTAS + FEW_ROWS * D);
-    static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + JOIN_BYTES;
-    static constexpr int PIECE = FEW_ROWS * (D + 2);                         // floats of a piece in scratch: o, maxima, sums
+    static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + FEW_WARPS * ROWS * D * 4;      // ... and the warps' parts of o
+    static constexpr int PIECE = ROWS * (D + 2);                             // floats of a piece in scratch: o, maxima, sums
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr)
@@ -36,6 +38,12 @@ __device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t addr)
 {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
+__device__ __forceinline__ uint32_t transposed(uint32_t v)
+{
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -43,17 +51,18 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], 
 }
 __device__ __forceinline__ void few_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * FEW_WARPS) : "memory"); }
 
-// BOX: keys per copy, 16 or 32 (a page of 16, or larger ones)
-template <int D, int BOX>
+// NT: rows in eights.  BOX: keys per copy, 16 or 32 (a page of 16, or larger ones)
+template <int D, int BOX, int NT>
 __global__ void __launch_bounds__(FEW_THREADS, 1)
 attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnParams p)
 {
-    using S = FewShape<D>;
+    using S = FewShape<D, NT>;
+    constexpr int ROWS = S::ROWS;
     extern __shared__ unsigned char smem_dyn[];
     __shared__ volatile int s_abort;
     __shared__ int s_last;
     __shared__ AttnShared s_shared;
-    __shared__ float s_max[FEW_WARPS][FEW_ROWS], s_sum[FEW_WARPS][FEW_ROWS];
+    __shared__ float s_max[FEW_WARPS][ROWS], s_sum[FEW_WARPS][ROWS];
     __shared__ __align__(8) uint64_t s_bars[S::STAGES * (FEW_WARPS + 1)];
     const uint32_t smem0 = (s2u(smem_dyn) + 1023u) & ~1023u, bars = s2u(s_bars);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -69,8 +78,8 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     }
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const AttnTotals totals = attn_totals<FewCut>(p, s_shared);              // (its barriers publish the mbarriers)
-    AttnWalk<FewCut> u;
+    const AttnTotals totals = attn_totals<FewCut<NT>>(p, s_shared);          // (its barriers publish the mbarriers)
+    AttnWalk<FewCut<NT>> u;
 
     if (warp == FEW_WARPS) {
         // ---- producer: lane = (box of a tile, k or v); boxes behind the request's last key are not fetched
@@ -110,40 +119,43 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                 }
             }
     } else {
-        const int g = lane >> 2, tq = lane & 3;
+        const int g = lane >> 2, tq = lane & 3;              // an accumulator's lane: key (or column of o) g and g + 8, rows 2 tq and 2 tq + 1
+        const int km = lane >> 3, kr = lane & 7;             // ldmatrix: matrix and row that the lane points to
         float* join = reinterpret_cast<float*>(smem_dyn + (smem0 - s2u(smem_dyn)) + S::STAGES * S::STAGE_BYTES);
-        // ldmatrix: lane -> row of the matrix that it points to
-        const int km = lane >> 3, kr = lane & 7;
         int s = 0;
         uint32_t phase = 0;
         for (bool run = u.begin(p, totals, s_shared); run; run = u.next_run(p, totals, s_shared))
         for (; u.more(); u.step(p, totals)) {
-            const int rows = attn_block_rows(u.r, p.group.d, u.block, FEW_ROWS);
-            const int row0 = u.block * FEW_ROWS;
-            // keys that rows g and g + 8 see
-            const int seen0 = attn_seen(u.r, p.group.of(row0 + min(g, rows - 1))), seen1 = attn_seen(u.r, p.group.of(row0 + min(g + 8, rows - 1)));
-            const int seen_all = attn_seen(u.r, p.group.of(row0));             // by every row of the block
-            uint32_t qa[D / 16][4];
-            {
-                auto row_of = [&](int r) {
-                    const int at = row0 + min(r, rows - 1), tok = p.group.of(at);
-                    return p.q + (int64_t)(u.r.first + tok) * p.q_stride + ((u.head - tok) * (int)p.group.d + at) * D + 2 * tq;
-                };
-                const __nv_bfloat16 *q0 = row_of(g), *q1 = row_of(g + 8);
+            const int rows = attn_block_rows(u.r, p.group.d, u.block, ROWS);
+            const int row0 = u.block * ROWS;
+            // keys that the rows see: this lane's, and every row of the block
+            int seen[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) seen[n][i] = attn_seen(u.r, p.group.of(row0 + min(8 * n + 2 * tq + i, rows - 1)));
+            const int seen_all = attn_seen(u.r, p.group.of(row0));
+            uint32_t q[NT][D / 16][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int at = row0 + min(8 * n + g, rows - 1), tok = p.group.of(at);
+                const __nv_bfloat16* from = p.q + (int64_t)(u.r.first + tok) * p.q_stride + ((u.head - tok) * (int)p.group.d + at) * D + 2 * tq;
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
-                    qa[k][0] = *reinterpret_cast<const uint32_t*>(q0 + 16 * k);
-                    qa[k][1] = *reinterpret_cast<const uint32_t*>(q1 + 16 * k);
-                    qa[k][2] = *reinterpret_cast<const uint32_t*>(q0 + 16 * k + 8);
-                    qa[k][3] = *reinterpret_cast<const uint32_t*>(q1 + 16 * k + 8);
+                    q[n][k][0] = *reinterpret_cast<const uint32_t*>(from + 16 * k);
+                    q[n][k][1] = *reinterpret_cast<const uint32_t*>(from + 16 * k + 8);
                 }
             }
-            float o[D / 8][4];
+            float o[D / 16][NT][4], m[NT][2], l[NT][2];
 #pragma unroll
-            for (int i = 0; i < D / 8; ++i)
+            for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
-            float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+                for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[c][n][j] = 0.f;
+                m[n][0] = m[n][1] = -INFINITY;
+                l[n][0] = l[n][1] = 0.f;
+            }
             const int end = u.end(totals);
             for (int t = u.first(); t < end; ++t) {
                 attn_wait(full(s, warp), phase, &s_abort, p.status, 42);
@@ -153,77 +165,85 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                 auto place_of = [&](uint32_t base, int r, int c) {
                     return base + (r / BOX) * (BOX * D * 2) + (c >> 3) * (BOX * 128) + (r % BOX) * 128 + (((c & 7) ^ (r & 7)) << 4);
                 };
-                float sc[4][4];
+                float sc[2][NT][4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) sc[i][j] = 0.f;
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) sc[h][n][j] = 0.f;
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        uint32_t b[4];
-                        ldsm4(b, place_of(kb, 16 * h + (km >> 1) * 8 + kr, 2 * k + (km & 1)));
-                        mma_bf16(sc[2 * h], qa[k], b[0], b[1]);
-                        mma_bf16(sc[2 * h + 1], qa[k], b[2], b[3]);
+                        uint32_t a[4];
+                        ldsm4(a, place_of(kb, 16 * h + (km & 1) * 8 + kr, 2 * k + (km >> 1)));
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma_bf16(sc[h][n], a, q[n][k][0], q[n][k][1]);
                     }
+                const bool ragged = key0 + FEW_KEYS > seen_all;
+                float x[NT][2];
+                bool moved = false;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) sc[i][j] *= p.scale_log2;
-                if (key0 + FEW_KEYS > seen_all) {
+                    for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
+                        for (int j = 0; j < 4; ++j) {
+                            sc[h][n][j] *= p.scale_log2;
+                            if (ragged && key0 + 16 * h + g + 8 * (j >> 1) >= seen[n][j & 1]) sc[h][n][j] = -INFINITY;
+                        }
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            if (key0 + 8 * i + 2 * tq + (j & 1) >= (j < 2 ? seen0 : seen1)) sc[i][j] = -INFINITY;
+                    for (int i = 0; i < 2; ++i) {
+                        x[n][i] = fmaxf(m[n][i], fmaxf(fmaxf(sc[0][n][i], sc[0][n][i + 2]), fmaxf(sc[1][n][i], sc[1][n][i + 2])));
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1) x[n][i] = fmaxf(x[n][i], __shfl_xor_sync(~0u, x[n][i], d));
+                        moved |= x[n][i] != m[n][i];
+                    }
                 }
-                float x0 = m0, x1 = m1;
+                if (__any_sync(~0u, moved)) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x0 = fmaxf(x0, fmaxf(sc[i][0], sc[i][1]));
-                    x1 = fmaxf(x1, fmaxf(sc[i][2], sc[i][3]));
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const float f = x[n][i] == -INFINITY ? 1.f : exp2f(m[n][i] - x[n][i]);
+                            m[n][i] = x[n][i];
+                            l[n][i] *= f;
+#pragma unroll
+                            for (int c = 0; c < D / 16; ++c) { o[c][n][i] *= f; o[c][n][i + 2] *= f; }
+                        }
                 }
+                uint32_t pb[2][NT][2];
 #pragma unroll
-                for (int d = 1; d < 4; d <<= 1) {
-                    x0 = fmaxf(x0, __shfl_xor_sync(~0u, x0, d));
-                    x1 = fmaxf(x1, __shfl_xor_sync(~0u, x1, d));
-                }
-                if (__any_sync(~0u, x0 != m0 || x1 != m1)) {
-                    const float a0 = x0 == -INFINITY ? 1.f : exp2f(m0 - x0), a1 = x1 == -INFINITY ? 1.f : exp2f(m1 - x1);
-                    m0 = x0; m1 = x1;
-                    l0 *= a0; l1 *= a1;
+                for (int n = 0; n < NT; ++n) {
+                    const float b0 = m[n][0] == -INFINITY ? 0.f : m[n][0], b1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
 #pragma unroll
-                    for (int i = 0; i < D / 8; ++i) { o[i][0] *= a0; o[i][1] *= a0; o[i][2] *= a1; o[i][3] *= a1; }
-                }
-                const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;
-                uint32_t pa[2][4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float e0 = exp2f(sc[i][0] - b0), e1 = exp2f(sc[i][1] - b0), e2 = exp2f(sc[i][2] - b1), e3 = exp2f(sc[i][3] - b1);
-                    l0 += e0 + e1;
-                    l1 += e2 + e3;
-                    // bf16 is what the tensor cores take beside bf16 values; the sum keeps the weights as they were
-                    pa[i >> 1][2 * (i & 1)] = pack_bf16(e0, e1);
-                    pa[i >> 1][2 * (i & 1) + 1] = pack_bf16(e2, e3);
+                    for (int h = 0; h < 2; ++h) {
+                        const float e0 = exp2f(sc[h][n][0] - b0), e1 = exp2f(sc[h][n][1] - b1), e2 = exp2f(sc[h][n][2] - b0), e3 = exp2f(sc[h][n][3] - b1);
+                        l[n][0] += e0 + e2;
+                        l[n][1] += e1 + e3;
+                        // bf16 is what the tensor cores take beside bf16 values; the sum keeps the weights as they were
+                        pb[h][n][0] = transposed(pack_bf16(e0, e1));
+                        pb[h][n][1] = transposed(pack_bf16(e2, e3));
+                    }
                 }
                 const int left = u.r.keys - key0;                            // keys of this warp that exist
 #pragma unroll
                 for (int c = 0; c < D / 16; ++c)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        uint32_t b[4];
-                        ldsm4_trans(b, place_of(vb, 16 * h + (km & 1) * 8 + kr, 2 * c + (km >> 1)));
+                        uint32_t a[4];
+                        ldsm4_trans(a, place_of(vb, 16 * h + (km >> 1) * 8 + kr, 2 * c + (km & 1)));
                         if (left < FEW_KEYS) {                               // values behind the last key may be anything, and 0 * NaN is not 0
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
-                                const int key = 16 * h + (j & 1) * 8 + 2 * tq;
-                                if (key >= left) b[j] = 0;
-                                else if (key + 1 >= left) b[j] &= 0xFFFFu;
+                                const int key = 16 * h + (j >> 1) * 8 + 2 * tq;
+                                if (key >= left) a[j] = 0;
+                                else if (key + 1 >= left) a[j] &= 0xFFFFu;
                             }
                         }
-                        mma_bf16(o[2 * c], pa[h], b[0], b[1]);
-                        mma_bf16(o[2 * c + 1], pa[h], b[2], b[3]);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma_bf16(o[c][n], a, pb[h][n][0], pb[h][n][1]);
                     }
                 __syncwarp();
                 if (lane == 0) bar_arrive(empty(s));
@@ -231,50 +251,60 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             }
             // ---- the four warps' parts: maxima, then everything at the common one
 #pragma unroll
-            for (int d = 1; d < 4; d <<= 1) {
-                l0 += __shfl_xor_sync(~0u, l0, d);
-                l1 += __shfl_xor_sync(~0u, l1, d);
-            }
-            if (tq == 0) {
-                s_max[warp][g] = m0; s_max[warp][g + 8] = m1;
-                s_sum[warp][g] = l0; s_sum[warp][g + 8] = l1;
-            }
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) l[n][i] += __shfl_xor_sync(~0u, l[n][i], d);
+                    if (g == 0) { s_max[warp][8 * n + 2 * tq + i] = m[n][i]; s_sum[warp][8 * n + 2 * tq + i] = l[n][i]; }
+                }
             few_sync();
             auto top_of = [&](int r) { return fmaxf(fmaxf(s_max[0][r], s_max[1][r]), fmaxf(s_max[2][r], s_max[3][r])); };
             auto factor = [&](float m, float top) { return m == -INFINITY ? 0.f : exp2f(m - top); };
-            const float f0 = factor(m0, top_of(g)), f1 = factor(m1, top_of(g + 8));
 #pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-                // columns of a row in eights, their order turned by the row: the eight rows of a store lie in different banks
-                float* at = join + (warp * FEW_ROWS + g) * D + (((i ^ g) & 7) | (i & ~7)) * 8 + 2 * tq;
-                *reinterpret_cast<float2*>(at) = make_float2(o[i][0] * f0, o[i][1] * f0);
-                *reinterpret_cast<float2*>(at + 8 * D) = make_float2(o[i][2] * f1, o[i][3] * f1);
-            }
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int r = 8 * n + 2 * tq + i;
+                    const float f = factor(m[n][i], top_of(r));
+                    // (columns of a row in eights, turned by the row: the lanes of a store lie in different banks)
+                    float* at = join + (warp * ROWS + r) * D;
+                    if (r < rows)
+#pragma unroll
+                        for (int c = 0; c < D / 16; ++c) {
+                            at[(16 * c + g) ^ (8 * tq)] = o[c][n][i] * f;
+                            at[(16 * c + 8 + g) ^ (8 * tq)] = o[c][n][i + 2] * f;
+                        }
+                }
             few_sync();
             const bool cut = u.cut(totals);
             const int opener = cut ? u.opener(totals) : 0, closer = cut ? u.closer(totals) : 0;
-            // a row's columns and what stands beside them; `slot` of scratch: the unit that a run opened, or the one that it continues
+            // a row's columns; `slot` of scratch: the unit that a run opened, or the one that it continues
             auto slot = [&](int r) { return p.partial + (int64_t)(2 * r + (r == opener ? 1 : 0)) * S::PIECE; };
-            auto store = [&](int r, int c, float v) {
+            auto store = [&](int r, int c, float4 v) {
                 const int at = row0 + r, tok = p.group.of(at);
                 const int64_t to = ((int64_t)(u.r.first + tok) * p.q_heads + (u.head - tok) * (int)p.group.d + at) * D + c;
-                if (p.out_f32) static_cast<float*>(p.out)[to] = v;
-                else static_cast<__nv_bfloat16*>(p.out)[to] = __float2bfloat16_rn(v);
+                if (p.out_f32) *reinterpret_cast<float4*>(static_cast<float*>(p.out) + to) = v;
+                else *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + to) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
             };
-            for (int e = threadIdx.x; e < rows * D; e += 32 * FEW_WARPS) {
-                const int r = e / D, c = e % D, place = ((((c >> 3) ^ (r & 7)) & 7) | ((c >> 3) & ~7)) * 8 + (c & 7);
-                float v = 0.f, l = 0.f;
+            for (int e = threadIdx.x; e < rows * (D / 4); e += 32 * FEW_WARPS) {
+                const int r = e / (D / 4), c = e % (D / 4) * 4;
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                float l = 0.f;
                 const float top = top_of(r);
 #pragma unroll
                 for (int w = 0; w < FEW_WARPS; ++w) {
-                    v += join[(w * FEW_ROWS + r) * D + place];
+                    const float4 a = *reinterpret_cast<const float4*>(join + (w * ROWS + r) * D + (c ^ (8 * ((r >> 1) & 3))));
+                    v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
                     l += s_sum[w][r] * factor(s_max[w][r], top);
                 }
-                if (!cut) store(r, c, l == 0.f ? 0.f : v / l);
-                else {
+                if (!cut) {
+                    const float f = l == 0.f ? 0.f : 1.f / l;
+                    store(r, c, make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
+                } else {
                     float* mine = slot(u.run);
-                    mine[r * D + c] = v;
-                    if (c == 0) { mine[FEW_ROWS * D + r] = top; mine[FEW_ROWS * D + FEW_ROWS + r] = l; }
+                    *reinterpret_cast<float4*>(mine + r * D + c) = v;
+                    if (c == 0) { mine[ROWS * D + r] = top; mine[ROWS * D + ROWS + r] = l; }
                 }
             }
             if (cut) {
@@ -285,56 +315,41 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                     if (s_last) p.arrived[opener] = 0;
                 }
                 few_sync();
-                if (s_last) {
-                    // Factors of the pieces' rows; then one, two or four groups of threads add their part of the pieces each, in order, and the
-                    // groups' sums are added in order.
-                    const int pieces = closer - opener + 1;
-                    float *fac = join, *acc = join + FEW_ROWS * FEW_MOST_CTAS;
-                    for (int i = threadIdx.x; i < rows * pieces; i += 32 * FEW_WARPS) {
-                        const int q = i / rows, r = i - q * rows;
-                        fac[q * FEW_ROWS + r] = __ldcg(slot(opener + q) + FEW_ROWS * D + r);
-                    }
-                    few_sync();
-                    if ((int)threadIdx.x < rows) {
-                        const int r = threadIdx.x;
-                        float top = -INFINITY, l = 0.f;
-                        for (int q = 0; q < pieces; ++q) top = fmaxf(top, fac[q * FEW_ROWS + r]);
-#pragma unroll 4
-                        for (int q = 0; q < pieces; ++q) {
-                            const float f = factor(fac[q * FEW_ROWS + r], top);
-                            fac[q * FEW_ROWS + r] = f;
-                            l = fmaf(f, __ldcg(slot(opener + q) + FEW_ROWS * D + FEW_ROWS + r), l);
-                        }
-                        s_sum[0][r] = l;
-                    }
-                    few_sync();
-                    const int groups = rows <= 4 ? 4 : rows <= 8 ? 2 : 1, each = 32 * FEW_WARPS / groups, group = threadIdx.x / each;
-                    const int q0 = pieces * group / groups, q1 = pieces * (group + 1) / groups;
-                    for (int e = threadIdx.x - group * each; e < rows * D / 4; e += each) {
-                        const int r = e / (D / 4);
+                if (s_last)
+                    // the pieces in order, eight at a time (all their loads in one latency), rescaled when a larger maximum comes
+                    for (int e = threadIdx.x; e < rows * (D / 4); e += 32 * FEW_WARPS) {
+                        const int r = e / (D / 4), c = e % (D / 4) * 4;
                         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                        for (int q = q0; q < q1; q += 4) {
-                            float4 a[4];
+                        float top = -INFINITY, l = 0.f;
+                        for (int r0 = opener; r0 <= closer; r0 += 8) {
+                            float4 a[8];
+                            float pm[8], pl[8], both = top;
 #pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                if (q + k < q1) a[k] = __ldcg(reinterpret_cast<const float4*>(slot(opener + q + k)) + e);
+                            for (int k = 0; k < 8; ++k) {
+                                pm[k] = -INFINITY;
+                                if (r0 + k <= closer) {
+                                    const float* from = slot(r0 + k);
+                                    pm[k] = __ldcg(from + ROWS * D + r);
+                                    pl[k] = __ldcg(from + ROWS * D + ROWS + r);
+                                    a[k] = __ldcg(reinterpret_cast<const float4*>(from + r * D + c));
+                                }
+                            }
 #pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                if (q + k < q1) {
-                                    const float f = fac[(q + k) * FEW_ROWS + r];
-                                    v.x = fmaf(a[k].x, f, v.x); v.y = fmaf(a[k].y, f, v.y); v.z = fmaf(a[k].z, f, v.z); v.w = fmaf(a[k].w, f, v.w);
+                            for (int k = 0; k < 8; ++k) both = fmaxf(both, pm[k]);
+                            const float f = factor(top, both);
+                            top = both;
+                            l *= f; v.x *= f; v.y *= f; v.z *= f; v.w *= f;
+#pragma unroll
+                            for (int k = 0; k < 8; ++k)
+                                if (r0 + k <= closer) {
+                                    const float h = factor(pm[k], top);
+                                    l = fmaf(pl[k], h, l);
+                                    v.x = fmaf(a[k].x, h, v.x); v.y = fmaf(a[k].y, h, v.y); v.z = fmaf(a[k].z, h, v.z); v.w = fmaf(a[k].w, h, v.w);
                                 }
                         }
-                        reinterpret_cast<float4*>(acc)[group * (rows * D / 4) + e] = v;
+                        const float f = l == 0.f ? 0.f : 1.f / l;
+                        store(r, c, make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
                     }
-                    few_sync();
-                    for (int e = threadIdx.x; e < rows * D; e += 32 * FEW_WARPS) {
-                        float v = 0.f;
-                        for (int w = 0; w < groups; ++w) v += acc[w * rows * D + e];
-                        const float l = s_sum[0][e / D];
-                        store(e / D, e % D, l == 0.f ? 0.f : v / l);
-                    }
-                }
             }
             few_sync();                                                      // the next unit writes what this one's threads read
         }

@@ -229,20 +229,20 @@ static bool rows_map(CUtensorMap* map, const void* base, int64_t tokens, int64_t
     return make_bf16_map(map, base, 4, dims, strides, box);
 }
 
-template <int D, int BOX>
+template <int D, int BOX, int NT>
 static int32_t attention_few(mpq_context* ctx, AttnParams p, const AttnKeys& kv, cudaStream_t s)
 {
     const int ctas = std::min(ctx->prop.multiProcessorCount, FEW_MOST_CTAS);
-    attention_scratch(ctx, &p, ctas, FewShape<D>::PIECE, 1, s);
+    attention_scratch(ctx, &p, ctas, FewShape<D, NT>::PIECE, 1, s);
     static PerDeviceOnce raised;
     if (raised.needs(ctx->device)) {
-        CU_TRY(ctx, cudaFuncSetAttribute(attention_few_kernel<D, BOX>, cudaFuncAttributeMaxDynamicSharedMemorySize, FewShape<D>::SMEM));
+        CU_TRY(ctx, cudaFuncSetAttribute(attention_few_kernel<D, BOX, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, FewShape<D, NT>::SMEM));
         raised.mark(ctx->device);
     }
     CUtensorMap map_k, map_v;
     if (!cache_map(&map_k, kv.k, kv, p.kv_heads, D, BOX, D / 64) || !cache_map(&map_v, kv.v, kv, p.kv_heads, D, BOX, D / 64)) return fail(ctx, MPQ_ERR_CUDA, "cuTensorMapEncodeTiled failed for the cache");
     ctx->launches += 1;
-    CU_TRY(ctx, launch_beside(ctx, attention_few_kernel<D, BOX>, dim3(ctas), FEW_THREADS, FewShape<D>::SMEM, 1, s, map_k, map_v, p));
+    CU_TRY(ctx, launch_beside(ctx, attention_few_kernel<D, BOX, NT>, dim3(ctas), FEW_THREADS, FewShape<D, NT>::SMEM, 1, s, map_k, map_v, p));
     return MPQ_OK;
 }
 
@@ -277,9 +277,13 @@ static int32_t attention_launch(mpq_context* ctx, const AttnParams& p, const Att
     const OnDevice on(ctx->device);
     CU_TRY(ctx, on.error);
     const int64_t most_new = kv.max_new > 0 ? std::min(kv.max_new, p.tokens) : p.tokens;
-    if (p.table && most_new * p.group.d <= FEW_ROWS) {
-        if (head_dim == 64) return kv.page_size == 16 ? attention_few<64, 16>(ctx, p, kv, s) : attention_few<64, 32>(ctx, p, kv, s);
-        return kv.page_size == 16 ? attention_few<128, 16>(ctx, p, kv, s) : attention_few<128, 32>(ctx, p, kv, s);
+    const int64_t rows = most_new * p.group.d;
+    if (p.table && rows <= 16) {
+        const bool wide = head_dim == 128, small = kv.page_size == 16;
+        if (rows <= 8) return wide ? (small ? attention_few<128, 16, 1>(ctx, p, kv, s) : attention_few<128, 32, 1>(ctx, p, kv, s))
+                                   : (small ? attention_few<64, 16, 1>(ctx, p, kv, s) : attention_few<64, 32, 1>(ctx, p, kv, s));
+        return wide ? (small ? attention_few<128, 16, 2>(ctx, p, kv, s) : attention_few<128, 32, 2>(ctx, p, kv, s))
+                    : (small ? attention_few<64, 16, 2>(ctx, p, kv, s) : attention_few<64, 32, 2>(ctx, p, kv, s));
     }
     if (p.table) return head_dim == 64 ? attention_many<64, true>(ctx, p, kv, s) : attention_many<128, true>(ctx, p, kv, s);
     return head_dim == 64 ? attention_many<64, false>(ctx, p, kv, s) : attention_many<128, false>(ctx, p, kv, s);
