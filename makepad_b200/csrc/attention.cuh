@@ -49,10 +49,11 @@ __device__ __forceinline__ AttnRequest attn_request(const AttnParams& p, int i)
     return attn_request(p.starts[i], p.starts[i + 1], p.tokens, p.lens != nullptr, p.lens ? p.lens[i] : 0, p.width << p.page_shift);
 }
 
-// How a kernel cuts its work: rows of a block, keys of a tile, what a unit costs beside its tiles, and whether a request may have many blocks
-template <int ROWS_, int TILE_, int EXTRA_, bool MANY_>
+// How a kernel cuts its work: rows of a block, keys of a tile, what a unit costs beside its tiles, tiles that a piece has at least, and whether a
+// request may have many blocks
+template <int ROWS_, int TILE_, int EXTRA_, int LEAST_, bool MANY_>
 struct AttnCut {
-    static constexpr int ROWS = ROWS_, TILE = TILE_, EXTRA = EXTRA_;
+    static constexpr int ROWS = ROWS_, TILE = TILE_, EXTRA = EXTRA_, LEAST = LEAST_;
     static constexpr bool MANY = MANY_;
 };
 template <class Cut>
@@ -210,13 +211,13 @@ struct AttnWalk {
             }
         unit = at;
         size(p);
-        if (!t.whole && lo >= unit + tiles) step(p, t);         // (what is left of the unit is what it costs beside its tiles)
+        if (!t.whole && attn_first(lo, unit, tiles, Cut::LEAST) == tiles) step(p, t);      // (what the run has of the unit is not worth a piece, or beside its tiles)
         return true;
     }
-    __device__ __forceinline__ bool more() const { return unit < hi; }
+    __device__ __forceinline__ bool more(const AttnTotals& t) const { return unit < hi && (t.whole || !attn_behind(hi, unit, tiles, Cut::LEAST)); }
     // tiles of the unit that are this run's: [first, end)
-    __device__ __forceinline__ int first() const { return lo <= unit ? 0 : lo - unit; }
-    __device__ __forceinline__ int end(const AttnTotals& t) const { return t.whole || unit + tiles <= hi ? tiles : hi - unit; }
+    __device__ __forceinline__ int first(const AttnTotals& t) const { return t.whole || lo <= unit ? 0 : attn_first(lo, unit, tiles, Cut::LEAST); }
+    __device__ __forceinline__ int end(const AttnTotals& t) const { return t.whole ? tiles : attn_end(hi, unit, tiles, Cut::LEAST); }
     __device__ __forceinline__ void step(const AttnParams& p, const AttnTotals& t)
     {
         unit += t.whole ? 1 : tiles + Cut::EXTRA;
@@ -234,9 +235,9 @@ struct AttnWalk {
         size(p);
     }
     // whether other runs have tiles of the unit, and the runs that have some
-    __device__ __forceinline__ bool cut(const AttnTotals& t) const { return !t.whole && (unit < lo || unit + tiles > hi); }
-    __device__ __forceinline__ int opener(const AttnTotals& t) const { return attn_owner(unit, t.total, t.runs); }
-    __device__ __forceinline__ int closer(const AttnTotals& t) const { return attn_owner(unit + tiles - 1, t.total, t.runs); }
+    __device__ __forceinline__ bool cut(const AttnTotals& t) const { return first(t) > 0 || end(t) < tiles; }
+    __device__ __forceinline__ int opener(const AttnTotals& t) const { return attn_opener(unit, tiles, Cut::LEAST, t.total, t.runs); }
+    __device__ __forceinline__ int closer(const AttnTotals& t) const { return attn_closer(unit, tiles, Cut::LEAST, t.total, t.runs); }
 };
 
 // Waits that give up: after that nothing is waited for any more, and the kernel runs to its end.  The first one is suspended, the second looks at the

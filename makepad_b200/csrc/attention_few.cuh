@@ -17,7 +17,7 @@ namespace mpq {
 constexpr int FEW_MOST_CTAS = 256, FEW_TILE = 128, FEW_WARPS = 4, FEW_KEYS = FEW_TILE / FEW_WARPS, FEW_THREADS = 32 * (FEW_WARPS + 1);
 // a unit's end (sums joined, pieces stored and counted) takes a CTA about as long as two tiles
 template <int NT>
-using FewCut = AttnCut<8 * NT, FEW_TILE, 2, false>;
+using FewCut = AttnCut<8 * NT, FEW_TILE, 2, 2, false>;
 static_assert(FEW_THREADS >= ATTN_ENTRIES, "an entry per thread");
 
 template <int D, int NT>
@@ -88,7 +88,7 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         int s = 0;
         uint32_t phase = 1;
         for (bool run = u.begin(p, totals, s_shared); run; run = u.next_run(p, totals, s_shared))
-            for (; u.more(); u.step(p, totals)) {
+            for (; u.more(totals); u.step(p, totals)) {
                 // (a tile's pages are looked up while the one before waits for its room)
                 const int32_t* row = p.table + u.request * p.width;
                 const int end = u.end(totals);
@@ -98,8 +98,8 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                     const int page = row[key >> p.page_shift];
                     return page < 0 || page >= p.pages ? (int)p.pages : page;                    // (beyond the cache: zeros)
                 };
-                int page = page_of(u.first());
-                for (int t = u.first(); t < end; ++t) {
+                int page = page_of(u.first(totals));
+                for (int t = u.first(totals); t < end; ++t) {
                     const int next = page_of(t + 1);
                     attn_wait(empty(s), phase, &s_abort, p.status, 41);
                     __syncwarp();
@@ -125,7 +125,7 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         int s = 0;
         uint32_t phase = 0;
         for (bool run = u.begin(p, totals, s_shared); run; run = u.next_run(p, totals, s_shared))
-        for (; u.more(); u.step(p, totals)) {
+        for (; u.more(totals); u.step(p, totals)) {
             const int rows = attn_block_rows(u.r, p.group.d, u.block, ROWS);
             const int row0 = u.block * ROWS;
             // keys that the rows see: this lane's, and every row of the block
@@ -157,7 +157,7 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                 l[n][0] = l[n][1] = 0.f;
             }
             const int end = u.end(totals);
-            for (int t = u.first(); t < end; ++t) {
+            for (int t = u.first(totals); t < end; ++t) {
                 attn_wait(full(s, warp), phase, &s_abort, p.status, 42);
                 const uint32_t kb = smem0 + s * S::STAGE_BYTES + warp * 2 * S::WARP_BYTES, vb = kb + S::WARP_BYTES;
                 const int key0 = t * FEW_TILE + warp * FEW_KEYS;

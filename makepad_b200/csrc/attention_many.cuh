@@ -25,7 +25,7 @@ namespace mpq {
 
 constexpr int MANY_ROWS = 256, MANY_TILE = 128, MANY_THREADS = 640;
 constexpr int MANY_REGS_WORK = 104, MANY_REGS_REST = 64;         // 4 x 104 + 64 = 5 x 96, what a thread is launched with
-using ManyCut = AttnCut<MANY_ROWS, MANY_TILE, 1, true>;
+using ManyCut = AttnCut<MANY_ROWS, MANY_TILE, 2, 3, true>;
 constexpr int MANY_POWERS = 4;                                    // every so many pairs of weights by a polynomial: see power2
 constexpr float MANY_LATE = 8.f;                                  // log2 of how far a row's maximum runs ahead of the one in use
 
@@ -347,13 +347,13 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             int at = 0;
             bool there = w.begin(p, totals, sh.totals);
             do {
-                while (there && !w.more()) there = w.next_run(p, totals, sh.totals);
+                while (there && !w.more(totals)) there = w.next_run(p, totals, sh.totals);
                 attn_wait(unit_empty + 8 * at, phase, &sh.abort, p.status, 63);
                 if (lane == 0) {
                     ManyUnit n = {};
                     n.there = there;
                     if (there) {
-                        n.first = w.first(); n.end = w.end(totals);
+                        n.first = w.first(totals); n.end = w.end(totals);
                         n.keys = w.r.keys; n.new_rows = w.r.rows; n.first_row = w.r.first;
                         n.row0 = w.block * MANY_ROWS; n.rows = attn_block_rows(w.r, p.group.d, w.block, MANY_ROWS);
                         n.head = w.head; n.request = w.request;

@@ -5,7 +5,8 @@
 // its last row sees (one, empty, where it sees none: its rows of zeros are written all the same).  The tiles of all units in order
 // (request, head, block) are cut into equal runs, one per CTA (or a few: attn_parts), wherever that falls: no shape leaves SMs idle.  What a unit
 // costs beside its tiles (its queries, its end) counts as `extra` tiles behind them that nobody works on.  A unit that a cut falls into has a piece in each
-// run from the one with its first tile to the one with its last.  A run opens at most one such unit (its last) and continues at most one (its first).
+// run from the one with its first tile to the one with its last.  A run opens at most one such unit (its last) and continues at most one (its first).  A piece costs the time of some tiles
+// (its sums are stored and counted, and read again): a cut closer than that to a unit's end moves there.
 #pragma once
 #include <stdint.h>
 
@@ -83,6 +84,19 @@ MPQ_BOTH int attn_owner(int t, int total, int runs)
     if (total < (1 << 20)) return (int)(((uint32_t)(t + 1) * (uint32_t)runs - 1) / (uint32_t)total);
     return (int)((((uint64_t)t + 1) * runs - 1) / (uint32_t)total);
 }
+// Tiles that a piece has at least, of a unit of `tiles` (more than half of them: then there is no piece).
+MPQ_BOTH int attn_least(int tiles, int least) { return least < tiles / 2 + 1 ? least : tiles / 2 + 1; }
+// Of the run [lo, hi): whether the unit whose first tile is `unit` begins behind it; the unit's first tile in it (it is the run's first unit, or 0); its end there.
+MPQ_BOTH bool attn_behind(int hi, int unit, int tiles, int least) { return hi - unit < attn_least(tiles, least); }
+MPQ_BOTH int attn_first(int lo, int unit, int tiles, int least)
+{
+    const int d = lo - unit, n = attn_least(tiles, least);
+    return d < n ? 0 : d > tiles - n ? tiles : d;              // (tiles: all of it is another run's)
+}
+MPQ_BOTH int attn_end(int hi, int unit, int tiles, int least) { return hi - unit > tiles - attn_least(tiles, least) ? tiles : hi - unit; }
+// runs with the unit's first and last piece
+MPQ_BOTH int attn_opener(int unit, int tiles, int least, int total, int runs) { return attn_owner(unit + attn_least(tiles, least) - 1, total, runs); }
+MPQ_BOTH int attn_closer(int unit, int tiles, int least, int total, int runs) { return attn_owner(unit + tiles - attn_least(tiles, least), total, runs); }
 constexpr int ATTN_MOST_RUNS = 2048;
 constexpr int64_t ATTN_MOST_TILES = 1ll << 30;         // of a call: what has more (hours of work) is not begun, and says so in the status word
 

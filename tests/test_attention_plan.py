@@ -29,6 +29,41 @@ int main()
         }
     }
     if (attn_owner((1 << 30) - 1, 1 << 30, ATTN_MOST_RUNS) != ATTN_MOST_RUNS - 1) ++bad;
+    // units of unlike lengths in a row, cut into runs: every tile belongs to one run, pieces are counted by exactly the runs from opener to closer, and
+    // none is shorter than it has to be
+    for (int trial = 0; trial < 3000; ++trial) {
+        const int units = pick(1, 60), extra = pick(0, 3), least = pick(1, 4), longest = trial % 3 ? 12 : 90;
+        std::vector<int> at, tiles;
+        int total = 0;
+        for (int i = 0; i < units; ++i) { at.push_back(total); tiles.push_back(pick(1, longest)); total += tiles[i] + extra; }
+        const int want = pick(1, 200), runs = want < total ? want : total;
+        std::vector<std::vector<int>> had(units), by(units);
+        for (int i = 0; i < units; ++i) had[i].assign(tiles[i], 0);
+        for (int v = 0; v < runs; ++v) {
+            const int lo = attn_run(v, total, runs), hi = attn_run(v + 1, total, runs);
+            int i = 0;
+            while (i + 1 < units && at[i + 1] <= lo) ++i;
+            if (attn_first(lo, at[i], tiles[i], least) == tiles[i]) ++i;
+            for (; i < units && at[i] < hi && !attn_behind(hi, at[i], tiles[i], least); ++i) {
+                const int first = lo <= at[i] ? 0 : attn_first(lo, at[i], tiles[i], least), end = attn_end(hi, at[i], tiles[i], least);
+                if (first >= end || end > tiles[i]) { ++bad; continue; }
+                for (int t = first; t < end; ++t) ++had[i][t];
+                if (first > 0 || end < tiles[i]) {
+                    if (end - first < (least < tiles[i] / 2 + 1 ? 1 : 0)) ++bad;
+                    if (first == 0 && attn_opener(at[i], tiles[i], least, total, runs) != v) ++bad;
+                    if (end == tiles[i] && attn_closer(at[i], tiles[i], least, total, runs) != v) ++bad;
+                    by[i].push_back(v);
+                }
+            }
+        }
+        for (int i = 0; i < units; ++i) {
+            for (int n : had[i]) bad += n != 1;
+            if (by[i].empty()) continue;
+            const int o = attn_opener(at[i], tiles[i], least, total, runs), c = attn_closer(at[i], tiles[i], least, total, runs);
+            if ((int)by[i].size() != c - o + 1 || by[i].front() != o || by[i].back() != c) ++bad;
+            if (o >= runs || c >= runs) ++bad;
+        }
+    }
     // parts: one for little work or few keys, never runs of fewer tiles than ATTN_LEAST_RUN unless there is one part
     for (int trial = 0; trial < 2000; ++trial) {
         const int total = pick(1, 1 << 20);
