@@ -15,7 +15,7 @@
 // ROLES, 20 warps: 0..15 softmax and epilogue (tile, half, quarter of the rows).  16 and 17 issue the MMAs, a tile each: one warp for both had its
 // own bookkeeping between the tiles' products.  18 fetches keys and values (TMA, by pages or by rows), 19 walks the units and says to the others what
 // each is, ahead of them.  A tile's rows of Q (any number of heads shares a head of keys, so they are no box) are copied by its softmax teams behind
-// their last weights, while the last product runs.  Tensor memory: S0, S1, O0, O1 of 128 columns each, all of it.
+// their last weights, while the last product runs (as boxes, where they are some, they came no sooner).  Tensor memory: S0, S1, O0, O1 of 128 columns each, all of it.
 #pragma once
 #include <type_traits>
 
@@ -404,15 +404,15 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             for (int i = 0; i < 32; ++i)
                 if (i >= from) x[i] = 0xFF800000u;
         };
-        // The next unit's rows of Q, 16 bytes at a time into the swizzled tile: chunk c of every sixteenth (or thirty-second) row; token and head of
-        // the row go on with it.  (The tile is free: this thread has seen the last S that was made of it.)
+        // The next unit's rows of Q into the swizzled tile, 16 bytes at a time: chunk c of every sixteenth (or thirty-second) row; token and head of the
+        // row go on with it.  The tile is free: this thread has seen the last S that was made of it.  True where q_there has to follow.
         auto fetch_q = [&] {
-            constexpr int CH = D / 8, STEP = 256 / CH;
             attn_spin(unit_full + 8 * unit_at, unit_phase, &sh.abort, p.status, 64);
             const ManyUnit& n = sh.units[unit_at];
-            const int rows = n.rows - 128 * t;
             if (!n.there || n.first >= n.ends[t]) return false;
-            const int c = threadIdx.x % CH, r0 = (threadIdx.x & 255) / CH, group = p.group.d;
+            const int rows = n.rows - 128 * t, group = p.group.d;
+            constexpr int CH = D / 8, STEP = 256 / CH;
+            const int c = threadIdx.x % CH, r0 = (threadIdx.x & 255) / CH;
             const int tok_step = p.group.of(STEP), head_step = STEP - tok_step * group;
             int tok = p.group.of(n.row0 + 128 * t + r0), head = n.row0 + 128 * t + r0 - tok * group;
             const __nv_bfloat16* base = p.q + (int64_t)n.first_row * p.q_stride + (int64_t)n.head * group * D + c * 8;
@@ -550,6 +550,45 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             }
             // ---- the unit's end: O, unscaled, and the sums of both halves
             const bool some = first < end, fetched = fetch_q();
+            // Rows leave through shared memory, 64 bytes of each of the warp's rows at a time (16-byte chunks, their order turned so that neither side meets a bank
+            // twice): four lanes store 64 bytes of a row.  Where they go is found while the last product runs.
+            const int size = p.out_f32 ? 4 : 2;
+            char* to_row[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int q = quarter * 32 + 8 * i + (lane >> 2), to = u.row0 + 128 * t + min(q, rows - 1), token = p.group.of(to);
+                const int64_t place = (int64_t)(u.first_row + token) * p.q_heads + (u.head - token) * (int)p.group.d + to;
+                to_row[i] = q < rows ? static_cast<char*>(p.out) + (place * D + half * (D / 2)) * size + (lane & 3) * 16 : nullptr;
+            }
+            auto send = [&](int c, const uint32_t (&w)[16]) {                  // from column c of this thread's half on
+                const uint32_t mine = s2u(room) + lane * 64, theirs = s2u(room) + (lane >> 2) * 64;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + ((i ^ ((lane >> 1) & 3)) << 4)), "r"(w[4 * i]), "r"(w[4 * i + 1]), "r"(w[4 * i + 2]), "r"(w[4 * i + 3]) : "memory");
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint4 v;
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(theirs + i * 512 + (((lane & 3) ^ ((lane >> 3) & 3)) << 4)) : "memory");
+                    if (to_row[i]) *reinterpret_cast<uint4*>(to_row[i] + c * size) = v;
+                }
+                __syncwarp();
+            };
+            auto send32 = [&](int c, const uint32_t (&o)[32], float f) {       // 32 columns, times f
+                uint32_t w[16];
+                if (p.out_f32) {
+#pragma unroll
+                    for (int h = 0; h < 32; h += 16) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(__uint_as_float(o[h + i]) * f);
+                        send(c + h, w);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) w[i] = pack_bf16(__uint_as_float(o[2 * i]) * f, __uint_as_float(o[2 * i + 1]) * f);
+                    send(c, w);
+                }
+            };
             if (some) {
                 attn_spin(o_full + 8 * t, o_phase, &sh.abort, p.status, 60);
                 o_phase ^= 1u;
@@ -561,58 +600,21 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             team_sync<64>(pair);                                               // (rows go there now)
             const bool cut = u.cut;
             const int opener = u.opener, closer = u.closer;
-            // 64 bytes of each of the warp's rows from column c of this thread's half on: through shared memory (16-byte chunks, their order turned so that neither
-            // side meets a bank twice), so that four lanes store 64 bytes of a row
-            const int64_t out0 = ((int64_t)u.first_row * p.q_heads + u.head * (int)p.group.d) * D + half * (D / 2);
-            auto send = [&](int c, const uint32_t (&w)[16]) {
-                const uint32_t mine = s2u(room) + lane * 64;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + ((i ^ ((lane >> 1) & 3)) << 4)), "r"(w[4 * i]), "r"(w[4 * i + 1]), "r"(w[4 * i + 2]), "r"(w[4 * i + 3]) : "memory");
-                __syncwarp();
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int q = 8 * i + (lane >> 2), to = u.row0 + 128 * t + quarter * 32 + q;
-                    uint4 v;
-                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(s2u(room) + q * 64 + (((lane & 3) ^ ((q >> 1) & 3)) << 4)) : "memory");
-                    if (quarter * 32 + q < rows) {
-                        const int token = p.group.of(to);
-                        const int64_t place = out0 + (int64_t)token * (p.q_heads - (int)p.group.d) * D + (int64_t)to * D + c;
-                        *reinterpret_cast<uint4*>(static_cast<char*>(p.out) + place * (p.out_f32 ? 4 : 2) + (lane & 3) * 16) = v;
-                    }
-                }
-                __syncwarp();
-            };
-            auto send16 = [&](int c, const float (&v)[16], uint32_t (&held)[16]) {      // sixteen columns, and (bf16) the sixteen before
-                if (p.out_f32) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) held[i] = __float_as_uint(v[i]);
-                    send(c, held);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) held[i + (c & 16 ? 8 : 0)] = pack_bf16(v[2 * i], v[2 * i + 1]);
-                    if (c & 16) send(c - 16, held);
-                }
-            };
             // a piece: [column / 4][row][4], so that a warp's threads lie beside each other; then maxima, sums
             const int mine = 128 * t + row, col4 = half * (D / 8);
             auto slot = [&](int r) { return p.partial + (int64_t)(2 * r + (r == opener ? 1 : 0)) * S::PIECE; };
-            uint32_t held[16];
             if (some) {
-                const float scale = cut ? 1.f : l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-                for (int c = 0; c < D / 2; c += 16) {
-                    uint32_t o[16];
-                    tc_ld16(to + c, o);
+                const float scale = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+                for (int c = 0; c < D / 2; c += 32) {
+                    uint32_t o[32];
+                    tc_ld32(to + c, o);
                     tc_ld_wait_for(o);
-                    float v[16];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(o[i]) * scale;
-                    if (!cut) send16(c, v, held);
+                    if (!cut) send32(c, o, scale);
                     else {
-                        float4* to4 = reinterpret_cast<float4*>(slot(u.run)) + (col4 + (c >> 2)) * MANY_ROWS + mine;
+                        uint4* to4 = reinterpret_cast<uint4*>(slot(u.run)) + (col4 + (c >> 2)) * MANY_ROWS + mine;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) to4[i * MANY_ROWS] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                        for (int i = 0; i < 8; ++i) to4[i * MANY_ROWS] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                     }
                 }
                 tc_fence_before();
@@ -636,9 +638,9 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     float sum = 0.f;
 #pragma unroll 1
                     for (int c = 0; c < D / 2; c += 32) {
-                        float v[2][16], top = -INFINITY;
+                        float v[32], top = -INFINITY;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i >> 4][i & 15] = 0.f;
+                        for (int i = 0; i < 32; ++i) v[i] = 0.f;
                         sum = 0.f;
                         for (int r = opener; r <= closer; ++r) {
                             const float* head = slot(r) + MANY_ROWS * D + mine;
@@ -653,15 +655,14 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                             sum = fmaf(sum, f, ll * g);
 #pragma unroll
                             for (int i = 0; i < 8; ++i) {
-                                float* w = &v[i >> 2][4 * (i & 3)];
+                                float* w = &v[4 * i];
                                 w[0] = fmaf(a[i].x, g, w[0] * f); w[1] = fmaf(a[i].y, g, w[1] * f); w[2] = fmaf(a[i].z, g, w[2] * f); w[3] = fmaf(a[i].w, g, w[3] * f);
                             }
                         }
-                        const float scale = sum == 0.f ? 0.f : 1.f / sum;
+                        uint32_t o[32];
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i >> 4][i & 15] *= scale;
-                        send16(c, v[0], held);
-                        send16(c + 16, v[1], held);
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(v[i]);
+                        send32(c, o, sum == 0.f ? 0.f : 1.f / sum);
                     }
                 }
                 team_sync<256>(9 + t);                                         // (sh.last is the next unit's then)
