@@ -25,7 +25,7 @@ namespace mpq {
 
 constexpr int MANY_ROWS = 256, MANY_TILE = 128, MANY_THREADS = 640;
 constexpr int MANY_REGS_WORK = 104, MANY_REGS_REST = 64;         // 4 x 104 + 64 = 5 x 96, what a thread is launched with
-using ManyCut = AttnCut<MANY_ROWS, MANY_TILE, 2, 3, true>;
+using ManyCut = AttnCut<MANY_ROWS, MANY_TILE, 1, 4, true>;
 constexpr int MANY_POWERS = 4;                                    // every so many pairs of weights by a polynomial: see power2
 constexpr float MANY_LATE = 8.f;                                  // log2 of how far a row's maximum runs ahead of the one in use
 
@@ -459,21 +459,24 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     hide(x[0], left);
                     hide(x[1], left - 32);
                 }
-                float y[4];
+                // this thread's maximum
+                auto top_of = [&] {
+                    float y[4];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const uint32_t* z = &x[c >> 1][16 * (c & 1)];
-                    y[c] = max_nan(__uint_as_float(z[0]), __uint_as_float(z[1]), __uint_as_float(z[2]));
+                    for (int c = 0; c < 4; ++c) {
+                        const uint32_t* z = &x[c >> 1][16 * (c & 1)];
+                        y[c] = max_nan(__uint_as_float(z[0]), __uint_as_float(z[1]), __uint_as_float(z[2]));
 #pragma unroll
-                    for (int i = 3; i < 15; i += 2) y[c] = max_nan(y[c], __uint_as_float(z[i]), __uint_as_float(z[i + 1]));
-                }
-                float top = max_nan(max_nan(y[0], y[1], __uint_as_float(x[0][15])), max_nan(y[2], y[3], __uint_as_float(x[0][31])), max_nan(__uint_as_float(x[1][15]), __uint_as_float(x[1][31]), -INFINITY));
-                // (the other team's reading of the last one is behind its arrival at p_full, which this S waited for)
-                // (the other team's reading of the last one is behind its arrival at p_full, which this S waited for)
-                say(top);
-                // The weights against the maximum in use, beside the exchange of this tile's: only then is it looked at whether they stand (the first
-                // tile of a unit has none to begin with).
+                        for (int i = 3; i < 15; i += 2) y[c] = max_nan(y[c], __uint_as_float(z[i]), __uint_as_float(z[i + 1]));
+                    }
+                    return max_nan(max_nan(y[0], y[1], __uint_as_float(x[0][15])), max_nan(y[2], y[3], __uint_as_float(x[0][31])), max_nan(__uint_as_float(x[1][15]), __uint_as_float(x[1][31]), -INFINITY));
+                };
+                // The weights stand against the maximum in use; this tile's is found and exchanged beside them, and only then is it looked at whether they are
+                // right (the first tile of a unit has none to begin with).  (The other team's reading of the last one is behind its arrival at p_full, which this
+                // S waited for.)
                 if (j == first) {
+                    const float top = top_of();
+                    say(top);
                     m = max_nan(top, hear(), -INFINITY);
                     if (m == INFINITY) m = NAN;                                // (what inf - inf would make of the row)
                 }
@@ -511,9 +514,14 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     uint32_t w[16];
                     sum[0] = sum[1] = 0.f;
                     weights(x[0], w, 0, with_powers);
-                    if (j > first) top = max_nan(top, hear(), -INFINITY);
+                    float top = 0.f;
+                    if (j > first) {
+                        top = top_of();
+                        say(top);
+                    }
                     weights(x[0], w, 1, with_powers);
                     if (j > first) {
+                        top = max_nan(top, hear(), -INFINITY);
                         if (top == INFINITY) top = NAN;
                         if (__any_sync(~0u, !((top - m) * p.scale_log2 <= MANY_LATE))) {
                             // the maximum moves (this S came behind the last product into O), and the weights are made once more: the scores are still there
