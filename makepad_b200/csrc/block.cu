@@ -66,10 +66,9 @@ constexpr int64_t MOST = 0x7FFFFFFF;
 template <class X, class Y>
 static cudaError_t norm_launch(const mpq_context* ctx, const NormParams& p, int64_t M, cudaStream_t s)
 {
-    // One group of eight columns per thread while there are fewer rows than SMs (latency), up to four beyond (fewer barriers per byte).
-    const int groups = p.H / 8;
-    int nv = 1;
-    while (nv < 4 && ((M > ctx->prop.multiProcessorCount && groups > 128 * nv) || groups > 1024 * nv)) nv *= 2;
+    // One group of eight columns per thread where that makes a CTA.  (Several per thread, for fewer barriers per byte, are slower: 8192 rows of 8192 columns,
+    // bf16, with both norms and a gate, 1 / 2 / 4 / 8 groups 160 / 162 / 171 / 208 us; 2000 rows without the first norm 43 / 46 / 50 / 63.)
+    const int groups = p.H / 8, nv = groups <= 1024 ? 1 : groups <= 2048 ? 2 : 4;
     const unsigned threads = (unsigned)((groups + nv - 1) / nv + 31) / 32 * 32;
     auto kernel = nv == 1 ? residual_norm_kernel<1, X, Y> : nv == 2 ? residual_norm_kernel<2, X, Y> : residual_norm_kernel<4, X, Y>;
     return launch_beside(ctx, kernel, dim3((unsigned)M), threads, 0, 1, s, p);

@@ -5,7 +5,7 @@
 //   r' = r + alpha * gate * t                           gate: one value per column, or per element
 //   y  = r' / sqrt(mean(r'^2) + eps) * weight           what the next block reads
 //
-// A CTA has a row, a thread NV groups of eight columns, which stay in registers from the load to the last store: x and r are
+// A CTA has a row, a thread NV groups of eight columns (one, up to 8192 columns), which stay in registers from the load to the last store: x and r are
 // read once, r' and y written once.  Sums of squares are fp32, in a fixed order.  Bound: HBM, (x + 4 + 4 + y) bytes per element;
 // the weights and a gate of one row are read by every CTA and come from L1 / L2.
 #pragma once
