@@ -76,8 +76,7 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    asm volatile("griddepcontrol.launch_dependents;");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    start_beside();
     const AttnTotals totals = attn_totals<FewCut<NT>>(p, s_shared);          // (its barriers publish the mbarriers)
     AttnWalk<FewCut<NT>> u;
 
@@ -329,9 +328,9 @@ attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                                 pm[k] = -INFINITY;
                                 if (r0 + k <= closer) {
                                     const float* from = slot(r0 + k);
-                                    pm[k] = __ldcg(from + ROWS * D + r);
-                                    pl[k] = __ldcg(from + ROWS * D + ROWS + r);
-                                    a[k] = __ldcg(reinterpret_cast<const float4*>(from + r * D + c));
+                                    pm[k] = load_l2(from + ROWS * D + r);
+                                    pl[k] = load_l2(from + ROWS * D + ROWS + r);
+                                    a[k] = load_l2(reinterpret_cast<const float4*>(from + r * D + c));
                                 }
                             }
 #pragma unroll

@@ -194,8 +194,7 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = (uint32_t)uniform((int)sh.tmem);
-    asm volatile("griddepcontrol.launch_dependents;");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    start_beside();
     const AttnTotals totals = attn_totals<ManyCut>(p, sh.totals);
     // the units, for the warps that are told of them: the next one, or false behind the last
     int unit_at = 0;
@@ -654,9 +653,9 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                             const float* head = slot(r) + MANY_ROWS * D + mine;
                             const float4* from = reinterpret_cast<const float4*>(slot(r)) + (col4 + (c >> 2)) * MANY_ROWS + mine;
                             float4 a[8];
-                            const float mm = __ldcg(head), ll = __ldcg(head + MANY_ROWS);
+                            const float mm = load_l2(head), ll = load_l2(head + MANY_ROWS);
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) a[i] = __ldcg(from + i * MANY_ROWS);
+                            for (int i = 0; i < 8; ++i) a[i] = load_l2(from + i * MANY_ROWS);
                             if (mm == -INFINITY) continue;                     // (nothing of this piece is seen: its o need not be there)
                             const float both = max_nan(top, mm, mm), f = top == -INFINITY ? 0.f : ex2(top - both), g = ex2(mm - both);
                             top = both;

@@ -77,8 +77,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_plan_kernel(const __grid_cons
     __shared__ PlanSums s_warp[33];
     __shared__ int s_long;
     int *s_given = s_req, *s_need = s_req + p.n, *s_start = s_req + 2 * p.n, *s_kept = s_req + 3 * p.n, *s_before = s_req + 4 * p.n;
-    asm volatile("griddepcontrol.launch_dependents;");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    start_beside();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = blockIdx.x, ranks = gridDim.x;
     if (tid == 0) s_long = 0;
@@ -204,8 +203,7 @@ template <class X, bool INTERLEAVED>
 __global__ void __launch_bounds__(APPEND_THREADS) kv_append_kernel(const __grid_constant__ AppendParams p)
 {
     __shared__ float s_cos[APPEND_MOST_D / 2], s_sin[APPEND_MOST_D / 2];
-    asm volatile("griddepcontrol.launch_dependents;");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    start_beside();
     const int64_t t = blockIdx.x;
     const int64_t slot = p.slots ? p.slots[t] : 0;
     if (slot < 0) return;                                       // a row behind the last token of the step

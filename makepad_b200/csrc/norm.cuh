@@ -13,6 +13,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "pdl.cuh"
+
 namespace mpq {
 
 struct NormParams {
@@ -87,8 +89,7 @@ template <int NV, class X, class Y>
 __global__ void __launch_bounds__(1024) residual_norm_kernel(const __grid_constant__ NormParams p)
 {
     __shared__ float s_sums[2][32];
-    asm volatile("griddepcontrol.launch_dependents;");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    start_beside();
     const int64_t row = blockIdx.x, base = row * p.H;
     const int step = blockDim.x * 8, c0 = threadIdx.x * 8;
     const X* x = static_cast<const X*>(p.x) + base;

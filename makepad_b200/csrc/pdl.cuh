@@ -8,6 +8,27 @@
 
 namespace mpq {
 
+// A kernel's first steps: the one behind it may start, then everything that the ones in front of it have written is there.
+__device__ __forceinline__ void start_beside()
+{
+    asm volatile("griddepcontrol.launch_dependents;");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// from L2: what other CTAs of the same kernel have stored
+__device__ __forceinline__ float load_l2(const float* p)
+{
+    float v;
+    asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 load_l2(const float4* p)
+{
+    float4 v;
+    asm volatile("ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+    return v;
+}
+
 // evict-first: read once
 __device__ __forceinline__ float load_once(const float* p)
 {

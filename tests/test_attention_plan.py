@@ -120,3 +120,16 @@ def test_the_cut_of_the_work():
         subprocess.check_call(["g++", "-std=c++17", "-O1", "-Wall", "-I", os.path.join(ROOT, "makepad_b200", "csrc"), src, "-o", exe])
         out = subprocess.run([exe], capture_output=True, text=True)
         assert out.returncode == 0 and out.stdout.strip() == "0", out.stdout + out.stderr
+
+
+def test_the_new_kernels_read_what_is_in_front_of_them_by_ordinary_loads():
+    """Behind start_beside() there is no load through the read-only path, and no pointer that would let the compiler choose it."""
+    csrc = os.path.join(ROOT, "makepad_b200", "csrc")
+    kernels = 0
+    for f in ("norm.cuh", "kv_cache.cuh", "attention.cuh", "attention_few.cuh", "attention_many.cuh"):
+        text = open(os.path.join(csrc, f)).read()
+        assert "__ldg" not in text and "__restrict__" not in text and "__ldc" not in text, f
+        for kernel in text.split("__global__ ")[1:]:
+            kernels += 1
+            assert "start_beside();" in kernel[:kernel.index("\n}")], (f, kernel[:100])
+    assert kernels == 5
