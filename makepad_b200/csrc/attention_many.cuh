@@ -38,7 +38,7 @@ struct ManyUnit {
     int cut, opener, closer, run;            // whether other runs have tiles of the unit, and which; this one
 };
 struct ManyShared {
-    uint64_t q_full[2], s_full[2], p_half[2], p_full[2], o_full[2], o_empty[2], kv_full[8], kv_empty[8], unit_full[MANY_UNITS], unit_empty[MANY_UNITS], told[16], turn[2];
+    uint64_t q_full[2], s_full[2], p_half[2], p_full[2], o_full[2], o_empty[2], kv_full[8], kv_empty[8], unit_full[MANY_UNITS], unit_empty[MANY_UNITS], told[16], turn[2], pair[8], team[2];
     ManyUnit units[MANY_UNITS];
     AttnShared totals;
     uint32_t tmem;
@@ -144,9 +144,6 @@ __device__ __forceinline__ void tc_ld_wait_for(uint32_t (&r)[N])
 #pragma unroll
     for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
 }
-template <int N>
-__device__ __forceinline__ void team_sync(int barrier) { asm volatile("bar.sync %0, %1;" ::"r"(barrier), "n"(N) : "memory"); }
-
 // PAGED: boxes of a page's keys; else boxes of 128 rows beside the queries
 template <int D, bool PAGED>
 __global__ void __launch_bounds__(MANY_THREADS, 1)
@@ -180,6 +177,8 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             bar_init(kv_empty + 8 * s, 2);
         }
         for (int i = 0; i < 16; ++i) bar_init(s2u(&sh.told[i]), 1);
+        for (int i = 0; i < 8; ++i) bar_init(s2u(&sh.pair[i]), 2);
+        for (int i = 0; i < 2; ++i) bar_init(s2u(&sh.team[i]), 8);
         for (int i = 0; i < MANY_UNITS; ++i) {
             bar_init(unit_full + 8 * i, 1);
             bar_init(unit_empty + 8 * i, 19);
@@ -379,24 +378,28 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         const int t = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3, row = quarter * 32 + lane;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         const uint32_t ts = tmem + lanes + 128 * t, to = tmem + lanes + 256 + 128 * t + half * (D / 2);
-        const int pair = 1 + 4 * t + quarter;                                  // barrier of the two warps with these rows
-        uint32_t s_phase = 0, o_phase = 0;
+        uint32_t phases = 0;                                                   // of s_full, o_full, told, team and pair: a bit each (every register counts here)
         // This warp's 2 KB, and those of the warp with the other half: a row's maximum or sum there (a float per lane) while a unit is worked on, at its
         // end rows on their way out.
         unsigned char* room = smem_many + (2 + S::STAGES) * S::TILE_BYTES + warp * 2048;
         float *tell = reinterpret_cast<float*>(room) + lane, *told = reinterpret_cast<float*>(room + (half ? -4 : 4) * 2048) + lane;
-        const uint32_t tell_bar = s2u(&sh.told[warp]), told_bar = s2u(&sh.told[warp ^ 4]);
-        uint32_t told_phase = 0;
         // the larger of this thread's and the other half's
         auto say = [&](float v) {
             *tell = v;
             __syncwarp();
-            if (lane == 0) bar_arrive(tell_bar);
+            if (lane == 0) bar_arrive(s2u(&sh.told[warp]));
         };
         auto hear = [&] {
-            attn_spin(told_bar, told_phase, &sh.abort, p.status, 65);
-            told_phase ^= 1u;
+            attn_spin(s2u(&sh.told[warp ^ 4]), phases >> 2 & 1u, &sh.abort, p.status, 65);
+            phases ^= 4u;
             return *told;
+        };
+        // Warps meet (the two with these rows; the tile's eight) at barriers that give up, and not at bar.sync: a warp that has given up goes to its end.
+        auto meet = [&](uint64_t* bar, uint32_t bit, int code) {
+            __syncwarp();
+            if (lane == 0) bar_arrive(s2u(bar));
+            attn_spin(s2u(bar), phases >> bit & 1u, &sh.abort, p.status, code);
+            phases ^= 1u << bit;
         };
         auto hide = [](uint32_t (&x)[32], int from) {                          // scores of keys that the row does not see
 #pragma unroll
@@ -407,6 +410,7 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         // row go on with it.  The tile is free: this thread has seen the last S that was made of it.  True where q_there has to follow.
         auto fetch_q = [&] {
             attn_spin(unit_full + 8 * unit_at, unit_phase, &sh.abort, p.status, 64);
+            if (sh.abort) return false;
             const ManyUnit& n = sh.units[unit_at];
             if (!n.there || n.first >= n.ends[t]) return false;
             const int rows = n.rows - 128 * t, group = p.group.d;
@@ -445,8 +449,8 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             int left = origin + tok, left_all = origin + p.group.of(u.row0 + 128 * t);
             float m = -INFINITY, l = 0.f;                                      // m in units of the scores as they come; l of this half
             for (int j = first; j < end; ++j, left -= MANY_TILE, left_all -= MANY_TILE) {
-                attn_spin(s_full + 8 * t, s_phase, &sh.abort, p.status, 59);
-                s_phase ^= 1u;
+                attn_spin(s_full + 8 * t, phases & 1u, &sh.abort, p.status, 59);
+                phases ^= 1u;
                 tc_fence_after();
                 uint32_t x[2][32];
 #pragma unroll
@@ -597,14 +601,14 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 }
             };
             if (some) {
-                attn_spin(o_full + 8 * t, o_phase, &sh.abort, p.status, 60);
-                o_phase ^= 1u;
+                attn_spin(o_full + 8 * t, phases >> 1 & 1u, &sh.abort, p.status, 60);
+                phases ^= 2u;
                 tc_fence_after();
             }
             if (fetched) q_there();
             say(l);                                                            // (behind o_full, so behind the other team's last reading, too)
             l += hear();
-            team_sync<64>(pair);                                               // (rows go there now)
+            meet(&sh.pair[4 * t + quarter], 4, 67);                             // (both have read: rows go there now)
             const bool cut = u.cut;
             const int opener = u.opener, closer = u.closer;
             // a piece: [column / 4][row][4], so that a warp's threads lie beside each other; then maxima, sums
@@ -633,13 +637,13 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     head[mine] = m == -INFINITY ? m : m * p.scale_log2;
                     head[MANY_ROWS + mine] = l;
                 }
-                team_sync<256>(9 + t);
+                meet(&sh.team[t], 3, 68);
                 if ((threadIdx.x & 255) == 0) {
                     const uint32_t before = attn_arrive(p.arrived + 2 * opener + t);
                     sh.last[t] = before == (uint32_t)(closer - opener);
                     if (sh.last[t]) p.arrived[2 * opener + t] = 0;
                 }
-                team_sync<256>(9 + t);
+                meet(&sh.team[t], 3, 69);
                 if (sh.last[t]) {
                     // the pieces in order, rescaled when a larger maximum comes; 32 columns at a time
                     float sum = 0.f;
@@ -672,7 +676,7 @@ attention_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                         send32(c, o, sum == 0.f ? 0.f : 1.f / sum);
                     }
                 }
-                team_sync<256>(9 + t);                                         // (sh.last is the next unit's then)
+                meet(&sh.team[t], 3, 70);                                         // (sh.last is the next unit's then)
             }
         }
     }

@@ -57,6 +57,7 @@ int log2_of(int64_t v) { int s = 0; while ((1ll << s) < v) ++s; return s; }
 bool page_ok(int64_t page_size) { return power_of_two(page_size) && page_size >= 16 && page_size <= 256; }
 
 constexpr int64_t MOST = 0x7FFFFFFF;
+constexpr int64_t MOST_KEYS = 1ll << 30;      // of a request, and rows of a call: what is added to one stays an int
 
 }  // namespace
 
@@ -109,7 +110,7 @@ extern "C" int32_t mpq_kv_plan(mpq_context* ctx, int64_t n, const int32_t* new_l
         return fail(ctx, MPQ_ERR_INVALID_ARG, "null pointer");
     if (n <= 0 || max_blocks <= 0 || pages <= 0 || tokens < 0 || tokens > MOST || pages > MOST) return fail(ctx, MPQ_ERR_SHAPE, "n, max_blocks and pages must be positive, tokens not negative, all below 2^31");
     if (!page_ok(page_size)) return fail(ctx, MPQ_ERR_SHAPE, "page_size must be a power of two from 16 to 256 (%d)", page_size);
-    if (max_blocks > MOST / page_size) return fail(ctx, MPQ_ERR_SHAPE, "max_blocks * page_size must be below 2^31");
+    if (max_blocks > MOST_KEYS / page_size) return fail(ctx, MPQ_ERR_SHAPE, "max_blocks * page_size must be at most 2^30");
     if (n > PLAN_MOST_N) return fail(ctx, MPQ_ERR_UNSUPPORTED, "more than %d requests", PLAN_MOST_N);
     const OnDevice on(ctx->device);
     CU_TRY(ctx, on.error);
@@ -174,7 +175,7 @@ struct AttnKeys {
 static int32_t attention_check(mpq_context* ctx, const AttnParams& p, const AttnKeys& kv, int64_t n, int64_t q_heads, int64_t kv_heads, int32_t head_dim, float scale)
 {
     if (!p.q || !kv.k || !kv.v || !p.starts || !p.out) return fail(ctx, MPQ_ERR_INVALID_ARG, "null pointer");
-    if (p.tokens <= 0 || p.tokens > MOST || n <= 0 || n > MOST) return fail(ctx, MPQ_ERR_SHAPE, "tokens and n must be positive and below 2^31");
+    if (p.tokens <= 0 || p.tokens > MOST_KEYS || n <= 0 || n > MOST) return fail(ctx, MPQ_ERR_SHAPE, "tokens and n must be positive, tokens at most 2^30, n below 2^31");
     if (q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || q_heads > 4096)
         return fail(ctx, MPQ_ERR_SHAPE, "q_heads must be a multiple of kv_heads, at most 4096 (%lld and %lld)", (long long)q_heads, (long long)kv_heads);
     if (p.tokens * p.group.d > MOST) return fail(ctx, MPQ_ERR_UNSUPPORTED, "tokens * q_heads / kv_heads must be below 2^31");
@@ -302,7 +303,7 @@ extern "C" int32_t mpq_paged_attention(mpq_context* ctx, const uint16_t* q_dev, 
     if (!lens_dev || !block_table_dev) return fail(ctx, MPQ_ERR_INVALID_ARG, "null pointer");
     if (!page_ok(page_size) || pages <= 0 || pages > MOST) return fail(ctx, MPQ_ERR_SHAPE, "pages must be positive, page_size a power of two from 16 to 256 (%lld pages of %d)", (long long)pages, page_size);
     if (pages >= MOST / kv_heads) return fail(ctx, MPQ_ERR_UNSUPPORTED, "pages * kv_heads must be below 2^31");
-    if (max_blocks <= 0 || max_blocks > MOST / page_size) return fail(ctx, MPQ_ERR_SHAPE, "max_blocks * page_size must be positive and below 2^31");
+    if (max_blocks <= 0 || max_blocks > MOST_KEYS / page_size) return fail(ctx, MPQ_ERR_SHAPE, "max_blocks * page_size must be positive and at most 2^30");
     if (max_new < 0) return fail(ctx, MPQ_ERR_SHAPE, "max_new must not be negative");
     p.lens = lens_dev; p.table = block_table_dev;
     p.width = max_blocks; p.pages = pages; p.page_shift = log2_of(page_size);

@@ -616,3 +616,78 @@ def test_calls_on_another_stream(ctx):
     s.synchronize()
     assert torch.equal(got, want)
     ctx.check(ctx.lib.mpq_context_poll_status(ctx.h))
+
+
+def test_two_contexts_at_once():
+    """Calls of two contexts on two streams, beside each other: each has its own pieces and counters."""
+    torch, m = _t(), _m()
+    contexts = [m.Context(0), m.Context(0)]
+    data, want = [], []
+    for i, c in enumerate(contexts):
+        k, v, table = _paged_case(10 * i, [1, 300], [5000, 4000], 2, 128, 16)
+        q = _randn(20 + i, 301, 8, 128, dtype=torch.bfloat16)
+        rows = [_randn(30 + i + j, 2000, h, 64, dtype=torch.bfloat16) for j, h in enumerate((8, 2, 2))]
+        data.append((q, k, v, _ints([0, 1, 301]), _ints([5000, 4000]), _ints(table), rows, _ints([0, 700, 2000])))
+
+    def run(c, d):
+        return [m.paged_attention(c, d[0], *d[1:6]), m.paged_attention(c, d[0][:1].contiguous(), d[1], d[2], _ints([0, 1]), d[4][:1].contiguous(), d[5][:1].contiguous(), max_new=1),
+                m.prompt_attention(c, *d[6], d[7])]
+    for c, d in zip(contexts, data):
+        want.append(run(c, d))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(10):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(run(contexts[i], data[i]))
+    torch.cuda.synchronize()
+    for i, c in enumerate(contexts):
+        for g in got[i]:
+            for a, b in zip(g, want[i]):
+                assert torch.equal(a, b)
+        c.check(c.lib.mpq_context_poll_status(c.h))
+
+
+@pytest.mark.parametrize("kind", ["few", "many", "prompt"])
+def test_a_first_call_inside_a_capture(kind):
+    """Without room for pieces (none can be had in a capture) units stay whole: other last bits, the same attention."""
+    torch, m = _t(), _m()
+    ctx = m.Context(0)
+    new, lens, D = ([1, 1, 1], [5000, 40, 0], 128) if kind == "few" else ([200, 1, 30], [3000, 700, 30], 128)
+    k, v, table = _paged_case(1, new, lens, 2, D, 16)
+    starts = [0, new[0], new[0] + new[1], sum(new)]
+    q = _randn(2, sum(new), 8, D, dtype=torch.bfloat16)
+    rows = [_randn(3 + j, 1500, h, D, dtype=torch.bfloat16) for j, h in enumerate((8, 2, 2))]
+    args = (_ints(starts), _ints(lens), _ints(table))
+    at = _ints([0, 1000, 1500])
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        out = m.prompt_attention(ctx, *rows, at) if kind == "prompt" else m.paged_attention(ctx, q, k, v, *args, max_new=max(new))
+    graph.replay()
+    graph.replay()
+    torch.cuda.synchronize()
+    if kind == "prompt":
+        for a, b in ((0, 1000), (1000, 1500)):
+            want, mass = _attention_reference(rows[0][a:b], rows[1][a:b], rows[2][a:b], D ** -0.5)
+            assert _off(out[a:b], want, mass, D, D ** -0.5 * 16 ** 2) <= 1
+    else:
+        for i, (a, t) in enumerate(zip(new, lens)):
+            want, mass = _attention_reference(q[starts[i]:starts[i + 1]], _gathered(k, table[i], t, 16), _gathered(v, table[i], t, 16), D ** -0.5)
+            assert _off(out[starts[i]:starts[i + 1]], want, mass, D, D ** -0.5 * 16 ** 2) <= 1, i
+    ctx.check(ctx.lib.mpq_context_poll_status(ctx.h))
+    ctx.close()
+
+
+def test_scale_zero_and_wide_groups(ctx):
+    """Equal weights; more query heads per head of keys than a tile has rows."""
+    torch, m = _t(), _m()
+    _check_paged(ctx, [1, 3, 200], [100, 700, 300], 4, 2, 64, 16, scale=0.0)
+    _check_paged(ctx, [1, 5], [333, 40], 300, 1, 64, 16)
+    _check_paged(ctx, [40], [400], 130, 1, 128, 32)
+    q, k, v = _randn(1, 70, 272, 64, dtype=torch.bfloat16), _randn(2, 70, 1, 64, dtype=torch.bfloat16), _randn(3, 70, 1, 64, dtype=torch.bfloat16)
+    got = m.prompt_attention(ctx, q, k, v, _ints([0, 3, 70]))
+    for a, b in ((0, 3), (3, 70)):
+        want, mass = _attention_reference(q[a:b], k[a:b], v[a:b], 0.125)
+        assert _off(got[a:b], want, mass, 64, 0.125 * 13 ** 2) <= 1
