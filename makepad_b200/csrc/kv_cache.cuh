@@ -197,7 +197,7 @@ struct AppendParams {
     int q_heads, kv_heads, head_dim, rot;
 };
 
-constexpr int APPEND_THREADS = 256, APPEND_MOST_D = 256;
+constexpr int APPEND_THREADS = 128, APPEND_MOST_D = 256;
 
 template <class X, bool INTERLEAVED>
 __global__ void __launch_bounds__(APPEND_THREADS) kv_append_kernel(const __grid_constant__ AppendParams p)
@@ -209,14 +209,14 @@ __global__ void __launch_bounds__(APPEND_THREADS) kv_append_kernel(const __grid_
     if (slot < 0) return;                                       // a row behind the last token of the step
     const X* x = static_cast<const X*>(p.x) + t * p.x_stride;
     const int d = p.head_dim, half = p.rot / 2, per_head = d / 16, heads = p.q_heads + 2 * p.kv_heads, items = heads * per_head;
-    if ((int)threadIdx.x < half) {
-        const double angle = (double)p.positions[t] * p.freq[threadIdx.x];
+    for (int i = threadIdx.x; i < half; i += APPEND_THREADS) {
+        const double angle = (double)p.positions[t] * p.freq[i];
         const double turns = rint(angle * 0.15915494309189533577);
         const float a = (float)fma(turns, -6.283185307179586477, angle);
         float s, c;
         sincosf(a, &s, &c);
-        s_cos[threadIdx.x] = c;
-        s_sin[threadIdx.x] = s;
+        s_cos[i] = c;
+        s_sin[i] = s;
     }
     __syncthreads();
     const bool cached = p.slots && slot < p.slot_end;
