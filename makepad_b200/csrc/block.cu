@@ -121,7 +121,7 @@ extern "C" int32_t mpq_kv_plan(mpq_context* ctx, int64_t n, const int32_t* new_l
         raised.mark(ctx->device);
     }
     const PlanParams p = {new_lens_dev, lens_dev, lens_out_dev, block_table_dev, free_dev, free_count_dev, free_count_out_dev, starts_dev, positions_dev, slots_dev, missing_dev,
-                          (int)n, page_size, (int)pages, (int)max_blocks, tokens};
+                          (int)n, log2_of(page_size), (int)pages, (int)max_blocks, tokens};
     // one CTA while it has about one token and one request per thread
     const unsigned ctas = n <= PLAN_THREADS / 2 && tokens <= PLAN_THREADS ? 1 : PLAN_CLUSTER;
     ctx->launches += 1;

@@ -20,8 +20,9 @@ namespace mpq {
 // that no thread waits for another's store.
 //
 // One cluster, every CTA of which makes the sums for itself (a thread has up to PLAN_PER requests), then takes its share of
-// pages and tokens.  The lengths and the count are read before the cluster's barrier and written behind it: they may be
-// updated in place.  Bound: latency of one launch, two reads and a store.
+// pages and, behind a barrier, of tokens.  The lengths and the count are read before the first barrier and written behind it: they may be
+// updated in place.  Bound: latency.  64 requests of a token each 4.4 us (one CTA; of it 2.3 launch and sums), 1000 requests with 29 000 tokens and
+// 28 000 pages given back 14.0 (a search per token and page, and 64-bit ones: 17.2; clusters of sixteen: 14.1).
 struct PlanParams {
     const int32_t *new_lens, *lens;
     int32_t *lens_out, *table, *free;
@@ -29,7 +30,7 @@ struct PlanParams {
     int32_t *count_out, *starts, *positions;
     int64_t* slots;
     int32_t* missing;
-    int n, page_size, pages, width;
+    int n, page_shift, pages, width;
     int64_t tokens;
 };
 
@@ -48,26 +49,24 @@ struct PlanRequest {
 
 __device__ __forceinline__ PlanRequest plan_request(const PlanParams& p, int i)
 {
-    const int fresh = p.new_lens[i], old = max(0, min(p.lens[i], (int)min((long long)p.width * p.page_size, 0x7FFFFFFFll)));
+    const int fresh = p.new_lens[i], old = max(0, min(p.lens[i], p.width << p.page_shift)), up = (1 << p.page_shift) - 1;
     PlanRequest r;
     r.old = old;
-    r.had = (int)(((long long)old + p.page_size - 1) / p.page_size);
+    r.had = (old + up) >> p.page_shift;
     const bool ended = fresh < 0;
     r.before = ended ? 0 : old;
     r.grow = ended ? 0 : fresh;
     r.kept = ended ? 0 : r.had;
-    r.need = ((long long)r.before + r.grow + p.page_size - 1) / p.page_size - r.kept;
+    r.need = (((long long)r.before + r.grow + up) >> p.page_shift) - r.kept;
     return r;
 }
 
 // last index with at[index] <= v among n ascending numbers, at[0] = 0
-__device__ __forceinline__ int plan_find(const int* at, int n, long long v)
+__device__ __forceinline__ int plan_find(const int* at, int n, int v)
 {
-    int lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if ((long long)at[mid] <= v) lo = mid; else hi = mid;
-    }
+    int lo = 0;
+    for (int step = 1 << (31 - __clz(n)); step; step >>= 1)
+        if (lo + step < n && at[lo + step] <= v) lo += step;
     return lo;
 }
 
@@ -87,7 +86,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_plan_kernel(const __grid_cons
     PlanSums mine = {0, 0, 0};
     for (int i = i0; i < i1; ++i) {
         const PlanRequest r = plan_request(p, i);
-        if ((long long)r.before + r.grow > (long long)p.width * p.page_size) s_long = 1;
+        if ((long long)r.before + r.grow > (long long)p.width << p.page_shift) s_long = 1;
         mine.add(PlanSums{r.before == 0 && p.new_lens[i] < 0 ? r.had : 0, r.need, r.grow});
     }
     PlanSums run = mine;                       // inclusive over the warp, then over the CTA
@@ -145,35 +144,53 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_plan_kernel(const __grid_cons
             *p.missing = missing;
         }
     }
-    const long long first = (long long)rank * PLAN_THREADS + tid, stride = (long long)ranks * PLAN_THREADS;
-    // page of rank q among the wanted ones
-    auto page_of = [&](long long q) {
-        const long long e = held - 1 - q;
-        if (e < count) return p.free[e];
-        const int i = plan_find(s_given, p.n, e - count);
-        return p.table[(int64_t)i * p.width + (e - count - s_given[i])];
-    };
-    for (long long g = first; g < held - count; g += stride) {
-        const int i = plan_find(s_given, p.n, g);
-        p.free[count + g] = p.table[(int64_t)i * p.width + (g - s_given[i])];
-    }
-    for (long long q = first; q < wants; q += stride) {
-        const int i = plan_find(s_need, p.n, q);
-        p.table[(int64_t)i * p.width + s_kept[i] + (q - s_need[i])] = page_of(q);
-    }
-    const long long live = fits ? total.grow : 0;
-    for (long long t = first; t < p.tokens; t += stride) {
-        int pos = 0;
-        long long slot = -1;
-        if (t < live) {
-            const int i = plan_find(s_start, p.n, t);
-            pos = s_before[i] + (int)(t - s_start[i]);
-            const int b = pos / p.page_size;
-            const int page = b < s_kept[i] ? p.table[(int64_t)i * p.width + b] : page_of(s_need[i] + b - s_kept[i]);
-            slot = (long long)page * p.page_size + (pos - b * p.page_size);
+    // Numbers 0 .. end - 1 that requests have in a row from at[i] on: a thread takes one, or, with one search and a walk, four that lie a warp apart (so that a
+    // warp's stores are beside each other); it looks all of them up before it stores any.
+    auto each = [&](int end, const int* at, auto look, auto store) {
+        const int take = end > ranks * PLAN_THREADS ? 4 : 1;
+        for (long long w0 = (long long)(rank * (PLAN_THREADS / 32) + warp) * 32 * take; w0 < end; w0 += ranks * PLAN_THREADS * take) {
+            int who[4], v[4];
+            who[0] = plan_find(at, p.n, (int)min(w0 + lane, (long long)end - 1));
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const long long g = w0 + 32 * k + lane;
+                if (k < take && g < end) {
+                    if (k) who[k] = who[k - 1];
+                    while (who[k] + 1 < p.n && at[who[k] + 1] <= (int)g) ++who[k];
+                    v[k] = look((int)g, who[k], (int)g - at[who[k]]);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const long long g = w0 + 32 * k + lane;
+                if (k < take && g < end) store((int)g, who[k], (int)g - at[who[k]], v[k]);
+            }
         }
-        p.positions[t] = pos;
-        p.slots[t] = slot;
+    };
+    // pages given back
+    each((int)(held - count), s_given, [&](int, int i, int k) { return p.table[(int64_t)i * p.width + k]; }, [&](int g, int, int, int page) { p.free[count + g] = page; });
+    // pages taken: the one of rank q among them
+    each((int)wants, s_need,
+         [&](int q, int, int) {
+             const int e = (int)held - 1 - q, back = e - (int)count;
+             if (back < 0) return p.free[e];
+             const int i = plan_find(s_given, p.n, back);
+             return p.table[(int64_t)i * p.width + (back - s_given[i])];
+         },
+         [&](int, int i, int k, int page) { p.table[(int64_t)i * p.width + s_kept[i] + k] = page; });
+    // the tokens' slots, from the table as it is now
+    asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    const long long live = fits ? total.grow : 0;
+    each((int)live, s_start, [&](int, int i, int k) { return p.table[(int64_t)i * p.width + ((s_before[i] + k) >> p.page_shift)]; },
+         [&](int t, int i, int k, int page) {
+             const int pos = s_before[i] + k;
+             p.positions[t] = pos;
+             p.slots[t] = ((long long)page << p.page_shift) + (pos & ((1 << p.page_shift) - 1));
+         });
+    for (long long t = live + (long long)rank * PLAN_THREADS + tid; t < p.tokens; t += (long long)ranks * PLAN_THREADS) {
+        p.positions[t] = 0;
+        p.slots[t] = -1;
     }
 }
 
@@ -184,7 +201,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_plan_kernel(const __grid_cons
 // bits, reduced there to [-pi, pi] (in 32 bits position 100000 would be off by 0.004), sine and cosine are fp32.  One rounding, to bf16.
 //
 // A CTA has a token: 64 threads make its sines and cosines while all threads' rows are on their way.  An item is 16 elements of a head that
-// turn together: (8 + 8 a half apart, or 16 in a row).  Bound: HBM, (size of x + 2) bytes per element.
+// turn together: (8 + 8 a half apart, or 16 in a row).  Bound: HBM, (size of x + 2) bytes per element: 8000 bf16 rows of 80 heads of 128 55 us, 5.9 TB/s (the
+// sines are a CTA's latency: with 8 warps instead of 4, and half as many tokens on an SM, 61; with 2 56; rows of 36 heads of 64 19.3, 24.1 and 17.7).
 struct AppendParams {
     const void* x;
     int64_t x_stride;
