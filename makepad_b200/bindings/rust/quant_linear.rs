@@ -148,3 +148,49 @@ pub fn nvfp4_quantize(ctx: &Context, x: DevicePtr, x_is_bf16: bool, swiglu: bool
 pub fn swiglu(ctx: &Context, gate_up: DevicePtr, m: i64, f: i64, out: DevicePtr, stream: *mut c_void) -> Result<(), MpqError> {
     ctx.check(unsafe { (ctx.lib.mpq_swiglu)(ctx.raw, gate_up.0 as *const f32, m, f, out.0 as *mut f32, stream) })
 }
+
+/// Rows of a norm around a block: r' = residual + alpha * gate * (x, or its RMS norm times post_weight), y = RMS norm of r' times weight.
+/// Null pointers leave a part out; see mpq_residual_norm.
+pub struct NormRows {
+    pub x: DevicePtr, pub x_is_bf16: bool, pub m: i64, pub h: i64,
+    pub residual: DevicePtr, pub residual_out: DevicePtr, pub post_weight: DevicePtr, pub gate: DevicePtr, pub gate_stride: i64, pub alpha: f32,
+    pub weight: DevicePtr, pub eps: f32, pub y: DevicePtr, pub y_is_bf16: bool,
+}
+
+pub fn residual_norm(ctx: &Context, r: &NormRows, stream: *mut c_void) -> Result<(), MpqError> {
+    ctx.check(unsafe {
+        (ctx.lib.mpq_residual_norm)(ctx.raw, r.x.0, r.x_is_bf16 as i32, r.m, r.h, r.residual.0 as *const f32, r.residual_out.0 as *mut f32, r.post_weight.0 as *const f32,
+                                    r.gate.0 as *const f32, r.gate_stride, r.alpha, r.weight.0 as *const f32, r.eps, r.y.0, r.y_is_bf16 as i32, stream)
+    })
+}
+
+/// A paged cache of bf16 keys and values [pages][kv_heads][page_size][head_dim], and who has its pages (all device memory of the caller's).
+#[derive(Clone, Copy)]
+pub struct PagedCache {
+    pub k: DevicePtr, pub v: DevicePtr, pub pages: i64, pub page_size: i32, pub kv_heads: i32, pub head_dim: i32,
+    pub lens: DevicePtr, pub block_table: DevicePtr, pub max_blocks: i64, pub free: DevicePtr, pub free_count: DevicePtr, pub requests: i64,
+}
+
+/// Where mpq_kv_plan writes a step: starts i32 [requests + 1], positions i32 and slots i64 [tokens], missing i32 [1].
+#[derive(Clone, Copy)]
+pub struct Step { pub tokens: i64, pub starts: DevicePtr, pub positions: DevicePtr, pub slots: DevicePtr, pub missing: DevicePtr }
+
+impl PagedCache {
+    /// new_lens: i32 [requests] on the device, negative for a request that has ended; lengths and the count of free pages are updated in place.
+    pub fn plan(&self, ctx: &Context, new_lens: DevicePtr, step: &Step, stream: *mut c_void) -> Result<(), MpqError> {
+        ctx.check(unsafe {
+            (ctx.lib.mpq_kv_plan)(ctx.raw, self.requests, new_lens.0 as *const i32, self.lens.0 as *const i32, self.lens.0 as *mut i32, self.block_table.0 as *mut i32, self.max_blocks,
+                                  self.free.0 as *mut i32, self.pages, self.free_count.0 as *const i32, self.free_count.0 as *mut i32, self.page_size, step.tokens,
+                                  step.starts.0 as *mut i32, step.positions.0 as *mut i32, step.slots.0 as *mut i64, step.missing.0 as *mut i32, stream)
+        })
+    }
+
+    /// Attention of the step's rows q [tokens][q_heads][head_dim] (bf16), whose keys and values are in the cache; out fp32 or bf16.
+    pub fn attend(&self, ctx: &Context, q: DevicePtr, q_heads: i32, step: &Step, max_new: i64, scale: f32, out: DevicePtr, out_is_f32: bool, stream: *mut c_void) -> Result<(), MpqError> {
+        ctx.check(unsafe {
+            (ctx.lib.mpq_paged_attention)(ctx.raw, q.0 as *const u16, q_heads as i64 * self.head_dim as i64, step.tokens, q_heads, self.k.0 as *const u16, self.v.0 as *const u16, self.pages,
+                                          self.page_size, self.kv_heads, self.head_dim, self.requests, step.starts.0 as *const i32, self.lens.0 as *const i32,
+                                          self.block_table.0 as *const i32, self.max_blocks, max_new, scale, out.0, out_is_f32 as i32, stream)
+        })
+    }
+}

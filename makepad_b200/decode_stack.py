@@ -1,9 +1,9 @@
 """The 7B-shape decode layer stack: 32 layers of Q4 projections driven as one CUDA graph.
 
 Per layer: QKV 4096->12288, O 4096->4096, gate+up 4096->2*11008, down 11008->4096.
-Only the block-quantised linear operators are in scope (attention, norms and the
-activation function between them are not), so the chain is shape-only: every
-projection reads its own activation buffer.  The launches are nevertheless
+Only the block-quantised linear operators run here (whole layers, with norms and
+attention, are decoder.py's), so the chain is shape-only: every projection reads
+its own activation buffer.  The launches are nevertheless
 issued in stream order with programmatic dependent launch, exactly as a real
 decode step would issue them: each kernel prefetches its weights early and
 reads its activation only after the previous kernel has completed.
