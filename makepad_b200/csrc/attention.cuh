@@ -15,6 +15,7 @@
 #include <stdint.h>
 
 #include "attention_plan.h"
+#include "context.h"
 #include "norm.cuh"
 #include "nvfp4_ptx.cuh"
 #include "settle.cuh"
@@ -61,13 +62,15 @@ __device__ __forceinline__ int attn_unit_cost(const AttnParams& p, const AttnReq
 {
     return whole ? 1 : attn_block_tiles(r, p.group, b, Cut::ROWS, Cut::TILE) + Cut::EXTRA;
 }
+// What is too much stays too much: a sum of costs (each below 2^24) that is above 2^31, of lanes' shares above 2^26, goes no further, and any such call is above ATTN_MOST_TILES
+__device__ __forceinline__ uint32_t attn_sum(uint32_t sum, int more, uint32_t most) { return min(sum + (uint32_t)more, most); }
 // tiles of a request in one head, by a warp
 template <class Cut>
 __device__ __forceinline__ uint32_t attn_request_cost(const AttnParams& p, const AttnRequest& r, bool whole)
 {
     const int blocks = attn_blocks(r, p.group.d, Cut::ROWS);
     uint32_t sum = 0;
-    for (int b = threadIdx.x & 31; b < blocks; b += 32) sum += attn_unit_cost<Cut>(p, r, b, whole);
+    for (int b = threadIdx.x & 31; b < blocks; b += 32) sum = attn_sum(sum, attn_unit_cost<Cut>(p, r, b, whole), 1u << 26);
     return __reduce_add_sync(~0u, sum);
 }
 
@@ -98,7 +101,7 @@ __device__ __forceinline__ AttnTotals attn_totals(const AttnParams& p, AttnShare
             const AttnRequest r = attn_request(p, i);
             keys += r.keys;
             const int blocks = by_warps ? 0 : attn_blocks(r, p.group.d, Cut::ROWS);
-            for (int b = 0; b < blocks; ++b) cost += attn_unit_cost<Cut>(p, r, b, t.whole);
+            for (int b = 0; b < blocks; ++b) cost = attn_sum(cost, attn_unit_cost<Cut>(p, r, b, t.whole), 1u << 31);
         }
         if (!by_warps) sh.cost[threadIdx.x] = cost;
     }
@@ -128,7 +131,7 @@ __device__ __forceinline__ AttnTotals attn_totals(const AttnParams& p, AttnShare
     for (int w = 0; w < ATTN_ENTRIES / 32; ++w) { total += sh.total[w]; keys += sh.keys[w]; }
     total *= p.kv_heads;
     if (total > ATTN_MOST_TILES) {
-        if (threadIdx.x == 0) atomicExch(p.status, 40);
+        if (threadIdx.x == 0) atomicExch(p.status, ATTN_TOO_MUCH);
         total = 0;
     }
     t.total = (int)total;

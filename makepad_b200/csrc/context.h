@@ -60,6 +60,7 @@ struct mpq_context {
 namespace mpq {
 
 constexpr int ATTN_COUNTERS = 4096;     // two for each run of an attention kernel, at most
+constexpr int ATTN_TOO_MUCH = 40;       // in the attention kernels' status word: not a wait that ran out
 constexpr uint32_t CTX_MAGIC = 0x4D505143u;
 
 inline int32_t fail(mpq_context* ctx, int32_t code, const char* fmt, ...)

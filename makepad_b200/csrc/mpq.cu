@@ -1448,6 +1448,7 @@ extern "C" int32_t mpq_context_poll_status(mpq_context* ctx)
             cudaMemset(ctx->q4_partials, 0, (size_t)ctx->q4_partials_ctas * Q4S_SLOT_BYTES_PER_CTA);
         if (i == 2) cudaMemset(stat + 256, 0, Q4_STATIC_SLOT_BYTES);
         if (i == 3) cudaMemset(ctx->attn_arrived, 0, ATTN_COUNTERS * sizeof(uint32_t));
+        if (i == 3 && v == ATTN_TOO_MUCH) return fail(ctx, MPQ_ERR_UNSUPPORTED, "an attention call of more than 2^30 tiles of keys was not begun");
         return fail(ctx, MPQ_ERR_PEER_TIMEOUT, "a bounded device-side wait ran out (%s kernel, code %d)", names[i], v);
     }
     return MPQ_OK;

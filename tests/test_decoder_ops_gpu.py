@@ -618,6 +618,22 @@ def test_calls_on_another_stream(ctx):
     ctx.check(ctx.lib.mpq_context_poll_status(ctx.h))
 
 
+def test_more_work_than_a_call_may_have():
+    """2^24 tokens of one prompt are 2^32 + 2^17 tiles with the units' ends: not 2^17.  Nothing is begun, and the status says why."""
+    torch, m = _t(), _m()
+    own = m.Context(0)
+    rows = torch.zeros((1 << 24, 1, 64), dtype=torch.bfloat16, device="cuda")
+    out = torch.ones_like(rows)
+    m.prompt_attention(own, rows, rows, rows, _ints([0, 1 << 24]), out=out)
+    with pytest.raises(m.MpqError) as e:
+        own.check(own.lib.mpq_context_poll_status(own.h))
+    assert e.value.status == m._lib.ERR_UNSUPPORTED and bool((out == 1).all())
+    own.check(own.lib.mpq_context_poll_status(own.h))
+    m.prompt_attention(own, rows[:300], rows[:300], rows[:300], _ints([0, 300]), out=out[:300])       # the context goes on
+    own.check(own.lib.mpq_context_poll_status(own.h))
+    assert bool((out[:300] == 0).all()) and bool((out[300:] == 1).all())
+
+
 def test_two_contexts_at_once():
     """Calls of two contexts on two streams, beside each other: each has its own pieces and counters."""
     torch, m = _t(), _m()
