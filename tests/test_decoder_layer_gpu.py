@@ -193,6 +193,37 @@ def test_a_captured_decode_step(ctx):
     assert torch.equal(graphed["cache"].lens, eager["cache"].lens) and graphed["cache"].lens.tolist() == [20] * n
 
 
+@pytest.mark.parametrize("kind", ["q4", "nvfp4"])
+@pytest.mark.parametrize("room", [12, 40, 150])
+def test_rows_behind_the_last_token_touch_nothing(ctx, kind, room):
+    """A step with room for more rows than it has tokens: whatever the others hold, the tokens' rows and the cache are the same."""
+    import makepad_b200 as m
+    torch = _t()
+    layers, last = _layers(ctx, kind, 2, 256, 8, 2, 64, 512, True)
+    new = torch.tensor([3, 0, 5, 1], dtype=torch.int32, device="cuda")
+    rows = torch.randn(room, 256, device="cuda", generator=torch.Generator(device="cuda").manual_seed(6))
+    got = []
+    for dead in (0.0, math.nan, 3e38):
+        x = rows.clone()
+        x[9:] = dead
+        cache = m.PagedCache(ctx, 2, 8, 2, 64, 4, 2, 16)
+        step = cache.plan(new, room)
+        r = torch.zeros(room, 256, device="cuda")
+        r[9:] = dead
+        spoilt = [torch.full((room, w), math.nan, dtype=t, device="cuda") for w in (256, 512, 768, 1024) for t in (torch.float32, torch.bfloat16)]
+        del spoilt                                       # (what is allocated next lies there)
+        x, post = x.to(layers[0].dtype), None
+        for i, l in enumerate(layers):
+            r, x = l(r, x, step, cache, i, post=post)
+            post = l.ffn_post
+        got.append((_finish(ctx, layers, last, r, x)[:9], *cache.k, *cache.v))
+    assert bool(torch.isfinite(got[0][0]).all())
+    for other in got[1:]:
+        for a, b in zip(got[0], other):
+            assert torch.equal(a, b)
+    ctx.check(ctx.lib.mpq_context_poll_status(ctx.h))
+
+
 def test_layers_refuse_what_does_not_fit(ctx):
     import makepad_b200 as m
     torch = _t()

@@ -618,6 +618,37 @@ def test_calls_on_another_stream(ctx):
     ctx.check(ctx.lib.mpq_context_poll_status(ctx.h))
 
 
+@pytest.mark.parametrize("new,max_new", [([1, 1], 1), ([70, 3], 0)])
+def test_a_cache_behind_32_bits(ctx, new, max_new):
+    """Pages whose elements lie beyond 2^32 of a cache, and rows of q that lie 2^32 elements apart, give what a small cache and packed rows give."""
+    torch, m = _t(), _m()
+    q_heads, kv_heads, D, page, T = 8, 2, 128, 64, sum(new)
+    lens, pages = [130, 75], (1 << 32) // (2 * 64 * 128) + 8
+    starts, lens_dev, table = _ints([0, new[0], T]), _ints(lens), [[0, 1, 2], [3, 4, 0]]
+    qkv = _randn(5, T, (q_heads + 2 * kv_heads) * D)
+    places = [(i, lens[i] - n + j) for i, n in enumerate(new) for j in range(n)]
+    freq, positions = m.rotary_frequencies(ctx, D), _ints([t for _, t in places])
+    small = [_randn(6 + i, 5, kv_heads, page, D, dtype=torch.bfloat16) for i in (0, 1)]
+    outs, kept = [], []
+    for base in (0, pages - 5):
+        k, v = (torch.empty(pages, kv_heads, page, D, dtype=torch.bfloat16, device="cuda") for _ in (0, 1)) if base else (s.clone() for s in small)
+        if base:
+            k[base:] = small[0]
+            v[base:] = small[1]
+        slots = torch.tensor([(table[i][t // page] + base) * page + t % page for i, t in places], dtype=torch.int64, device="cuda")
+        q, _, _ = m.kv_append(ctx, qkv, q_heads, kv_heads, positions=positions, frequencies=freq, k_cache=k, v_cache=v, slots=slots)
+        if base and T < 5:
+            far = torch.empty(5 << 30, dtype=torch.bfloat16, device="cuda").as_strided((T, q_heads, D), (4 << 30, D, 1))
+            far.copy_(q)
+            q = far
+        outs.append(m.paged_attention(ctx, q, k, v, starts, lens_dev, _ints(table) + base, max_new=max_new))
+        kept.append((k[base:base + 5].clone(), v[base:base + 5].clone()))
+        del k, v, q
+    assert torch.equal(outs[0], outs[1]) and all(torch.equal(a, b) for a, b in zip(*kept))
+    assert not torch.equal(kept[0][0], small[0])
+    ctx.check(ctx.lib.mpq_context_poll_status(ctx.h))
+
+
 def test_more_work_than_a_call_may_have():
     """2^24 tokens of one prompt are 2^32 + 2^17 tiles with the units' ends: not 2^17.  Nothing is begun, and the status says why."""
     torch, m = _t(), _m()
