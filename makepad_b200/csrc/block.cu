@@ -67,11 +67,17 @@ constexpr int64_t MOST_KEYS = 1ll << 30;      // of a request, and rows of a cal
 template <class X, class Y>
 static cudaError_t norm_launch(const mpq_context* ctx, const NormParams& p, int64_t M, cudaStream_t s)
 {
-    // One group of eight columns per thread where that makes a CTA.  (Several per thread, for fewer barriers per byte, are slower: 8192 rows of 8192 columns,
-    // bf16, with both norms and a gate, 1 / 2 / 4 / 8 groups 160 / 162 / 171 / 208 us; 2000 rows without the first norm 43 / 46 / 50 / 63.)
-    const int groups = p.H / 8, nv = groups <= 1024 ? 1 : groups <= 2048 ? 2 : 4;
+    // Groups of eight columns per thread, and CTAs on an SM.  Two groups: 8192 bf16 rows of 4096 columns, both norms and a gate, 72 us (one group, twice the warps at their
+    // barriers, 76; four 71), 500 rows 6.4 (6.8; 7.8), fp32 rows of 8192 columns 199 (203; 214).  A row of more than 4096 bf16 columns with a norm behind the block has nothing on its
+    // way while its first sum is made: three such rows on an SM instead of two want four groups (8192 rows of 8192 columns 139, two groups 152, one 160), where there are so many
+    // rows (64: 5.1 and 4.8).
+    const int groups = p.H / 8;
+    const bool three = sizeof(X) == 2 && p.post_weight && groups > 512 && groups <= 1024 && M > ctx->prop.multiProcessorCount;
+    const int nv = three || groups > 2048 ? 4 : 2;
     const unsigned threads = (unsigned)((groups + nv - 1) / nv + 31) / 32 * 32;
-    auto kernel = nv == 1 ? residual_norm_kernel<1, X, Y> : nv == 2 ? residual_norm_kernel<2, X, Y> : residual_norm_kernel<4, X, Y>;
+    auto kernel = groups <= 1024 ? residual_norm_kernel<512, 2, 2, X, Y> : groups <= 2048 ? residual_norm_kernel<1024, 1, 2, X, Y> : residual_norm_kernel<1024, 1, 4, X, Y>;
+    if constexpr (sizeof(X) == 2)
+        if (three) kernel = residual_norm_kernel<256, 3, 4, X, Y>;
     return launch_beside(ctx, kernel, dim3((unsigned)M), threads, 0, 1, s, p);
 }
 

@@ -5,10 +5,11 @@
 //   r' = r + alpha * gate * t                           gate: one value per column, or per element
 //   y  = r' / sqrt(mean(r'^2) + eps) * weight           what the next block reads
 //
-// A CTA has a row, a thread NV groups of eight columns (one, up to 8192 columns), which stay in registers from the load to the last store: x and r are
-// read once, r' and y written once.  Sums of squares are fp32, in a fixed order.  Bound: HBM, (x + 4 + 4 + y) bytes per element (8192 bf16 rows of 8192 columns, both norms, a gate: 160 us, 5.0 TB/s; CTAs that
-// stay, with a ring of rows ahead of them, 174: a row's two sums then wait for each other);
-// the weights and a gate of one row are read by every CTA and come from L1 / L2.
+// A CTA has a row, a thread NV groups of eight columns, which stay in registers (x as it came) from the load to the last store: x and r are
+// read once, r' and y written once.  Sums of squares are fp32, in a fixed order.  Bound: HBM, (x + 4 + 4 + y) bytes per element: 8192 bf16 rows of 8192 columns, both norms,
+// a gate 139 us (in place, 5.8 TB/s; 153 with other rows to write to); without the norm behind the block 119, 6.8 TB/s.  What is between is the first sum, during which a row has no traffic: rows on an SM count.  (CTAs that stay, the
+// next row's loads in registers and the weights in shared memory: 151; in a ring of bulk copies 174, of cp.async 197.)
+// The weights and a gate of one row are read by every CTA and come from L1 / L2.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -86,20 +87,37 @@ __device__ __forceinline__ float norm_block_sum(float v, float* sums)
     return v;
 }
 
-template <int NV, class X, class Y>
-__global__ void __launch_bounds__(1024) residual_norm_kernel(const __grid_constant__ NormParams p)
+// Eight columns as they lie in memory
+template <class X>
+struct RawEight;
+template <>
+struct RawEight<__nv_bfloat16> {
+    uint4 a;
+    __device__ __forceinline__ void load(const __nv_bfloat16* p) { a = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ Eight eight() const { return eight_of_bf16(a); }
+};
+template <>
+struct RawEight<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float* p) { a = *reinterpret_cast<const float4*>(p); b = *reinterpret_cast<const float4*>(p + 4); }
+    __device__ __forceinline__ Eight eight() const { return Eight{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}}; }
+};
+
+template <int THREADS, int CTAS, int NV, class X, class Y>
+__global__ void __launch_bounds__(THREADS, CTAS) residual_norm_kernel(const __grid_constant__ NormParams p)
 {
     __shared__ float s_sums[2][32];
     start_beside();
     const int64_t row = blockIdx.x, base = row * p.H;
     const int step = blockDim.x * 8, c0 = threadIdx.x * 8;
     const X* x = static_cast<const X*>(p.x) + base;
-    Eight t[NV], r[NV];
+    RawEight<X> raw[NV];
+    Eight r[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = c0 + i * step;
-        if (c < p.H) t[i] = load_eight(x + c);
-        else t[i] = Eight{};
+        raw[i] = RawEight<X>{};
+        if (c < p.H) raw[i].load(x + c);
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -107,43 +125,43 @@ __global__ void __launch_bounds__(1024) residual_norm_kernel(const __grid_consta
         if (p.residual && c < p.H) r[i] = load_eight(p.residual + base + c);
         else r[i] = Eight{};
     }
+    float scale = 1.f;
     if (p.post_weight) {
         float sq = 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sq = fmaf(t[i].v[j], t[i].v[j], sq);
-        const float scale = 1.f / sqrtf(norm_block_sum(sq, s_sums[0]) / (float)p.H + p.eps);
-#pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = c0 + i * step;
-            if (c < p.H) {
-                const Eight w = load_eight(p.post_weight + c);
+            const Eight t = raw[i].eight();
 #pragma unroll
-                for (int j = 0; j < 8; ++j) t[i].v[j] = t[i].v[j] * scale * w.v[j];
-            }
+            for (int j = 0; j < 8; ++j) sq = fmaf(t.v[j], t.v[j], sq);
         }
+        scale = 1.f / sqrtf(norm_block_sum(sq, s_sums[0]) / (float)p.H + p.eps);
     }
     float sq = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = c0 + i * step;
         if (c < p.H) {
+            Eight t = raw[i].eight();
+            if (p.post_weight) {
+                const Eight w = load_eight(p.post_weight + c);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) t.v[j] = t.v[j] * scale * w.v[j];
+            }
             if (p.gate) {
                 const Eight g = load_eight(p.gate + row * p.gate_stride + c);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) t[i].v[j] *= g.v[j];
+                for (int j = 0; j < 8; ++j) t.v[j] *= g.v[j];
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                r[i].v[j] = fmaf(p.alpha, t[i].v[j], r[i].v[j]);
+                r[i].v[j] = fmaf(p.alpha, t.v[j], r[i].v[j]);
                 sq = fmaf(r[i].v[j], r[i].v[j], sq);
             }
             if (p.residual_out) store_eight(p.residual_out + base + c, r[i]);
         }
     }
     if (!p.y) return;
-    const float scale = 1.f / sqrtf(norm_block_sum(sq, s_sums[1]) / (float)p.H + p.eps);
+    scale = 1.f / sqrtf(norm_block_sum(sq, s_sums[1]) / (float)p.H + p.eps);
     Y* y = static_cast<Y*>(p.y) + base;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
