@@ -19,7 +19,7 @@ namespace mpq {
 constexpr int FEW_MOST_CTAS = 256, FEW_TILE = 128, FEW_WARPS = 4, FEW_KEYS = FEW_TILE / FEW_WARPS, FEW_THREADS = 32 * (FEW_WARPS + 1);
 // a unit's end (sums joined, pieces stored and counted) takes a CTA about as long as two tiles
 template <int NT>
-using FewCut = AttnCut<8 * NT, FEW_TILE, 2, 2, false>;
+using FewCut = AttnCut<8 * NT, FEW_TILE, 2, 2, false, 0>;
 static_assert(FEW_THREADS >= ATTN_ENTRIES, "an entry per thread");
 
 template <int D, int NT>

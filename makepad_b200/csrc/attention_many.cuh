@@ -29,7 +29,7 @@ namespace mpq {
 
 constexpr int MANY_ROWS = 256, MANY_TILE = 128, MANY_THREADS = 640;
 constexpr int MANY_REGS_WORK = 104, MANY_REGS_REST = 64;         // 4 x 104 + 64 = 5 x 96, what a thread is launched with
-using ManyCut = AttnCut<MANY_ROWS, MANY_TILE, 1, 4, true>;
+using ManyCut = AttnCut<MANY_ROWS, MANY_TILE, 1, 4, true, 6>;
 constexpr int MANY_POWERS = 4;                                    // every so many pairs of weights by a polynomial: see power2
 constexpr float MANY_LATE = 8.f;                                  // log2 of how far a row's maximum runs ahead of the one in use
 

@@ -432,6 +432,20 @@ def test_paged_attention_long(ctx, new, length, heads):
     _check_paged(ctx, new, lens, *heads, 32)
 
 
+@pytest.mark.parametrize("new,lens,heads", [([40] * 16, [700] * 16, (32, 8, 64)), ([40] * 19, [700] * 19, (32, 8, 64)), ([40, 0, 33] + [40] * 10, [700, 900, 33] + [1400] * 10, (16, 8, 128)),
+                                            ([40] * 3, [5000, 40, 41], (8, 2, 128)), ([64, 20], [900, 2000], (8, 8, 128))])
+def test_paged_attention_about_a_unit_for_each_cta(ctx, new, lens, heads):
+    """Fewer units than SMs, and a few more; of like lengths, and not."""
+    _check_paged(ctx, new, lens, *heads, 64)
+
+
+@pytest.mark.parametrize("length", [41, 600, 5000])
+def test_paged_attention_of_a_few_among_many_requests(ctx, length):
+    """Several requests to an entry of the sums, most of them without new tokens."""
+    new = [40 if i in (0, 77, 399) else 0 for i in range(400)]
+    _check_paged(ctx, new, [length if k else 30 for k in new], 8, 2, 128, 16)
+
+
 def test_paged_attention_many_requests(ctx):
     r = random.Random(1)
     lens = [r.randint(1, 300) for _ in range(700)]
