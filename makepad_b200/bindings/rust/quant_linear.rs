@@ -194,3 +194,25 @@ impl PagedCache {
         })
     }
 }
+
+/// Rotary positions of rows [q heads | k heads | v heads][head_dim]: angle = positions[t] * frequencies[i] (f64, rot_dim / 2 of them; rot_dim 0: none).
+pub struct Rotary { pub positions: DevicePtr, pub frequencies: DevicePtr, pub rot_dim: i32, pub interleaved: bool }
+
+/// QKV rows of a step: q rounded to bf16 rows, k and v into the cache at the step's slots.
+pub fn append(ctx: &Context, qkv: DevicePtr, is_bf16: bool, row_stride: i64, q_heads: i32, rotary: &Rotary, step: &Step, q: DevicePtr, cache: &PagedCache, stream: *mut c_void) -> Result<(), MpqError> {
+    ctx.check(unsafe {
+        (ctx.lib.mpq_kv_append)(ctx.raw, qkv.0, is_bf16 as i32, row_stride, step.tokens, q_heads, cache.kv_heads, cache.head_dim, rotary.positions.0 as *const i32,
+                                rotary.frequencies.0 as *const f64, rotary.rot_dim, rotary.interleaved as i32, q.0 as *mut u16, null_mut(), null_mut(), step.slots.0 as *const i64,
+                                cache.k.0 as *mut u16, cache.v.0 as *mut u16, cache.pages, cache.page_size, stream)
+    })
+}
+
+/// Whole prompts, packed at starts (i32 [n + 1]); q, k and v bf16 rows, one behind the other.
+pub fn prompt_attention(ctx: &Context, q: DevicePtr, k: DevicePtr, v: DevicePtr, tokens: i64, q_heads: i32, kv_heads: i32, head_dim: i32, n: i64, starts: DevicePtr, scale: f32, out: DevicePtr,
+                        out_is_f32: bool, stream: *mut c_void) -> Result<(), MpqError> {
+    let (wide, narrow) = (q_heads as i64 * head_dim as i64, kv_heads as i64 * head_dim as i64);
+    ctx.check(unsafe {
+        (ctx.lib.mpq_prompt_attention)(ctx.raw, q.0 as *const u16, wide, k.0 as *const u16, narrow, v.0 as *const u16, narrow, tokens, q_heads, kv_heads, head_dim, n, starts.0 as *const i32,
+                                       scale, out.0, out_is_f32 as i32, stream)
+    })
+}
