@@ -110,10 +110,15 @@ extern "C" int32_t mpq_context_create(int32_t device, mpq_context** out)
         delete c;
         return fail(nullptr, MPQ_ERR_CUDA, "");
     }
-    // (here and not in the first attention call: that one may be in a capture)
+    // (Here and not in the first attention call, which may be in a capture.  Another stream may be in one now, too: nothing of this is
+    // recorded there, so the thread's mode lets it pass, and the zeros do not go by the legacy stream, which would end that capture.)
     void* counters = nullptr;
-    if (cudaMalloc(&counters, (ATTN_COUNTERS + 1) * sizeof(uint32_t)) != cudaSuccess || cudaMemset(counters, 0, (ATTN_COUNTERS + 1) * sizeof(uint32_t)) != cudaSuccess ||
-        cudaStreamSynchronize(nullptr) != cudaSuccess) {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    const bool counts = cudaMalloc(&counters, (ATTN_COUNTERS + 1) * sizeof(uint32_t)) == cudaSuccess &&
+                        cudaMemsetAsync(counters, 0, (ATTN_COUNTERS + 1) * sizeof(uint32_t), c->upload_stream) == cudaSuccess && cudaStreamSynchronize(c->upload_stream) == cudaSuccess;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (!counts) {
         cudaFree(counters);
         cudaStreamDestroy(c->upload_stream);
         delete c;
