@@ -300,7 +300,7 @@ int32_t mpq_kv_append(mpq_context* ctx, const void* qkv_dev, int32_t x_is_bf16, 
  * (0: not known); it chooses the kernel, not the result.  An entry of the table outside the cache reads as zeros; what lies behind
  * lens[i] in the last page is not used, whatever it holds.  k and v of the new tokens are read by rows that do not see them:
  * they must be finite.  Sums are fp32, the weights of v are rounded to bf16.
- * scale must be finite and not negative.  tokens and max_blocks * page_size at most 2^30, tokens * q_heads / kv_heads below 2^31.  The pieces of units that CTAs share
+ * scale must be finite and not negative.  n at most 2^20; tokens and max_blocks * page_size at most 2^30, tokens * q_heads / kv_heads below 2^31.  The pieces of units that CTAs share
  * lie in the context's scratch (one stream per context at a time; graphs captured on one context must not run beside each other), which the first call outside a
  * capture reserves.  A call of more than 2^30 tiles (128 keys of a head and a block of rows) is not begun: mpq_context_poll_status gives MPQ_ERR_UNSUPPORTED. */
 int32_t mpq_paged_attention(mpq_context* ctx, const uint16_t* q_dev, int64_t q_row_stride, int64_t tokens, int32_t q_heads, const uint16_t* k_cache_dev,

@@ -75,7 +75,6 @@ __device__ __forceinline__ uint32_t attn_request_cost(const AttnParams& p, const
     return __reduce_add_sync(~0u, sum);
 }
 
-constexpr int ATTN_ENTRIES = 160;
 struct AttnShared {
     uint32_t cost[ATTN_ENTRIES];            // tiles of a head, of `per` requests each
     long long total[5], keys[5], units[5];  // of 32 entries each
@@ -93,7 +92,7 @@ __device__ __forceinline__ AttnTotals attn_totals(const AttnParams& p, AttnShare
     const int warps = blockDim.x >> 5, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     AttnTotals t;
     t.whole = !p.partial;
-    t.per = (p.n + ATTN_ENTRIES - 1) / ATTN_ENTRIES;
+    t.per = attn_per(p.n);
     long long keys = 0, units = 0;
     int most = 0;
     uint32_t cost = 0;
@@ -182,6 +181,17 @@ struct AttnWalk {
         blocks = attn_blocks(r, p.group.d, Cut::ROWS);
         fetch(p, request + 1);
     }
+    // to the next request with rows (there is one: the run goes on), a lane for each of 32
+    __device__ __forceinline__ void skip(const AttnParams& p)
+    {
+        for (uint32_t some = 0; !some && ++request < p.n;) {
+            const int i = request + (threadIdx.x & 31);
+            some = __ballot_sync(~0u, i < p.n && attn_request(p, i).rows > 0);
+            request += some ? __ffs(some) - 1 : 31;
+        }
+        fetch(p, request);
+        enter(p);
+    }
     __device__ __forceinline__ void size(const AttnParams& p) { tiles = attn_block_tiles(r, p.group, block, Cut::ROWS, Cut::TILE); }
 
     // a lane's `own` tiles behind all lanes in front of it and `at`: the lane with tile lo, and everything in front of it passed
@@ -254,10 +264,9 @@ struct AttnWalk {
             block = 0;
             if (++head >= p.kv_heads) {
                 head = 0;
-                do {
-                    ++request;
-                    enter(p);
-                } while (!blocks);                               // (there is one: unit < hi)
+                ++request;
+                enter(p);
+                if (!blocks) skip(p);
             }
         }
         size(p);

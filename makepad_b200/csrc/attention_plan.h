@@ -98,6 +98,11 @@ MPQ_BOTH int attn_end(int hi, int unit, int tiles, int least) { return hi - unit
 MPQ_BOTH int attn_opener(int unit, int tiles, int least, int total, int runs) { return attn_owner(unit + attn_least(tiles, least) - 1, total, runs); }
 MPQ_BOTH int attn_closer(int unit, int tiles, int least, int total, int runs) { return attn_owner(unit + tiles - attn_least(tiles, least), total, runs); }
 constexpr int ATTN_MOST_RUNS = 2048;
+// Requests of a call: every CTA adds them up in ATTN_ENTRIES entries and walks through those of one entry, and through the ones without rows, while others
+// wait for it: 3 and 10 ms (many rows, few) for this many of which only the first and the last have rows.  The waits give up after a few hundred.
+constexpr int64_t ATTN_MOST_REQUESTS = 1 << 20;
+constexpr int ATTN_ENTRIES = 160;
+MPQ_BOTH int attn_per(int n) { return (n + ATTN_ENTRIES - 1) / ATTN_ENTRIES; }
 constexpr int64_t ATTN_MOST_TILES = 1ll << 30;         // of a call: what has more (hours of work) is not begun, and says so in the status word
 
 // Into how many parts, one after the other, all tiles are cut before each part is cut into a run per CTA: so many that the keys and values of a part

@@ -181,7 +181,8 @@ struct AttnKeys {
 static int32_t attention_check(mpq_context* ctx, const AttnParams& p, const AttnKeys& kv, int64_t n, int64_t q_heads, int64_t kv_heads, int32_t head_dim, float scale)
 {
     if (!p.q || !kv.k || !kv.v || !p.starts || !p.out) return fail(ctx, MPQ_ERR_INVALID_ARG, "null pointer");
-    if (p.tokens <= 0 || p.tokens > MOST_KEYS || n <= 0 || n > MOST) return fail(ctx, MPQ_ERR_SHAPE, "tokens and n must be positive, tokens at most 2^30, n below 2^31");
+    if (p.tokens <= 0 || p.tokens > MOST_KEYS || n <= 0) return fail(ctx, MPQ_ERR_SHAPE, "tokens and n must be positive, tokens at most 2^30");
+    if (n > ATTN_MOST_REQUESTS) return fail(ctx, MPQ_ERR_UNSUPPORTED, "more than %lld requests", (long long)ATTN_MOST_REQUESTS);
     if (q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || q_heads > 4096)
         return fail(ctx, MPQ_ERR_SHAPE, "q_heads must be a multiple of kv_heads, at most 4096 (%lld and %lld)", (long long)q_heads, (long long)kv_heads);
     if (p.tokens * p.group.d > MOST) return fail(ctx, MPQ_ERR_UNSUPPORTED, "tokens * q_heads / kv_heads must be below 2^31");
