@@ -7,6 +7,8 @@
  * device memory on the context's GPU.  Handles are owned by the library and
  * released by their _destroy call.  "stream" is a cudaStream_t passed as
  * void* (NULL = the legacy default stream); forward calls only enqueue work.
+ * What a decoder layer calls (linears on device arrays, quantisation, SwiGLU,
+ * everything between the projections) leaves the current device as it was.
  *
  * Reference interface replaced: none exists.  The makepad/makepad snapshot has
  * no quantised-linear operator, tensor type or CUDA binding; its only AI code
@@ -257,7 +259,7 @@ int32_t mpq_nvfp4_dequantize(mpq_context* ctx, int64_t R, int64_t K, const uint8
 /* No counterpart in the reference.  Rows are packed: the new tokens of request i of n are rows starts[i] .. starts[i+1]-1 of
  * the activations (starts: n+1 int32 on the device, ascending from 0); rows behind starts[n] belong to nobody and are
  * left as they are.  bf16 arrays are uint16_t bits.  All pointers 16-byte aligned unless a scalar or int array.  The lengths are read
- * on the device: a captured call follows them.  These calls leave the current device as it was. */
+ * on the device: a captured call follows them. */
 
 /* Norms around a block and the residual sum between them, per row of H columns (H a multiple of 8, at most 32768):
  *   t = x;  t = t / sqrt(mean(t^2) + eps) * post_weight   if post_weight is given (the norm behind the block)

@@ -38,20 +38,6 @@ cudaError_t launch_beside(const mpq_context* ctx, void (*kernel)(P...), dim3 gri
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 
-// The context's device for the length of a call; the caller's is set again behind it.
-class OnDevice {
-public:
-    explicit OnDevice(int device)
-    {
-        if ((error = cudaGetDevice(&before_)) == cudaSuccess && before_ != device && (error = cudaSetDevice(device)) == cudaSuccess) moved_ = true;
-    }
-    ~OnDevice() { if (moved_) cudaSetDevice(before_); }
-    cudaError_t error;
-private:
-    int before_ = 0;
-    bool moved_ = false;
-};
-
 bool power_of_two(int64_t v) { return v > 0 && !(v & (v - 1)); }
 int log2_of(int64_t v) { int s = 0; while ((1ll << s) < v) ++s; return s; }
 bool page_ok(int64_t page_size) { return power_of_two(page_size) && page_size >= 16 && page_size <= 256; }

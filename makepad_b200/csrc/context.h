@@ -11,6 +11,7 @@
 #include "../../include/mpq.h"
 #include "host_pages.h"
 #include "nvfp4.cuh"
+#include "on_device.h"
 #include "scratch.h"
 #include "upload.h"
 

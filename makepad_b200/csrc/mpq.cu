@@ -1090,7 +1090,8 @@ extern "C" int32_t mpq_q4_linear_forward(mpq_context* ctx, const mpq_weight* w, 
     int32_t st = q4_validate(ctx, w, x_dev, M, y_dev);
     if (st) return st;
     if (!aligned16(x_dev) || !aligned16(y_dev)) return fail(ctx, MPQ_ERR_ALIGN, "x and y must be 16-byte aligned");
-    CU_TRY(ctx, cudaSetDevice(ctx->device));
+    const OnDevice on(ctx->device);
+    CU_TRY(ctx, on.error);
     return q4_forward_checked(ctx, w, x_dev, M, y_dev, w->q4.N, (cudaStream_t)stream);
 }
 
@@ -1130,7 +1131,8 @@ extern "C" int32_t mpq_swiglu(mpq_context* ctx, const float* gate_up_dev, int64_
 {
     int32_t st = swiglu_check(ctx, gate_up_dev, M, F, out_dev);
     if (st) return st;
-    CU_TRY(ctx, cudaSetDevice(ctx->device));
+    const OnDevice on(ctx->device);
+    CU_TRY(ctx, on.error);
     return swiglu_launch(ctx, gate_up_dev, M, F, out_dev, (cudaStream_t)stream);
 }
 
@@ -1142,7 +1144,8 @@ extern "C" int32_t mpq_q4_linear_forward_swiglu(mpq_context* ctx, const mpq_weig
     int32_t st = q4_validate(ctx, w, gate_up_dev, M, y_dev);
     if (st) return st;
     if (!aligned16(gate_up_dev) || !aligned16(y_dev)) return fail(ctx, MPQ_ERR_ALIGN, "gate_up and y must be 16-byte aligned");
-    CU_TRY(ctx, cudaSetDevice(ctx->device));
+    const OnDevice on(ctx->device);
+    CU_TRY(ctx, on.error);
     const Q4Dev& q = w->q4;
     cudaStream_t s = (cudaStream_t)stream;
     Q4StreamPlan pl;
@@ -1238,7 +1241,8 @@ extern "C" int32_t mpq_q4_linear_forward_static(mpq_context* ctx, const mpq_weig
     if (st) return st;
     if (!aligned16(x_dev) || !aligned16(y_dev)) return fail(ctx, MPQ_ERR_ALIGN, "x and y must be 16-byte aligned");
     if (ctx->device < 0 || ctx->device >= PerDeviceOnce::MAX_DEVICES) return fail(ctx, MPQ_ERR_UNSUPPORTED, "device index %d beyond the static table", ctx->device);
-    CU_TRY(ctx, cudaSetDevice(ctx->device));
+    const OnDevice on(ctx->device);
+    CU_TRY(ctx, on.error);
     if (!g_q4_static_ptr[ctx->device]) {                  // set-up: the first call on this device
         void* p = nullptr;
         CU_TRY(ctx, cudaGetSymbolAddress(&p, g_q4_static_scratch));
@@ -1431,7 +1435,8 @@ extern "C" int32_t mpq_q4_linear_forward_allreduce(mpq_context* ctx, const mpq_w
     Q4StreamPlan pl;
     if (M > 4 || !q4_stream_plan(ctx, w->q4, (int)M, &pl))
         return fail(ctx, MPQ_ERR_UNSUPPORTED, "the fused all-reduce needs M <= 4 and an activation that fits in shared memory");
-    CU_TRY(ctx, cudaSetDevice(ctx->device));
+    const OnDevice on(ctx->device);
+    CU_TRY(ctx, on.error);
     return q4_stream_forward(ctx, w->q4, pl, x_dev, (int)M, y_dev, w->q4.N, ex, (cudaStream_t)stream);
 }
 
@@ -1500,7 +1505,8 @@ extern "C" int32_t mpq_nvfp4_gemm_forward(mpq_context* ctx, const mpq_weight* w,
     if (w->device != ctx->device) return fail(ctx, MPQ_ERR_INVALID_ARG, "weight lives on device %d, context on %d", w->device, ctx->device);
     if (M <= 0 || M > (1LL << 30)) return fail(ctx, MPQ_ERR_SHAPE, "NVFP4 GEMM needs 1 <= M <= 2^30 (M=%lld)", (long long)M);
     if (!aligned16(a_codes_dev) || !aligned16(a_sf_dev) || !aligned16(c_bf16_dev)) return fail(ctx, MPQ_ERR_ALIGN, "A, SFA and C must be 16-byte aligned");
-    CU_TRY(ctx, cudaSetDevice(ctx->device));
+    const OnDevice on(ctx->device);
+    CU_TRY(ctx, on.error);
     std::string err;
     int launches = 0;
     int32_t st = nvfp4_gemm_launch(ctx->fp4, w->fp4, a_codes_dev, a_sf_dev, a_tensor_scale, M, c_bf16_dev, ctx->device,
@@ -1531,7 +1537,8 @@ extern "C" int32_t mpq_nvfp4_quantize_activations(mpq_context* ctx, const void* 
     if (M <= 0 || K <= 0 || K % 16) return fail(ctx, MPQ_ERR_SHAPE, "NVFP4 needs M > 0 and K a positive multiple of 16");
     if (!(tensor_scale > 0.f)) return fail(ctx, MPQ_ERR_INVALID_ARG, "tensor_scale must be positive");
     if (!aligned16(x_dev) || (reinterpret_cast<uintptr_t>(codes_dev) & 7u)) return fail(ctx, MPQ_ERR_ALIGN, "x must be 16-byte, codes 8-byte aligned");
-    CU_TRY(ctx, cudaSetDevice(ctx->device));
+    const OnDevice on(ctx->device);
+    CU_TRY(ctx, on.error);
     ctx->launches += 1;
     CU_TRY(ctx, nvfp4_quantize_launch(x_dev, x_is_bf16 != 0, false, M, K, tensor_scale, codes_dev, sf_dev, ctx->pdl, (cudaStream_t)stream));
     return MPQ_OK;
@@ -1545,7 +1552,8 @@ extern "C" int32_t mpq_nvfp4_quantize_swiglu(mpq_context* ctx, const void* gate_
     if (M <= 0 || F <= 0 || F % 16) return fail(ctx, MPQ_ERR_SHAPE, "NVFP4 needs M > 0 and F a positive multiple of 16");
     if (!(tensor_scale > 0.f)) return fail(ctx, MPQ_ERR_INVALID_ARG, "tensor_scale must be positive");
     if (!aligned16(gate_up_dev) || (reinterpret_cast<uintptr_t>(codes_dev) & 7u)) return fail(ctx, MPQ_ERR_ALIGN, "gate_up must be 16-byte, codes 8-byte aligned");
-    CU_TRY(ctx, cudaSetDevice(ctx->device));
+    const OnDevice on(ctx->device);
+    CU_TRY(ctx, on.error);
     ctx->launches += 1;
     CU_TRY(ctx, nvfp4_quantize_launch(gate_up_dev, x_is_bf16 != 0, true, M, F, tensor_scale, codes_dev, sf_dev, ctx->pdl, (cudaStream_t)stream));
     return MPQ_OK;

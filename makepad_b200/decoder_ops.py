@@ -9,7 +9,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 from . import _lib
-from .quant_linear import Context, MpqError, _raw, _torch
+from .quant_linear import Context, MpqError, _raw, _stream, _torch
 
 
 class KvStep(NamedTuple):
@@ -20,10 +20,6 @@ class KvStep(NamedTuple):
     slots: object         # int64 [tokens], -1 behind the last token
     free_count: object    # int32 [1]
     missing: object       # int32 [1]: 0, or why nothing grew
-
-
-def _stream_of(ctx: Context) -> int:
-    return _torch()._C._cuda_getCurrentRawStream(ctx.device)
 
 
 def _bad(text: str, status: int = _lib.ERR_INVALID_ARG):
@@ -71,7 +67,7 @@ def residual_norm(ctx: Context, x, residual=None, weight=None, *, eps: float = 1
     r = residual if inplace else x.new_empty(M, H, dtype=f32)
     y = x.new_empty(M, H, dtype=out_dtype) if norm else None
     ctx.check(ctx.lib.mpq_residual_norm(_raw(ctx.h), xp, x.dtype is torch.bfloat16, M, H, rp, r.data_ptr(), pp, gp, stride, alpha, wp, eps,
-                                        None if y is None else y.data_ptr(), out_dtype is torch.bfloat16, _stream_of(ctx)))
+                                        None if y is None else y.data_ptr(), out_dtype is torch.bfloat16, _stream(ctx)))
     return r, y
 
 
@@ -96,7 +92,7 @@ def kv_plan(ctx: Context, new_lens, lens, block_table, free, free_count, *, page
     if inplace:
         lens_out, count_out = lens, free_count
     ctx.check(ctx.lib.mpq_kv_plan(_raw(ctx.h), n, np_, lp, lens_out.data_ptr(), tp, blocks, fp, free.numel(), cp, count_out.data_ptr(), page_size, tokens,
-                                  starts.data_ptr(), positions.data_ptr(), slots.data_ptr(), missing.data_ptr(), _stream_of(ctx)))
+                                  starts.data_ptr(), positions.data_ptr(), slots.data_ptr(), missing.data_ptr(), _stream(ctx)))
     return KvStep(starts, lens_out, positions, slots, count_out, missing)
 
 
@@ -141,7 +137,7 @@ def kv_append(ctx: Context, qkv, q_heads: int, kv_heads: int, *, positions=None,
     q = qkv.new_empty(T, q_heads, D, dtype=bf16)
     k, v = (qkv.new_empty(T, kv_heads, D, dtype=bf16), qkv.new_empty(T, kv_heads, D, dtype=bf16)) if rows else (None, None)
     ctx.check(ctx.lib.mpq_kv_append(_raw(ctx.h), qkv.data_ptr(), qkv.dtype is bf16, qkv.stride(0) if T > 1 else wide, T, q_heads, kv_heads, D, pp, fp, rot, interleaved,
-                                    q.data_ptr(), None if k is None else k.data_ptr(), None if v is None else v.data_ptr(), sp, kp, vp, pages, size, _stream_of(ctx)))
+                                    q.data_ptr(), None if k is None else k.data_ptr(), None if v is None else v.data_ptr(), sp, kp, vp, pages, size, _stream(ctx)))
     return q, k, v
 
 
@@ -188,7 +184,7 @@ def paged_attention(ctx: Context, q, k_cache, v_cache, starts, lens, block_table
     sp, lp, tp = _need(ctx, "starts", starts, i32, (n + 1,)), _need(ctx, "lens", lens, i32, (n,)), _need(ctx, "block_table", block_table, i32, (n, blocks))
     out = _out(ctx, q, out_dtype, out)
     ctx.check(ctx.lib.mpq_paged_attention(_raw(ctx.h), qp, stride, T, heads, kp, vp, pages, size, kv_heads, D, n, sp, lp, tp, blocks, max_new,
-                                          D ** -0.5 if scale is None else scale, out.data_ptr(), out.dtype is torch.float32, _stream_of(ctx)))
+                                          D ** -0.5 if scale is None else scale, out.data_ptr(), out.dtype is torch.float32, _stream(ctx)))
     return out
 
 
@@ -204,5 +200,5 @@ def prompt_attention(ctx: Context, q, k, v, starts, *, scale: float = None, out_
     sp = _need(ctx, "starts", starts, torch.int32, (n + 1,))
     out = _out(ctx, q, out_dtype, out)
     ctx.check(ctx.lib.mpq_prompt_attention(_raw(ctx.h), qp, qs, kp, ks, vp, vs, T, heads, k.shape[1], D, n, sp, D ** -0.5 if scale is None else scale,
-                                           out.data_ptr(), out.dtype is torch.float32, _stream_of(ctx)))
+                                           out.data_ptr(), out.dtype is torch.float32, _stream(ctx)))
     return out

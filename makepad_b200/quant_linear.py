@@ -46,11 +46,10 @@ def _torch():
     return _torch_module
 
 
-def _stream() -> int:
-    """The current stream of the current device.  (The stream object that torch.cuda.current_stream() builds costs more host
+def _stream(ctx: "Context") -> int:
+    """The current stream of the context's device, whichever device is current.  (The stream object that torch.cuda.current_stream() builds costs more host
     time than the launch itself.)"""
-    torch = _torch()
-    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+    return _torch()._C._cuda_getCurrentRawStream(ctx.device)
 
 
 class Context:
@@ -105,7 +104,7 @@ class _Weight:
         """Exact fp32 [N][K] export read back from the device layout (torch tensor on the GPU)."""
         import torch
         out = torch.empty((self.N, self.K), dtype=torch.float32, device=f"cuda:{self.ctx.device}")
-        self.ctx.check(self.ctx.lib.mpq_weight_dequantize(self.ctx.h, self.h, out.data_ptr(), _stream()))
+        self.ctx.check(self.ctx.lib.mpq_weight_dequantize(self.ctx.h, self.h, out.data_ptr(), _stream(self.ctx)))
         return out
 
     def save(self, path: str):
@@ -225,12 +224,12 @@ class QuantLinear:
                 shape = x.shape
             M = shape[0]
             y = x.new_empty(M, w.N) if out is None else out
-            ctx.check(ctx.lib.mpq_q4_linear_forward(_raw(ctx.h), _raw(w.h), x.data_ptr(), M, y.data_ptr(), _stream()))
+            ctx.check(ctx.lib.mpq_q4_linear_forward(_raw(ctx.h), _raw(w.h), x.data_ptr(), M, y.data_ptr(), _stream(ctx)))
             return y
         codes, sf, ts = x
         M = codes.shape[0]
         y = codes.new_empty((M, w.N), dtype=torch.bfloat16) if out is None else out
-        ctx.check(ctx.lib.mpq_nvfp4_gemm_forward(_raw(ctx.h), _raw(w.h), codes.data_ptr(), sf.data_ptr(), ts, M, y.data_ptr(), _stream()))
+        ctx.check(ctx.lib.mpq_nvfp4_gemm_forward(_raw(ctx.h), _raw(w.h), codes.data_ptr(), sf.data_ptr(), ts, M, y.data_ptr(), _stream(ctx)))
         return y
 
     __call__ = forward
@@ -246,7 +245,7 @@ class QuantLinear:
             raise MpqError(_lib.ERR_INVALID_ARG, "gate_up must be a contiguous fp32 CUDA tensor")
         g2 = gate_up if gate_up.dim() == 2 and gate_up.shape[1] == 2 * w.K else gate_up.reshape(-1, 2 * w.K)
         y = g2.new_empty(g2.shape[0], w.N) if out is None else out
-        ctx.check(ctx.lib.mpq_q4_linear_forward_swiglu(_raw(ctx.h), _raw(w.h), g2.data_ptr(), g2.shape[0], y.data_ptr(), _stream()))
+        ctx.check(ctx.lib.mpq_q4_linear_forward_swiglu(_raw(ctx.h), _raw(w.h), g2.data_ptr(), g2.shape[0], y.data_ptr(), _stream(ctx)))
         return y
 
 
@@ -255,7 +254,7 @@ def swiglu(ctx: Context, gate_up):
     import torch
     M, F2 = gate_up.shape
     out = torch.empty((M, F2 // 2), dtype=torch.float32, device=gate_up.device)
-    ctx.check(ctx.lib.mpq_swiglu(ctx.h, gate_up.data_ptr(), M, F2 // 2, out.data_ptr(), _stream()))
+    ctx.check(ctx.lib.mpq_swiglu(ctx.h, gate_up.data_ptr(), M, F2 // 2, out.data_ptr(), _stream(ctx)))
     return out
 
 
@@ -270,5 +269,5 @@ def nvfp4_quantize(ctx: Context, x, tensor_scale: float = 1.0, swiglu_fused: boo
     sf = x.new_empty((M, K // 16), dtype=torch.uint8)
     fn = ctx.lib.mpq_nvfp4_quantize_swiglu if swiglu_fused else ctx.lib.mpq_nvfp4_quantize_activations
     ctx.check(fn(_raw(ctx.h), x.data_ptr(), 1 if x.dtype == torch.bfloat16 else 0, M, K, tensor_scale,
-                 codes.data_ptr(), sf.data_ptr(), _stream()))
+                 codes.data_ptr(), sf.data_ptr(), _stream(ctx)))
     return codes, sf
