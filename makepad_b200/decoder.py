@@ -52,10 +52,14 @@ class DecoderLayer:
         self.activation_scales = tuple(float(a) for a in (activation_scales if activation_scales is not None else (1.0,) * 4))
         if len(self.activation_scales) != 4 or not all(2.0 ** -126 <= a <= 2.0 ** 126 for a in self.activation_scales):
             _bad("activation_scales are four positive fp32 numbers: of the rows in front of qkv, o, gate_up and down")
+        if q_heads <= 0 or kv_heads <= 0:
+            _bad("q_heads and kv_heads must be positive", _lib.ERR_SHAPE)
         H, heads = qkv.w.K, q_heads + 2 * kv_heads
         if qkv.w.N % heads or o.w.K * heads != qkv.w.N * q_heads or o.w.N != H or gate_up.w.K != H or down.w.N != H or gate_up.w.N != 2 * down.w.K:
             _bad("the projections' shapes do not fit together", _lib.ERR_SHAPE)
         self.q_heads, self.kv_heads, self.head_dim = q_heads, kv_heads, qkv.w.N // heads
+        if self.head_dim not in (64, 128) or q_heads % kv_heads:
+            _bad(f"the attention has heads of 64 or 128, query heads a multiple of kv_heads ({q_heads} and {kv_heads} heads of {self.head_dim})", _lib.ERR_SHAPE)
         self.attn_norm, self.ffn_norm, self.attn_post, self.ffn_post = attn_norm, ffn_norm, attn_post, ffn_post
         self.frequencies = rotary_frequencies(self.ctx, self.head_dim) if frequencies is None else frequencies
         self.interleaved, self.eps, self.alpha = interleaved, eps, alpha
