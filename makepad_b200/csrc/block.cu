@@ -8,6 +8,7 @@
 #include "kv_cache.cuh"
 #include "launch.h"
 #include "norm.cuh"
+#include "overlap.h"
 #include "per_device.h"
 
 using namespace mpq;
@@ -176,6 +177,10 @@ static int32_t attention_check(mpq_context* ctx, const AttnParams& p, const Attn
     if (p.q_stride < q_heads * head_dim || p.q_stride % 8) return fail(ctx, MPQ_ERR_SHAPE, "a row stride must be a multiple of 8 and hold the heads");
     if (!(scale >= 0.f) || scale - scale != 0.f) return fail(ctx, MPQ_ERR_INVALID_ARG, "scale must be finite and not negative");
     if (!aligned16(p.q) || !aligned16(kv.k) || !aligned16(kv.v) || !aligned16(p.out)) return fail(ctx, MPQ_ERR_ALIGN, "q, k, v and out must be 16-byte aligned");
+    // (other CTAs still read what one has written)
+    const int64_t out_bytes = p.tokens * q_heads * head_dim * (p.out_f32 ? 4 : 2);
+    if (overlaps(p.out, out_bytes, p.q, p.tokens, q_heads * head_dim * 2, (__int128)p.q_stride * 2) || overlaps(p.out, out_bytes, p.starts, 4 * (n + 1)))
+        return fail(ctx, MPQ_ERR_INVALID_ARG, "out must not overlap an input");
     return MPQ_OK;
 }
 
@@ -298,6 +303,10 @@ extern "C" int32_t mpq_paged_attention(mpq_context* ctx, const uint16_t* q_dev, 
     if (pages >= MOST / kv_heads) return fail(ctx, MPQ_ERR_UNSUPPORTED, "pages * kv_heads must be below 2^31");
     if (max_blocks <= 0 || max_blocks > MOST_KEYS / page_size) return fail(ctx, MPQ_ERR_SHAPE, "max_blocks * page_size must be positive and at most 2^30");
     if (max_new < 0) return fail(ctx, MPQ_ERR_SHAPE, "max_new must not be negative");
+    const int64_t out_bytes = tokens * q_heads * head_dim * (out_is_f32 ? 4 : 2), cache_bytes = pages * kv_heads * page_size * head_dim * 2;
+    if (overlaps(out_dev, out_bytes, k_cache_dev, cache_bytes) || overlaps(out_dev, out_bytes, v_cache_dev, cache_bytes) || overlaps(out_dev, out_bytes, lens_dev, 4 * n) ||
+        overlaps(out_dev, out_bytes, block_table_dev, 4 * n * max_blocks))
+        return fail(ctx, MPQ_ERR_INVALID_ARG, "out must not overlap an input");
     p.lens = lens_dev; p.table = block_table_dev;
     p.width = max_blocks; p.pages = pages; p.page_shift = log2_of(page_size);
     return attention_launch(ctx, p, kv, head_dim, (cudaStream_t)stream);
@@ -315,5 +324,8 @@ extern "C" int32_t mpq_prompt_attention(mpq_context* ctx, const uint16_t* q_dev,
     if (st) return st;
     for (int64_t stride : {k_row_stride, v_row_stride})
         if (stride < (int64_t)kv_heads * head_dim || stride % 8) return fail(ctx, MPQ_ERR_SHAPE, "a row stride must be a multiple of 8 and hold the heads");
+    const int64_t out_bytes = tokens * q_heads * head_dim * (out_is_f32 ? 4 : 2), row_bytes = 2ll * kv_heads * head_dim;
+    if (overlaps(out_dev, out_bytes, k_dev, tokens, row_bytes, (__int128)k_row_stride * 2) || overlaps(out_dev, out_bytes, v_dev, tokens, row_bytes, (__int128)v_row_stride * 2))
+        return fail(ctx, MPQ_ERR_INVALID_ARG, "out must not overlap an input");
     return attention_launch(ctx, p, kv, head_dim, (cudaStream_t)stream);
 }
