@@ -266,7 +266,8 @@ int32_t mpq_nvfp4_dequantize(mpq_context* ctx, int64_t R, int64_t K, const uint8
  *   residual_out = residual + alpha * gate * t            residual NULL: 0; gate NULL: 1
  *   y = residual_out / sqrt(mean(residual_out^2) + eps) * weight        weight NULL: 1
  * x [M][H] fp32 or bf16; residuals fp32 [M][H], residual_out may be residual or NULL; weights fp32 [H]; gate fp32 [M][gate_stride]
- * (a multiple of 4, at least H), or one row for all with gate_stride 0; y fp32 or bf16 [M][H], or NULL.  y must not overlap an input. */
+ * (a multiple of 4, at least H), or one row for all with gate_stride 0; y fp32 or bf16 [M][H], or NULL.  Outputs must not overlap, nor lie over an
+ * input; residual_out may also be an fp32 x. */
 int32_t mpq_residual_norm(mpq_context* ctx, const void* x_dev, int32_t x_is_bf16, int64_t M, int64_t H, const float* residual_dev,
                           float* residual_out_dev, const float* post_weight_dev, const float* gate_dev, int64_t gate_stride, float alpha,
                           const float* weight_dev, float eps, void* y_dev, int32_t y_is_bf16, void* stream);
@@ -291,7 +292,7 @@ int32_t mpq_kv_plan(mpq_context* ctx, int64_t n, const int32_t* new_lens_dev, co
  * (2i, 2i+1), by the angle positions[t] * frequencies[i] (fp64 [rot_dim/2]); everything is rounded to bf16 once.  q rows go to
  * q [tokens][q_heads][head_dim]; k and v rows to k, v [tokens][kv_heads][head_dim] unless NULL, and to the cache at slots[t] unless slots is NULL.
  * A row with slots[t] < 0 is skipped altogether; a slot behind the cache writes nothing there.  No slot may come twice.
- * head_dim a multiple of 16, at most 256. */
+ * Outputs must not overlap, nor lie over an input.  head_dim a multiple of 16, at most 256. */
 int32_t mpq_kv_append(mpq_context* ctx, const void* qkv_dev, int32_t x_is_bf16, int64_t row_stride, int64_t tokens, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
                       const int32_t* positions_dev, const double* frequencies_dev, int32_t rot_dim, int32_t interleaved, uint16_t* q_dev, uint16_t* k_dev, uint16_t* v_dev,
                       const int64_t* slots_dev, uint16_t* k_cache_dev, uint16_t* v_cache_dev, int64_t pages, int32_t page_size, void* stream);

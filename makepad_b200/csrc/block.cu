@@ -80,6 +80,15 @@ extern "C" int32_t mpq_residual_norm(mpq_context* ctx, const void* x_dev, int32_
     if (!(eps >= 0.f)) return fail(ctx, MPQ_ERR_INVALID_ARG, "eps must not be negative");
     for (const void* ptr : {x_dev, (const void*)residual_dev, (const void*)residual_out_dev, (const void*)post_weight_dev, (const void*)gate_dev, (const void*)weight_dev, (const void*)y_dev})
         if (!aligned16(ptr)) return fail(ctx, MPQ_ERR_ALIGN, "pointers must be 16-byte aligned");
+    // (a row of an output may lie over other rows' input, or over columns that other threads still read)
+    const int64_t row = 4 * H, all = M * row, x_bytes = M * H * (x_is_bf16 ? 2 : 4), y_bytes = M * H * (y_is_bf16 ? 2 : 4);
+    auto over = [&](const void* out, int64_t bytes) {
+        return overlaps(out, bytes, post_weight_dev, row) || overlaps(out, bytes, weight_dev, row) || overlaps(out, bytes, gate_dev, gate_stride ? M : 1, row, gate_stride ? (__int128)gate_stride * 4 : row);
+    };
+    const bool same_x = !x_is_bf16 && (const void*)residual_out_dev == x_dev;             // a thread reads its columns of x and of the residual in front of its stores
+    if (over(y_dev, y_bytes) || overlaps(y_dev, y_bytes, x_dev, x_bytes) || overlaps(y_dev, y_bytes, residual_dev, all) || overlaps(y_dev, y_bytes, residual_out_dev, all) ||
+        over(residual_out_dev, all) || (!same_x && overlaps(residual_out_dev, all, x_dev, x_bytes)) || (residual_out_dev != residual_dev && overlaps(residual_out_dev, all, residual_dev, all)))
+        return fail(ctx, MPQ_ERR_INVALID_ARG, "outputs must not overlap, nor lie over an input (residual_out may be residual, or x)");
     const OnDevice on(ctx->device);
     CU_TRY(ctx, on.error);
     const NormParams p = {x_dev, residual_dev, residual_out_dev, post_weight_dev, gate_dev, weight_dev, y_dev, gate_stride, (int)H, alpha, eps};
@@ -136,6 +145,16 @@ extern "C" int32_t mpq_kv_append(mpq_context* ctx, const void* qkv_dev, int32_t 
     if (slots_dev && (!page_ok(page_size) || pages <= 0 || pages > MOST)) return fail(ctx, MPQ_ERR_SHAPE, "pages must be positive, page_size a power of two from 16 to 256 (%lld pages of %d)", (long long)pages, page_size);
     for (const void* ptr : {qkv_dev, (const void*)q_dev, (const void*)k_dev, (const void*)v_dev, (const void*)k_cache_dev, (const void*)v_cache_dev})
         if (!aligned16(ptr)) return fail(ctx, MPQ_ERR_ALIGN, "rows and caches must be 16-byte aligned");
+    // (CTAs have a token each, and go in no order)
+    const int64_t kv_bytes = tokens * kv_heads * head_dim * 2, cache_bytes = slots_dev ? pages * kv_heads * page_size * head_dim * 2 : 0;
+    const struct { const void* at; int64_t bytes; } outs[] = {{q_dev, tokens * q_heads * head_dim * 2}, {k_dev, kv_bytes}, {v_dev, kv_bytes}, {k_cache_dev, cache_bytes}, {v_cache_dev, cache_bytes}};
+    const int size = x_is_bf16 ? 2 : 4;
+    for (const auto& o : outs) {
+        bool over = overlaps(o.at, o.bytes, qkv_dev, tokens, (int64_t)(q_heads + 2 * kv_heads) * head_dim * size, (__int128)row_stride * size) || overlaps(o.at, o.bytes, slots_dev, tokens * 8) ||
+                    (rot_dim && (overlaps(o.at, o.bytes, positions_dev, tokens * 4) || overlaps(o.at, o.bytes, frequencies_dev, rot_dim * 4)));
+        for (const auto* other = &o + 1; other != outs + 5; ++other) over |= overlaps(o.at, o.bytes, other->at, other->bytes);
+        if (over) return fail(ctx, MPQ_ERR_INVALID_ARG, "outputs must not overlap, nor lie over an input");
+    }
     const OnDevice on(ctx->device);
     CU_TRY(ctx, on.error);
     auto bf = [](uint16_t* ptr) { return reinterpret_cast<__nv_bfloat16*>(ptr); };

@@ -109,3 +109,54 @@ def test_paged_attention_does_not_write_over_what_it_reads(ctx, max_new):
     out = words.view(torch.bfloat16).view(n, 4, D)
     _refused(ctx, lambda: m.paged_attention(ctx, q, k, v, starts, words[100:100 + n], table, max_new=max_new, out=out))
     _refused(ctx, lambda: m.paged_attention(ctx, q, k, v, words[200:200 + n + 1], lens, table, max_new=max_new, out=out))
+
+
+@pytest.mark.gpu
+def test_norms_do_not_write_over_what_others_read(ctx):
+    import makepad_b200 as m
+    import torch
+    M, H = 6, 64
+    f32 = torch.float32
+
+    def call(x, residual=None, residual_out=None, post=None, gate=None, stride=0, weight=None, y=None):
+        p = lambda t: None if t is None else t.data_ptr()
+        ctx.check(ctx.lib.mpq_residual_norm(ctx.h, p(x), x.dtype is torch.bfloat16, M, H, p(residual), p(residual_out), p(post), p(gate), stride, 0.5, p(weight), 1e-6,
+                                            p(y), y is not None and y.dtype is torch.bfloat16, torch.cuda.current_stream().cuda_stream))
+    x, r, w, gate = torch.randn(M, H, device="cuda"), torch.randn(M, H, device="cuda"), torch.randn(H, device="cuda"), torch.randn(M, 80, device="cuda")
+    y = torch.empty(M, H, device="cuda")
+    want_r, want_y = m.residual_norm(ctx, x, r, w, alpha=0.5, gate=gate[:, :H].contiguous())
+    for out in (r.clone(), x.clone(), torch.empty_like(r)):                   # in place of the residual, or of x, or neither
+        args = (out if torch.equal(out, x) else x, out if torch.equal(out, r) else r, out)
+        call(*args, gate=gate, stride=80, weight=w, y=y)
+        assert torch.equal(out, want_r) and torch.equal(y, want_y)
+    both = torch.randn(8192, device="cuda")                                 # (a gate of six rows 1000 apart lies in it)
+    at = lambda n, rows=M, wide=H: both[n:n + rows * wide].view(rows, wide)
+    half = lambda n: both[n:].view(torch.bfloat16)[:M * H].view(M, H)
+    for bad in (dict(x=at(0), y=at(0)), dict(x=at(0), y=at(M * H - 4)), dict(x=x, residual=at(0), y=at(64)), dict(x=x, residual_out=at(0), y=at(0)), dict(x=x, residual_out=at(0), y=half(M * H - 4)),
+                dict(x=at(64), residual_out=at(0)), dict(x=x, residual=at(64), residual_out=at(0)), dict(x=half(0), residual_out=at(0)), dict(x=x, residual_out=at(0), post=both[M * H - 4:M * H + 60]),
+                dict(x=x, residual_out=at(0), weight=both[:64]), dict(x=x, y=at(0), weight=both[M * H - 64:M * H]), dict(x=x, y=at(0), gate=both[60:], stride=0),
+                dict(x=x, y=at(80), gate=both, stride=400), dict(x=x, residual_out=at(80, 1), y=at(8 * 80), gate=at(0), stride=80)):
+        _refused(ctx, lambda: call(**bad))
+    call(x, y=at(80), gate=both, stride=1000)                                 # rows of the gate on either side: 0..63 and 1000..1063, y 80..463
+    torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_append_does_not_write_over_what_others_read(ctx):
+    import torch
+    T, D, pages, page = 5, 64, 2, 16
+    room = torch.zeros(1 << 16, dtype=torch.bfloat16, device="cuda")
+    at = lambda n: room[n:].data_ptr()
+    positions, slots = torch.arange(T, dtype=torch.int32, device="cuda"), torch.arange(T, dtype=torch.int64, device="cuda")
+    freq = torch.ones(D // 2, dtype=torch.float64, device="cuda")
+
+    def call(qkv=0, bf16=1, stride=256, pos=positions.data_ptr(), f=freq.data_ptr(), q=8192, k=None, v=None, s=slots.data_ptr(), kc=16384, vc=24576):
+        ctx.check(ctx.lib.mpq_kv_append(ctx.h, at(qkv), bf16, stride, T, 2, 1, D, pos, f, D, 0, at(q), None if k is None else at(k), None if v is None else at(v), s, at(kc), at(vc), pages, page,
+                                        torch.cuda.current_stream().cuda_stream))
+    call()
+    call(k=32768, v=40960)
+    call(stride=2048, q=256, k=2048 + 256, v=4096 + 256)                      # between the rows
+    for bad in (dict(q=0), dict(q=1272), dict(bf16=0, q=2552), dict(stride=2048, q=8192), dict(k=8192 + 632), dict(k=9000, v=9312), dict(kc=8192), dict(vc=16384), dict(vc=16384 + 2040), dict(kc=1000),
+                dict(pos=at(8192)), dict(f=at(16384)), dict(s=at(24576)), dict(s=at(8192 + 632)), dict(k=16384 + 2000), dict(v=24576 - 296)):
+        _refused(ctx, lambda: call(**bad))
+    torch.cuda.synchronize()
