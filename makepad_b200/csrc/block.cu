@@ -56,10 +56,11 @@ static cudaError_t norm_launch(const mpq_context* ctx, const NormParams& p, int6
 {
     // Groups of eight columns per thread, and CTAs on an SM.  Two groups: 8192 bf16 rows of 4096 columns, both norms and a gate, 72 us (one group, twice the warps at their
     // barriers, 76; four 71), 500 rows 6.4 (6.8; 7.8), fp32 rows of 8192 columns 199 (203; 214).  A row of more than 4096 bf16 columns with a norm behind the block has nothing on its
-    // way while its first sum is made: three such rows on an SM instead of two want four groups (8192 rows of 8192 columns 139, two groups 152, one 160), where there are so many
-    // rows (64: 5.1 and 4.8).
-    const int groups = p.H / 8;
-    const bool three = sizeof(X) == 2 && p.post_weight && groups > 512 && groups <= 1024 && M > ctx->prop.multiProcessorCount;
+    // way while its first sum is made: four groups put a third row on an SM where two groups put two, above 5120 columns, once each SM has two.  Two groups and four, us:
+    // 8192 rows of 8192 columns 151 / 138, 300 rows 9.0 / 7.9, 150 rows 6.0 / 7.4; of 5632 columns 116 / 96, 8.0 / 7.0, 4.7 / 6.4.  Up to 5120 columns three rows of two groups fit as
+    // well, and four groups pay only for many rows: 8192 rows of 5120 columns 93 / 89, 2000 rows 26.7 / 26.7, 700 rows 10.6 / 12.3, 300 rows 5.8 / 6.8.
+    const int groups = p.H / 8, sms = ctx->prop.multiProcessorCount;
+    const bool three = sizeof(X) == 2 && p.post_weight && groups > 512 && groups <= 1024 && M > (groups > 640 ? 2 : 16) * (int64_t)sms;
     const int nv = three || groups > 2048 ? 4 : 2;
     const unsigned threads = (unsigned)((groups + nv - 1) / nv + 31) / 32 * 32;
     auto kernel = groups <= 1024 ? residual_norm_kernel<512, 2, 2, X, Y> : groups <= 2048 ? residual_norm_kernel<1024, 1, 2, X, Y> : residual_norm_kernel<1024, 1, 4, X, Y>;

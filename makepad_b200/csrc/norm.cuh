@@ -5,8 +5,9 @@
 //   r' = r + alpha * gate * t                           gate: one value per column, or per element
 //   y  = r' / sqrt(mean(r'^2) + eps) * weight           what the next block reads
 //
-// A CTA has a row, a thread NV groups of eight columns, which stay in registers (x as it came) from the load to the last store: x and r are
-// read once, r' and y written once.  Sums of squares are fp32, in a fixed order.  Bound: HBM, (x + 4 + 4 + y) bytes per element: 8192 bf16 rows of 8192 columns, both norms,
+// A CTA has a row, a thread NV groups of eight columns, which stay in registers (x as it came) from the load to the last store (above 16384 columns 1024 threads
+// have 64 registers for four groups, and some 120 to 240 bytes of a thread go through local memory: 2048 bf16 rows of 32768 columns, both norms and a gate, 197 us, 4.1 TB/s; of
+// 16384 columns 91 us, 4.4): x and r are read once, r' and y written once.  Sums of squares are fp32, in a fixed order.  Bound: HBM, (x + 4 + 4 + y) bytes per element: 8192 bf16 rows of 8192 columns, both norms,
 // a gate 139 us (in place, 5.8 TB/s; 153 with other rows to write to); without the norm behind the block 119, 6.8 TB/s.  What is between is the first sum, during which a row has no traffic: rows on an SM count.  (CTAs that stay, the
 // next row's loads in registers and the weights in shared memory: 151; in a ring of bulk copies 174, of cp.async 197.)
 // The weights and a gate of one row are read by every CTA and come from L1 / L2.
