@@ -300,7 +300,9 @@ int32_t mpq_kv_append(mpq_context* ctx, const void* qkv_dev, int32_t x_is_bf16, 
  * them its new tokens (their k and v are in the cache already), new token j sees the first lens[i] - new + j + 1.  A row without keys is 0.
  * q bf16, rows of q_heads * head_dim (64 or 128) q_row_stride elements apart (a multiple of 8); query head h reads head
  * h / (q_heads / kv_heads).  out [tokens][q_heads][head_dim], bf16 or fp32; must not overlap an input.  max_new: the most new tokens of a request, as far as the caller knows
- * (0: not known); it chooses the kernel, not the result.  An entry of the table outside the cache reads as zeros; what lies behind
+ * (0: not known, taken for `tokens`).  It chooses the kernel, not the result (but for last bits), and so the time: up to 16 rows per head of keys (max_new * q_heads / kv_heads)
+ * go to the one that reads the cache once.  Said too small, the cache is read once for every 8 or 16 rows (2 x 1024 tokens over 16000, 64 heads on 8: 8.1 ms instead of 0.54); left out,
+ * single tokens go to the kernel of many rows (64 requests of 1000 to 8000: 270 us instead of 206).  A captured call keeps its choice.  An entry of the table outside the cache reads as zeros; what lies behind
  * lens[i] in the last page is not used, whatever it holds.  k and v of the new tokens are read by rows that do not see them:
  * they must be finite.  Sums are fp32, the weights of v are rounded to bf16.
  * scale must be finite and not negative.  n at most 2^20; tokens and max_blocks * page_size at most 2^30, tokens * q_heads / kv_heads below 2^31.  The pieces of units that CTAs share

@@ -185,7 +185,8 @@ impl PagedCache {
         })
     }
 
-    /// Attention of the step's rows q [tokens][q_heads][head_dim] (bf16), whose keys and values are in the cache; out fp32 or bf16.
+    /// Attention of the step's rows q [tokens][q_heads][head_dim] (bf16), whose keys and values are in the cache; out fp32 or bf16.  max_new: the most new tokens of
+    /// a request, 0 if not known; it chooses the kernel (see mpq_paged_attention).
     pub fn attend(&self, ctx: &Context, q: DevicePtr, q_heads: i32, step: &Step, max_new: i64, scale: f32, out: DevicePtr, out_is_f32: bool, stream: *mut c_void) -> Result<(), MpqError> {
         ctx.check(unsafe {
             (ctx.lib.mpq_paged_attention)(ctx.raw, q.0 as *const u16, q_heads as i64 * self.head_dim as i64, step.tokens, q_heads, self.k.0 as *const u16, self.v.0 as *const u16, self.pages,

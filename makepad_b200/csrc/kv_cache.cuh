@@ -72,7 +72,7 @@ __device__ __forceinline__ int plan_find(const int* at, int n, int v)
 
 __global__ void __launch_bounds__(PLAN_THREADS) kv_plan_kernel(const __grid_constant__ PlanParams p)
 {
-    extern __shared__ int s_req[];            // [4][n]: pages given in front, pages wanted in front, tokens in front, pages kept
+    extern __shared__ int s_req[];            // [5][n]: pages given in front, pages wanted in front, tokens in front, pages kept, tokens before the step
     __shared__ PlanSums s_warp[33];
     __shared__ int s_long;
     int *s_given = s_req, *s_need = s_req + p.n, *s_start = s_req + 2 * p.n, *s_kept = s_req + 3 * p.n, *s_before = s_req + 4 * p.n;
@@ -200,8 +200,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_plan_kernel(const __grid_cons
 // A pair (a, b) of a head becomes (a cos - b sin, b cos + a sin) with the angle position * frequency.  The angle is a product in 64
 // bits, reduced there to [-pi, pi] (in 32 bits position 100000 would be off by 0.004), sine and cosine are fp32.  One rounding, to bf16.
 //
-// A CTA has a token: 64 threads make its sines and cosines while all threads' rows are on their way.  An item is 16 elements of a head that
-// turn together: (8 + 8 a half apart, or 16 in a row).  Bound: HBM, (size of x + 2) bytes per element: 8000 bf16 rows of 80 heads of 128 55 us, 5.9 TB/s (the
+// A CTA has a token: 64 threads make its sines and cosines, and behind a barrier all of them load and turn its rows (the other CTAs on the SM have theirs on the way meanwhile).
+// An item is 16 elements of a head that turn together: (8 + 8 a half apart, or 16 in a row).  Bound: HBM, (size of x + 2) bytes per element: 8000 bf16 rows of 80 heads of 128 55 us, 5.9 TB/s (the
 // sines are a CTA's latency: with 8 warps instead of 4, and half as many tokens on an SM, 61; with 2 56; rows of 36 heads of 64 19.3, 24.1 and 17.7).
 struct AppendParams {
     const void* x;

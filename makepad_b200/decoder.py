@@ -77,7 +77,7 @@ class DecoderLayer:
 
         residual fp32 [T][H]; x [T][H]: the last layer's output (the embedding, with a residual of zeros), which this layer's first norm adds, behind
         a norm with the weights `post` (the last layer's ffn_post) if given.  With `step` and `cache` the tokens attend to their
-        requests' pages; else the T rows are whole prompts, packed at `starts` with their `positions`."""
+        requests' pages (max_new: the most new tokens of a request, 1 for a step of single tokens, 0 if not known; see paged_attention); else the T rows are whole prompts, packed at `starts` with their `positions`."""
         ctx, T, (qkv_scale, o_scale, gate_up_scale, down_scale) = self.ctx, residual.shape[0], self.activation_scales
         residual, y = residual_norm(ctx, x, residual, self.attn_norm, eps=self.eps, alpha=self.alpha, post_weight=post, out_dtype=self.dtype, inplace=True)
         qkv = self._project(self.qkv, y, qkv_scale)

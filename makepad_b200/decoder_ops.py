@@ -169,8 +169,9 @@ def paged_attention(ctx: Context, q, k_cache, v_cache, starts, lens, block_table
     """Attention of the new tokens q bf16 [T][q_heads][D] (D 64 or 128) over their requests' pages -> [T][q_heads][D], bf16 or fp32.
 
     starts int32 [n + 1], lens int32 [n] (with the new tokens, whose k and v are in the cache), block_table int32 [n][max_blocks]; scale:
-    D^-1/2 if None; max_new: the most new tokens of a request, if known (it chooses the kernel, not the result).  k and v of new tokens must be
-    finite, also for the rows that do not see them; what lies behind lens[i] may be anything."""
+    D^-1/2 if None; max_new: the most new tokens of a request, 0 if not known.  It chooses the kernel: 1 for a step of single tokens (left out, such a step
+    takes a third longer), max(new) or 0 where requests have more (said too small, every 8 or 16 rows read the cache again: up to 15 times the time).  k and v of new
+    tokens must be finite, also for the rows that do not see them; what lies behind lens[i] may be anything.  out must not overlap an input."""
     torch = _torch()
     qp, stride = _head_rows(ctx, "q", q)
     T, heads, D = q.shape
@@ -190,7 +191,8 @@ def paged_attention(ctx: Context, q, k_cache, v_cache, starts, lens, block_table
 
 def prompt_attention(ctx: Context, q, k, v, starts, *, scale: float = None, out_dtype=None, out=None):
     """Causal attention of whole prompts, packed: q bf16 [T][q_heads][D], k and v bf16 [T][kv_heads][D] (D 64 or 128; rows may be parts of
-    wider ones) -> [T][q_heads][D], bf16 or fp32.  starts int32 [n + 1].  v must be finite throughout a prompt."""
+    wider ones) -> [T][q_heads][D], bf16 or fp32.  starts int32 [n + 1].  v must be finite throughout a prompt.  out must not overlap an
+    input."""
     torch = _torch()
     (qp, qs), (kp, ks), (vp, vs) = _head_rows(ctx, "q", q), _head_rows(ctx, "k", k), _head_rows(ctx, "v", v)
     T, heads, D = q.shape
