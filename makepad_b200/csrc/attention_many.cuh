@@ -13,7 +13,9 @@
 // A prompt of 8192 tokens, 32 heads on 8 of 128: 551 GFLOP in 0.48 ms (1.14 PFLOP/s; 0.55 ms when it runs for seconds and the power is capped).  A unit's end takes
 // about 4000 cycles, a piece of a cut one 8000 more.
 //
-// The maximum that the weights stand against follows late: only when a row's own maximum is 2^8 above it is O scaled (read, multiplied, written
+// The running maximum and sum are the published one-pass softmax (Milakov and Gimelshein 2018); that the maximum may follow late, and that some of the exponentials are
+// better made by fused multiply-adds (rounding to a whole exponent and a polynomial for the rest, after Cody and Waite), is known of attention on this chip, too: neither is this library's
+// idea.  The maximum that the weights stand against follows late: only when a row's own maximum is 2^8 above it is O scaled (read, multiplied, written
 // back); until then the weights just grow, which costs neither bf16 nor fp32 any of their bits.
 //
 // ROLES, 20 warps: 0..15 softmax and epilogue (tile, half, quarter of the rows).  16 and 17 issue the MMAs, a tile each: one warp for both had its
